@@ -24,7 +24,7 @@ ADDER_ERR_WORKSPACE, ADDER_ERR_HIP, ADDER_ERR_ALIAS, ADDER_ERR_UNSUPPORTED = -4,
 MAX_ELEMENTS = 0x7fffffff   # of one tensor; entry points answer ADDER_ERR_TOO_LARGE above it
 
 _i, _l, _f, _p, _sz = ctypes.c_int, ctypes.c_long, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t
-_szp = ctypes.POINTER(ctypes.c_size_t)
+_szp, _d = ctypes.POINTER(ctypes.c_size_t), ctypes.c_double
 
 _SIGNATURES = {
     "adder_strerror": (ctypes.c_char_p, [_i]),
@@ -76,6 +76,17 @@ _SIGNATURES = {
     "adder_cross_entropy_fwd_f32": (_i, [_p, _p, _p, _p, _i, _i, _p]),
     "adder_cross_entropy_bwd_f32": (_i, [_p, _p, _p, _p, _p, _i, _i, _p]),
     "adder_sgd_momentum_step_f32": (_i, [_i, _p, _p, _p, _p, _p, _f, _f, _f, _p]),
+    "adder_linear_fwd_workspace_bytes": (_i, [_l, _i, _i, _i, _szp]),
+    "adder_linear_fwd": (_i, [_p, _l, _p, _p, _p, _l, _p, _p, _i, _l, _i, _i, _i, _p, _sz, _p]),
+    "adder_linear_bwd_workspace_bytes": (_i, [_l, _i, _i, _i, _i, _szp]),
+    "adder_linear_bwd": (_i, [_p, _l, _p, _p, _l, _p, _p, _p, _p, _i, _l, _i, _i, _i, _p, _sz, _p]),
+    "adder_layer_norm_fwd": (_i, [_p, _l, _p, _p, _p, _p, _p, _f, _l, _i, _i, _i, _p]),
+    "adder_layer_norm_bwd_workspace_bytes": (_i, [_l, _i, _i, _szp]),
+    "adder_layer_norm_bwd": (_i, [_p, _l, _p, _l, _p, _p, _p, _p, _p, _p, _l, _i, _i, _i, _p, _sz, _p]),
+    "adder_adamw_step": (_i, [_i] + [_p] * 6 + [_d] * 5 + [_l, _p, _i, _p]),
+    "adder_adamw_step_8bit": (_i, [_i] + [_p] * 8 + [_d] * 5 + [_l, _p, _i, _p]),
+    "adder_adamw_advance": (_i, [_p, _d, _d, _p, _p]),
+    "adder_state_values": (_i, [_p, _i, _p, _p, _l, _i, _p]),
 }
 for _name, (_res, _args) in _SIGNATURES.items():
     _fn = getattr(lib, _name)

@@ -1,0 +1,286 @@
+// The AdamW step for many tensors in one launch:
+//     m = b1 m + (1 - b1) g,   v = b2 v + (1 - b2) g^2,
+//     p = p (1 - lr weight_decay) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+// with the moments held as floats, or as 8-bit codes of blocks of kStateBlock values that share the largest magnitude among
+// them as their scale s:
+//     m = sign(q) s (q / 127)^2, q in -127 .. 127,      v = s (q / 255)^4, q in 0 .. 255.
+// The roots give small values more codes than a straight scale would (the second moment reaches down to 2e-10 of the block's
+// largest), and they need no table.  Codes go to the nearest; a second moment that is not zero keeps a code that is not zero,
+// since its root divides.  The parameter is updated with the moments before they are rounded.
+// Memory decides: 28 bytes a float parameter with moments of 32 bits, 16 with moments of 8.  The table of tensors travels by
+// value in the kernel arguments, as that of the SGD step does.
+#include "layers.hpp"
+
+namespace adder {
+
+// 1 / (1 - b1^t), 1 / sqrt(1 - b2^t): from the host, or from the device where the step count lives there
+struct Corrections { float c1, c2; };
+__device__ __forceinline__ Corrections corrections(const AdamWArgs &a) {
+    return a.corr ? Corrections{a.corr[0], a.corr[1]} : Corrections{a.c1, a.c2};
+}
+
+struct AdamWBatch {
+    void *p[kAdamWBatchMax];
+    const void *g[kAdamWBatchMax];
+    float *m[kAdamWBatchMax], *v[kAdamWBatchMax];
+    int n[kAdamWBatchMax];
+    int first_block[kAdamWBatchMax + 1];   // workgroups [first_block[t], first_block[t + 1]) belong to tensor t
+};
+struct AdamW8Batch {
+    void *p[kAdamW8BatchMax];
+    const void *g[kAdamW8BatchMax];
+    int8_t *m[kAdamW8BatchMax];
+    uint8_t *v[kAdamW8BatchMax];
+    float *ms[kAdamW8BatchMax], *vs[kAdamW8BatchMax];
+    int n[kAdamW8BatchMax];
+    int first_block[kAdamW8BatchMax + 1];
+};
+
+// the last tensor whose first workgroup is not behind this one
+template <class B>
+__device__ __forceinline__ int tensor_of(const B &b, int count) {
+    int lo = 0, hi = count - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (b.first_block[mid] <= (int)blockIdx.x) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ float adamw_value(float p, float g, float &m, float &v, const AdamWArgs &a, const Corrections &c,
+                                             float rate, float decay) {
+    m = fmaf(a.b1, m, a.one_b1 * g);
+    v = fmaf(a.b2, v, a.one_b2 * g * g);
+    return fmaf(-rate * c.c1, m / fmaf(sqrtf(v), c.c2, a.eps), p * decay);
+}
+
+static constexpr int kAdamWThreads = 256, kAdamWChunk = 4 * kAdamWThreads;
+
+// Up to four values at p, of which `left` exist
+template <class T>
+__device__ __forceinline__ void ld4(const T *p, int left, float (&v)[4]) {
+    if (left >= 4) {
+        ld_strip<4>(p, v);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = e < left ? ldf(p + e) : 0.f;
+    }
+}
+template <class T>
+__device__ __forceinline__ void st4(T *p, int left, const float (&v)[4]) {
+    if (left >= 4) {
+        put4(p, v);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+            if (e < left) put(p + e, v[e]);
+    }
+}
+typedef uint8_t u8x4_any __attribute__((ext_vector_type(4), aligned(1)));
+__device__ __forceinline__ uint32_t ld_codes(const void *p, int left) {
+    const uint8_t *q = static_cast<const uint8_t *>(p);
+    if (left >= 4) return __builtin_bit_cast(uint32_t, *reinterpret_cast<const u8x4_any *>(q));
+    uint32_t u = 0;
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+        if (e < left) u |= (uint32_t)q[e] << (8 * e);
+    return u;
+}
+__device__ __forceinline__ void st_codes(void *p, int left, uint32_t u) {
+    uint8_t *q = static_cast<uint8_t *>(p);
+    if (left >= 4) {
+        *reinterpret_cast<u8x4_any *>(q) = __builtin_bit_cast(u8x4_any, u);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+            if (e < left) q[e] = (uint8_t)(u >> (8 * e));
+    }
+}
+
+template <class T>
+__global__ __launch_bounds__(kAdamWThreads) void adamw_kernel(const AdamWBatch b, int count, const AdamWArgs a) {
+    const int t = tensor_of(b, count);
+    const int i = ((int)blockIdx.x - b.first_block[t]) * kAdamWChunk + (int)threadIdx.x * 4, left = b.n[t] - i;
+    if (left <= 0) return;
+    T *p = static_cast<T *>(b.p[t]) + i;
+    const T *g = static_cast<const T *>(b.g[t]) + i;
+    float *m = b.m[t] + i, *v = b.v[t] + i;
+    const Corrections c = corrections(a);
+    const float rate = a.lr_ptr ? *a.lr_ptr : a.lr, decay = a.lr_ptr ? 1.f - rate * a.weight_decay : a.decay;
+    float pv[4], gv[4], mv[4], vv[4];
+    ld4(p, left, pv);
+    ld4(g, left, gv);
+    ld4(m, left, mv);
+    ld4(v, left, vv);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) pv[e] = adamw_value(pv[e], gv[e], mv[e], vv[e], a, c, rate, decay);
+    st4(p, left, pv);
+    st4(m, left, mv);
+    st4(v, left, vv);
+}
+
+// Largest of the 64 lanes' values; not a number where one of them is none (or infinite).
+__device__ __forceinline__ float wave_scale(float v) {
+    const bool bad = !(v < __builtin_inff());
+    float t = v;
+    t = fmaxf(t, dpp_row_move<0xB1>(t));
+    t = fmaxf(t, dpp_row_move<0x4E>(t));
+    t = fmaxf(t, dpp_row_move<0x141>(t));
+    t = fmaxf(t, dpp_row_move<0x140>(t));
+    t = fmaxf(t, __shfl_xor(t, 16, 64));
+    t = fmaxf(t, __shfl_xor(t, 32, 64));
+    return __any(bad) ? __builtin_nanf("") : t;
+}
+
+// What divides by a scale: up * inv * value is value / scale, where 1 / scale on its own may be infinite.  A scale of zero, or
+// one that is not a number, gives codes of zero.
+struct Inverse { float up, inv; };
+__device__ __forceinline__ Inverse inverse(float scale) {
+    const float up = scale < 0x1p-64f ? 0x1p64f : 1.f;
+    const float s = scale * up;
+    return Inverse{up, s > 0.f ? 1.f / s : 0.f};
+}
+
+__device__ __forceinline__ float first_moment(int q, float s) {
+    const float r = (float)q;
+    return r * fabsf(r) * (1.f / (127.f * 127.f)) * s;   // (the square is exact)
+}
+__device__ __forceinline__ float second_moment(unsigned q, float s) {
+    const float r = (float)q, r2 = r * r;
+    return r2 * r2 * (1.f / (255.f * 255.f * 255.f * 255.f)) * s;
+}
+
+// A wave takes a block of the state at a time, four values a lane.
+template <class T>
+__global__ __launch_bounds__(kAdamWThreads) void adamw_8bit_kernel(const AdamW8Batch b, int count, const AdamWArgs a) {
+    static_assert(kStateBlock == 256, "four values a lane");
+    const int t = tensor_of(b, count), lane = threadIdx.x & 63;
+    const int block = ((int)blockIdx.x - b.first_block[t]) * (kAdamWThreads / 64) + (int)(threadIdx.x >> 6);
+    const int i = block * kStateBlock + lane * 4, left = b.n[t] - i;
+    if (b.n[t] - block * kStateBlock <= 0) return;   // (the whole wave)
+    T *p = static_cast<T *>(b.p[t]) + i;
+    const T *g = static_cast<const T *>(b.g[t]) + i;
+    const Corrections c = corrections(a);
+    const float rate = a.lr_ptr ? *a.lr_ptr : a.lr, decay = a.lr_ptr ? 1.f - rate * a.weight_decay : a.decay;
+    const float ms = b.ms[t][block], vs = b.vs[t][block];
+    float pv[4], gv[4], mv[4], vv[4];
+    ld4(p, left, pv);
+    ld4(g, left, gv);
+    uint32_t mq = ld_codes(b.m[t] + i, left), vq = ld_codes(b.v[t] + i, left);
+    float mtop = 0.f, vtop = 0.f;
+    bool bad_m = false, bad_v = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        mv[e] = first_moment((int8_t)(mq >> (8 * e)), ms);
+        vv[e] = second_moment((vq >> (8 * e)) & 255u, vs);
+        pv[e] = adamw_value(pv[e], gv[e], mv[e], vv[e], a, c, rate, decay);
+        if (e < left) {
+            mtop = fmaxf(mtop, fabsf(mv[e]));
+            vtop = fmaxf(vtop, vv[e]);
+            bad_m = bad_m || mv[e] != mv[e];   // (fmaxf passes over what is not a number)
+            bad_v = bad_v || vv[e] != vv[e];
+        }
+    }
+    st4(p, left, pv);
+    const float nan = __builtin_nanf("");
+    const float ns = wave_scale(bad_m ? nan : mtop), ws = wave_scale(bad_v ? nan : vtop);
+    const Inverse im = inverse(ns), iv = inverse(ws);
+    mq = vq = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float rm = rintf(127.f * sqrtf(fabsf(mv[e]) * im.up * im.inv));
+        const float rv = rintf(255.f * sqrtf(sqrtf(vv[e] * iv.up * iv.inv)));
+        const int qm = (int)fminf(rm, 127.f), qv = (int)fminf(fmaxf(rv, vv[e] > 0.f ? 1.f : 0.f), 255.f);
+        mq |= (uint32_t)((mv[e] < 0.f ? -qm : qm) & 255) << (8 * e);
+        vq |= (uint32_t)qv << (8 * e);
+    }
+    st_codes(b.m[t] + i, left, mq);
+    st_codes(b.v[t] + i, left, vq);
+    if (lane == 0) {
+        b.ms[t][block] = ns;
+        b.vs[t][block] = ws;
+    }
+}
+
+// step[0] += 1, and the corrections of the new count: for steps whose count lives on the device, so that a captured graph counts
+// on.  In 64 bits: 1 - b2^t is a difference of nearly equal numbers for the first steps.
+__global__ void adamw_advance_kernel(float *step, double ln_b1, double ln_b2, float *corr) {
+    const double t = (double)*step + 1.0;
+    *step = (float)t;
+    corr[0] = (float)(-1.0 / expm1(t * ln_b1));
+    corr[1] = (float)(1.0 / sqrt(-expm1(t * ln_b2)));
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void state_values_kernel(const void *codes, int is_signed, const float *__restrict__ scales,
+                                                           T *__restrict__ out, long n) {
+    const long i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
+    const int left = (int)(n - i < 4 ? n - i : 4);
+    if (left <= 0) return;
+    const uint32_t q = ld_codes(static_cast<const uint8_t *>(codes) + i, left);
+    const float s = scales[i / kStateBlock];
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const unsigned u = (q >> (8 * e)) & 255u;
+        v[e] = is_signed ? first_moment((int8_t)u, s) : second_moment(u, s);
+    }
+    st4(out + i, left, v);
+}
+
+template <class B, class F>
+static int fill_blocks(B &b, int count, const long *n, F more) {
+    int blocks = 0;
+    for (int t = 0; t < count; ++t) {
+        b.n[t] = (int)n[t];
+        b.first_block[t] = blocks;
+        blocks += (int)ceil_div_l(n[t], kAdamWChunk);
+        more(t);
+    }
+    b.first_block[count] = blocks;
+    return blocks;
+}
+
+template <class T>
+int launch_adamw(int count, void *const *p, const void *const *g, float *const *m, float *const *v, const long *n, const AdamWArgs &a,
+                 hipStream_t s) {
+    AdamWBatch b;
+    const int blocks = fill_blocks(b, count, n, [&](int t) {
+        b.p[t] = p[t]; b.g[t] = g[t]; b.m[t] = m[t]; b.v[t] = v[t];
+    });
+    hipLaunchKernelGGL(adamw_kernel<T>, dim3(blocks), dim3(kAdamWThreads), 0, s, b, count, a);
+    return check_launch();
+}
+
+template <class T>
+int launch_adamw_8bit(int count, void *const *p, const void *const *g, int8_t *const *m, uint8_t *const *v, float *const *ms,
+                      float *const *vs, const long *n, const AdamWArgs &a, hipStream_t s) {
+    AdamW8Batch b;
+    const int blocks = fill_blocks(b, count, n, [&](int t) {
+        b.p[t] = p[t]; b.g[t] = g[t]; b.m[t] = m[t]; b.v[t] = v[t]; b.ms[t] = ms[t]; b.vs[t] = vs[t];
+    });
+    hipLaunchKernelGGL(adamw_8bit_kernel<T>, dim3(blocks), dim3(kAdamWThreads), 0, s, b, count, a);
+    return check_launch();
+}
+
+int launch_adamw_advance(float *step, double ln_b1, double ln_b2, float *corr, hipStream_t s) {
+    hipLaunchKernelGGL(adamw_advance_kernel, dim3(1), dim3(1), 0, s, step, ln_b1, ln_b2, corr);
+    return check_launch();
+}
+
+template <class T>
+int launch_state_values(const void *codes, int is_signed, const float *scales, T *out, long n, hipStream_t s) {
+    hipLaunchKernelGGL(state_values_kernel<T>, dim3((unsigned)ceil_div_l(n, 1024)), dim3(256), 0, s, codes, is_signed, scales, out, n);
+    return check_launch();
+}
+
+#define ADDER_ADAMW_INSTANCE(T)                                                                                                      \
+    template int launch_adamw<T>(int, void *const *, const void *const *, float *const *, float *const *, const long *,             \
+                                 const AdamWArgs &, hipStream_t);                                                                   \
+    template int launch_adamw_8bit<T>(int, void *const *, const void *const *, int8_t *const *, uint8_t *const *, float *const *,   \
+                                      float *const *, const long *, const AdamWArgs &, hipStream_t);                                \
+    template int launch_state_values<T>(const void *, int, const float *, T *, long, hipStream_t);
+ADDER_ADAMW_INSTANCE(float)
+ADDER_ADAMW_INSTANCE(bf16_t)
+
+}  // namespace adder

@@ -1,6 +1,7 @@
 // C ABI of libaddernet_hip.so: argument validation and dispatch.  Every check
 // that can fail does so before the first HIP call, so the error paths can be
 // exercised on a machine without a GPU.
+#include "checks.hpp"
 #include "common.hpp"
 
 #include <atomic>
@@ -56,26 +57,6 @@ static int make_dims(int N, int Ci, int H, int W, int Co, int kh, int kw, int st
     const long nx = (long)N * Ci * H * W, ny = (long)N * Co * d.Ho * d.Wo, nw = (long)Co * Ci * kh * kw;
     if (nx > kMaxElems || ny > kMaxElems || nw > kMaxElems) return ADDER_ERR_TOO_LARGE;
     return ADDER_OK;
-}
-
-static bool overlaps(const void *a, size_t na, const void *b, size_t nb) {
-    if (!a || !b) return false;
-    const uintptr_t pa = reinterpret_cast<uintptr_t>(a), pb = reinterpret_cast<uintptr_t>(b);
-    return pa < pb + nb && pb < pa + na;
-}
-
-struct Span { const void *p; size_t bytes; };
-
-// no output may overlap an input or another output
-template <int NO, int NI>
-static bool any_alias(const Span (&outs)[NO], const Span (&ins)[NI]) {
-    for (int o = 0; o < NO; ++o) {
-        for (int i = 0; i < NI; ++i)
-            if (overlaps(outs[o].p, outs[o].bytes, ins[i].p, ins[i].bytes)) return true;
-        for (int q = o + 1; q < NO; ++q)
-            if (overlaps(outs[o].p, outs[o].bytes, outs[q].p, outs[q].bytes)) return true;
-    }
-    return false;
 }
 
 // The out_* half of adder_bn_links: out_x with exactly one of out_coef and out_part (+ what belongs to it).

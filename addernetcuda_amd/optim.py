@@ -7,6 +7,8 @@ fused update takes two launches of 15 us for them, csrc/sgd.hip one of 5 us.  Sa
 dampening, ``maximize``, no momentum, parameters that are not contiguous float32 GPU tensors, sparse gradients) is
 left to ``torch.optim.SGD.step``.  As with the framework's fused update, a float learning rate is frozen into a
 captured graph; pass the rate as a one-element float32 device tensor to change it between replays.
+
+``AdamW`` does the same for ``torch.optim.AdamW`` (csrc/adamw.hip), with its state in 32 or in 8 bits.
 """
 import ctypes
 
@@ -82,3 +84,228 @@ class SGD(torch.optim.SGD):
             finally:
                 self.param_groups = kept
         return loss
+
+
+_ADAMW_MAX, _ADAMW8_MAX, STATE_BLOCK = 96, 64, 256   # ADDER_ADAMW_BATCH_MAX, ADDER_ADAMW_8BIT_BATCH_MAX, ADDER_STATE_BLOCK
+_PIECE = 1 << 30                                     # values of one entry of the kernel's table; longer tensors take several
+_CODES = {"exp_avg": torch.int8, "exp_avg_sq": torch.uint8}
+
+
+def state_values(codes, scales, dtype=torch.float32):
+    """The values that an 8-bit moment of ``AdamW`` stands for: ``codes`` int8 (``exp_avg``) or uint8 (``exp_avg_sq``), ``scales`` one float32
+    per ``STATE_BLOCK`` codes; a float32 or bfloat16 tensor shaped like ``codes``."""
+    if codes.dtype not in (torch.int8, torch.uint8):
+        raise RuntimeError(f"codes must be int8 or uint8, got {codes.dtype}")
+    if dtype not in _ADAMW_TYPES:
+        raise RuntimeError(f"dtype must be float32 or bfloat16, got {dtype}")
+    if not (codes.is_cuda and scales.device == codes.device):
+        raise RuntimeError("codes and scales must be CUDA tensors on one device")
+    n = codes.numel()
+    if scales.dtype != torch.float32 or scales.numel() != -(-n // STATE_BLOCK):
+        raise RuntimeError(f"scales must be {-(-n // STATE_BLOCK)} float32 values, got {scales.numel()} of {scales.dtype}")
+    codes, scales = codes.contiguous(), scales.contiguous()
+    out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
+    if n:
+        with on_device(codes.device):
+            check(lib.adder_state_values(codes.data_ptr(), int(codes.dtype == torch.int8), scales.data_ptr(), out.data_ptr(), n,
+                                         _ADAMW_TYPES[dtype], stream_ptr(codes.device)), "adder_state_values")
+    return out
+
+
+_ADAMW_TYPES = {torch.float32: 0, torch.bfloat16: 1}   # adder_type
+
+
+class AdamW(torch.optim.AdamW):
+    """``torch.optim.AdamW`` with the update of all parameters of a group in one launch (csrc/adamw.hip; up to 96 tensors, or 64 with
+    8-bit state), and its two moments in 32 bits or, with ``state_bits=8``, as 8-bit codes: 16 instead of 28 bytes of memory traffic a
+    float32 parameter and 2 instead of 8 bytes of memory.
+
+    Parameters: float32 or bfloat16, with gradients of their type.  With ``state_bits=32`` the state is that of ``torch.optim.AdamW``
+    (float32 ``exp_avg``, ``exp_avg_sq`` whatever the parameter's type; ``step``), and what the kernel does not cover (``amsgrad``,
+    ``maximize``, CPU or non-contiguous tensors, other types, sparse gradients) is left to ``torch.optim.AdamW.step``.  With
+    ``state_bits=8`` tensors of at least ``min_8bit_size`` values hold ``exp_avg`` (int8) and ``exp_avg_sq`` (uint8) with float32
+    ``exp_avg_scale`` and ``exp_avg_sq_scale``, one per ``STATE_BLOCK`` values (``state_values`` decodes them); smaller ones, whose state costs
+    nothing, keep 32 bits, and what the kernel does not cover is an error.
+
+    ``capturable=True`` keeps the step count on the device, so that a captured HIP graph counts on; the learning rate may then be a
+    one-element float32 device tensor."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, amsgrad=False, *, maximize=False,
+                 capturable=False, state_bits=32, min_8bit_size=4096):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits!r}")
+        if state_bits == 8 and (amsgrad or maximize):
+            raise ValueError("state_bits=8 takes neither amsgrad nor maximize")
+        super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, amsgrad=amsgrad, maximize=maximize,
+                         foreach=False, fused=False, capturable=capturable)
+        self.state_bits, self.min_8bit_size = state_bits, min_8bit_size
+
+    @staticmethod
+    def _kernel_takes(group, params, grads):
+        if group["amsgrad"] or group["maximize"]:
+            return False
+        lr = group["lr"]
+        if isinstance(lr, torch.Tensor) and not (lr.is_cuda and lr.dtype == torch.float32 and lr.numel() == 1):
+            return False
+        if any(isinstance(b, torch.Tensor) for b in group["betas"]):
+            return False
+        both = params + grads
+        types = list(map(_dtype, params))
+        return (set(map(_layout, both)) == {torch.strided} and set(map(_device, both)) == {params[0].device} and params[0].is_cuda
+                and set(types) <= _ADAMW_TYPES.keys() and types == list(map(_dtype, grads)) and all(map(_contiguous, both))
+                and list(map(_numel, params)) == list(map(_numel, grads)))
+
+    def _new_state(self, p, step):
+        state = self.state[p]
+        state["step"] = step
+        if self.state_bits == 8 and p.numel() >= self.min_8bit_size:
+            blocks = -(-p.numel() // STATE_BLOCK)
+            for name, dtype in _CODES.items():
+                state[name] = torch.zeros(p.shape, dtype=dtype, device=p.device)
+                state[name + "_scale"] = torch.zeros(blocks, dtype=torch.float32, device=p.device)
+        else:
+            for name in _CODES:
+                state[name] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+        return state
+
+    def load_state_dict(self, state_dict):
+        """As ``torch.optim.Optimizer.load_state_dict``, but 8-bit moments stay codes, and the others become float32."""
+        super().load_state_dict(state_dict)
+        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
+        own = [p for g in self.param_groups for p in g["params"]]
+        for i, p in zip(saved, own):
+            for name, value in state_dict["state"].get(i, {}).items():
+                if isinstance(value, torch.Tensor) and name != "step":
+                    coded = value.dtype in (torch.int8, torch.uint8)
+                    self.state[p][name] = value.to(device=p.device, dtype=value.dtype if coded else torch.float32, copy=True)
+        for group in self.param_groups:   # parameters of one count share its tensor again (see _kernel_step)
+            if group["capturable"]:
+                shared = {}
+                for p in group["params"]:
+                    if self.state.get(p):
+                        step = float(self.state[p]["step"])
+                        if step not in shared:
+                            shared[step] = torch.tensor(step, dtype=torch.float32, device=p.device)
+                        self.state[p]["step"] = shared[step]
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        rest = []
+        for group in self.param_groups:
+            params = [p for p in group["params"] if p.grad is not None]
+            if not params:
+                continue
+            grads = [p.grad for p in params]
+            if self._kernel_takes(group, params, grads):
+                self._kernel_step(group, params, grads)
+            elif self.state_bits == 8:
+                raise RuntimeError("state_bits=8 needs contiguous float32 or bfloat16 GPU parameters with gradients of their type, on one device")
+            else:
+                rest.append(group)
+        if rest:   # the groups the kernel does not take: the framework's own update, group by group
+            for group in rest:
+                for p in group["params"]:
+                    state = self.state.get(p)
+                    if state:   # (a tensor of its own for each: the framework counts them one by one)
+                        step = state["step"]
+                        state["step"] = (step.clone() if isinstance(step, torch.Tensor) else
+                                         torch.tensor(float(step), device=p.device if group["capturable"] else "cpu"))
+            kept = self.param_groups
+            try:
+                self.param_groups = rest
+                super().step()
+            finally:
+                self.param_groups = kept
+        return loss
+
+    def _counted(self, group, params):
+        """The states of ``params`` with their step counts as the kernel wants them: an int or, with ``capturable``, a tensor on the
+        device that the parameters of one count share (one tiny launch counts them all)."""
+        of, capturable = self.state, group["capturable"]
+        states = [of[p] for p in params]
+        if not all(states):
+            fresh = torch.zeros((), dtype=torch.float32, device=params[0].device) if capturable else 0
+            states = [state or self._new_state(p, fresh) for p, state in zip(params, states)]
+        if capturable:
+            for state in states:
+                if not (isinstance(state["step"], torch.Tensor) and state["step"].is_cuda and state["step"].dtype == torch.float32):
+                    state["step"] = torch.tensor(float(state["step"]), dtype=torch.float32, device=params[0].device)
+            if len(params) < len(group["params"]):   # parameters without a gradient now do not count on with the others
+                used = {id(state["step"]) for state in states}
+                for p in group["params"]:
+                    if p.grad is None and of.get(p) and id(of[p]["step"]) in used:
+                        of[p]["step"] = of[p]["step"].clone()
+        else:
+            for state in states:
+                if type(state["step"]) is not int:
+                    state["step"] = int(state["step"])
+        return states
+
+    def _kernel_step(self, group, params, grads):
+        capturable, dev = group["capturable"], params[0].device
+        states = self._counted(group, params)
+        batches = {}   # one launch per step count and storage type of the parameter and of its state: almost always one
+        for p, g, state in zip(params, grads, states):
+            step, m = state["step"], state["exp_avg"]
+            if m.dtype not in _STATE_TYPES:   # what torch.optim.AdamW made for a group that it had to take before
+                for name in _CODES:
+                    state[name] = state[name].float()
+                m = state["exp_avg"]
+            batches.setdefault((id(step) if capturable else step, p.dtype, m.dtype), []).append((p, g, state))
+        lr = group["lr"]
+        lr_ptr, lr_val = (lr.data_ptr(), 0.0) if isinstance(lr, torch.Tensor) else (None, float(lr))
+        b1, b2 = group["betas"]
+        with on_device(dev):
+            stream = stream_ptr(dev)
+            advanced = {}
+            for (_, dtype, kept), batch in batches.items():
+                corr, count, step = None, 0, batch[0][2]["step"]
+                if capturable:
+                    if id(step) not in advanced:
+                        corr = advanced[id(step)] = torch.empty(2, dtype=torch.float32, device=dev)
+                        check(lib.adder_adamw_advance(step.data_ptr(), b1, b2, corr.data_ptr(), stream), "adder_adamw_advance")
+                    corr = advanced[id(step)].data_ptr()
+                else:
+                    count = step + 1
+                _adamw_launches(batch, kept == torch.int8,
+                                (lr_ptr, lr_val, b1, b2, group["eps"], group["weight_decay"], count, corr, _ADAMW_TYPES[dtype], stream))
+                if not capturable:
+                    for _, _, state in batch:
+                        state["step"] = count
+
+
+_dtype, _device, _layout = torch.Tensor.dtype.__get__, torch.Tensor.device.__get__, torch.Tensor.layout.__get__
+_numel, _contiguous, _data_ptr = torch.Tensor.numel, torch.Tensor.is_contiguous, torch.Tensor.data_ptr
+_STATE_TYPES = (torch.float32, torch.int8)
+
+
+def _adamw_launches(batch, coded, tail):
+    params, grads, states = zip(*batch)
+    call, most, what = ((lib.adder_adamw_step_8bit, _ADAMW8_MAX, "adder_adamw_step_8bit") if coded
+                        else (lib.adder_adamw_step, _ADAMW_MAX, "adder_adamw_step"))
+    sizes = list(map(_numel, params))
+    moments = [[state["exp_avg"] for state in states], [state["exp_avg_sq"] for state in states]]
+    fits, types = [sizes, sizes], list(_CODES.values()) if coded else [torch.float32, torch.float32]
+    if coded:
+        moments += [[state["exp_avg_scale"] for state in states], [state["exp_avg_sq_scale"] for state in states]]
+        fits += [[-(-n // STATE_BLOCK) for n in sizes]] * 2
+        types += [torch.float32, torch.float32]
+    for tensors, fit, dtype in zip(moments, fits, types):   # (a state that was set by hand, or a parameter that was replaced)
+        if not (list(map(_numel, tensors)) == fit and set(map(_dtype, tensors)) == {dtype} and all(map(_contiguous, tensors))
+                and set(map(_device, tensors)) == {params[0].device}):
+            raise RuntimeError(f"{what}: the state does not fit its parameter")
+    columns = [list(map(_data_ptr, c)) for c in (params, grads, *moments)]
+    if min(sizes) == 0 or max(sizes) > _PIECE:   # empty tensors have no entry, long ones several
+        e = params[0].element_size()
+        widths = [e, e, 1, 1, 4 / STATE_BLOCK, 4 / STATE_BLOCK] if coded else [e, e, 4, 4]
+        cut = [(t, at) for t, n in enumerate(sizes) for at in range(0, n, _PIECE)]
+        columns = [[c[t] + int(at * w) for t, at in cut] for c, w in zip(columns, widths)]
+        sizes = [min(_PIECE, sizes[t] - at) for t, at in cut]
+    for i in range(0, len(sizes), most):
+        k = min(most, len(sizes) - i)
+        pointers, longs = ctypes.c_void_p * k, ctypes.c_long * k
+        check(call(k, *[pointers(*c[i:i + k]) for c in columns], longs(*sizes[i:i + k]), *tail), what)

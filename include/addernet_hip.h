@@ -30,6 +30,8 @@
  *   [optional]  the classifier head of the ResNets: average pool, matrix product, BatchNorm (adder_head_*)
  *   [optional]  the cross-entropy loss in one launch each way (adder_cross_entropy_*)
  *   [optional]  the momentum-SGD update of all parameters in one launch (adder_sgd_momentum_step_f32)
+ *   [layers]    what networks put beside adder layers, in float32 and bfloat16: linear layers (adder_linear_*), layer
+ *               normalisation (adder_layer_norm_*), the AdamW update (adder_adamw_*)
  */
 #ifndef ADDERNET_HIP_H
 #define ADDERNET_HIP_H
@@ -482,6 +484,78 @@ ADDER_API int adder_cross_entropy_bwd_f32(const float *logits, const long long *
 ADDER_API int adder_sgd_momentum_step_f32(int count, float *const *params, const float *const *grads,
                                           float *const *momentum_bufs, const long *n, const float *lr_device,
                                           float lr, float momentum, float weight_decay, void *stream);
+
+/* ------------------------------------------------------------------------
+ * [layers] Layers beside the adder layers.  No counterpart in the reference, which leaves its Linear layers (vgg.py) and its
+ * optimizer to the framework.
+ * `type` says how the tensors given as void * are stored; sums, statistics and moments are 32 bits in either.  Matrices are
+ * rows of neighbouring values; a row stride (in values) is 0, or at least the row's width.  Any alignment.  Tensors may have
+ * more than 2^31 - 1 elements.  Nothing depends on the order in which workgroups run: the same bits every time.
+ * ---------------------------------------------------------------------- */
+typedef enum adder_type { ADDER_TYPE_F32 = 0, ADDER_TYPE_BF16 = 1 } adder_type;
+
+/* Linear layer: z = x w' + bias, y = act(z) + residual; x (rows, in_features), w (out_features, in_features) dense,
+ * bias (out_features), residual and y (rows, out_features).
+ *   act: none, relu, gelu (z Phi(z), by the error function) or silu (z / (1 + exp(-z))).
+ *   adder_linear_fwd: bias and residual nullable.  pre (nullable): receives z (rows, out_features), which the backward of every
+ *     act but none needs.
+ *   adder_linear_bwd: dz = dy act'(pre); gx = dz w, gw = dz' x, gbias = sum over rows of dz; each of the three nullable.  The
+ *     residual's gradient is dy.  pre is not read where act is none; x only for gw, w only for gx.  bfloat16: dz is rounded
+ *     to bfloat16 for the two products (the matrix cores' operands), and not for gbias.
+ * Workspaces: the sizes that the queries give (0: none is needed), 256-byte aligned. */
+typedef enum adder_act { ADDER_ACT_NONE = 0, ADDER_ACT_RELU = 1, ADDER_ACT_GELU = 2, ADDER_ACT_SILU = 3 } adder_act;
+ADDER_API int adder_linear_fwd_workspace_bytes(long rows, int in_features, int out_features, int type, size_t *bytes);
+ADDER_API int adder_linear_fwd(const void *x, long x_row_stride, const void *w, const void *bias, const void *residual,
+                               long residual_row_stride, void *y, void *pre, int act, long rows, int in_features,
+                               int out_features, int type, void *ws, size_t ws_bytes, void *stream);
+ADDER_API int adder_linear_bwd_workspace_bytes(long rows, int in_features, int out_features, int act, int type, size_t *bytes);
+ADDER_API int adder_linear_bwd(const void *dy, long dy_row_stride, const void *pre, const void *x, long x_row_stride,
+                               const void *w, void *gx, void *gw, void *gbias, int act, long rows, int in_features,
+                               int out_features, int type, void *ws, size_t ws_bytes, void *stream);
+
+/* Layer normalisation of rows of `width` values: y = (x - mean) rstd weight + bias, rstd = 1 / sqrt(variance + eps) with the
+ * biased variance; weight and bias (width) nullable and stored as weight_type says (type, or float32 beside bfloat16 rows).
+ *   adder_layer_norm_fwd: save_mean, save_rstd (rows): both or neither; the backward needs them.
+ *   adder_layer_norm_bwd: gx (rows, width), gweight, gbias (width, weight_type): each nullable.  The workspace is needed for
+ *     gweight and gbias. */
+ADDER_API int adder_layer_norm_fwd(const void *x, long x_row_stride, const void *weight, const void *bias, void *y,
+                                   float *save_mean, float *save_rstd, float eps, long rows, int width, int type,
+                                   int weight_type, void *stream);
+ADDER_API int adder_layer_norm_bwd_workspace_bytes(long rows, int width, int type, size_t *bytes);
+ADDER_API int adder_layer_norm_bwd(const void *dy, long dy_row_stride, const void *x, long x_row_stride, const void *weight,
+                                   const float *save_mean, const float *save_rstd, void *gx, void *gweight, void *gbias,
+                                   long rows, int width, int type, int weight_type, void *ws, size_t ws_bytes, void *stream);
+
+/* The AdamW update of `count` tensors in one launch:
+ *     m = beta1 m + (1 - beta1) g,   v = beta2 v + (1 - beta2) g^2,
+ *     p = p (1 - lr weight_decay) - lr / (1 - beta1^step) m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
+ * params, grads (stored as `type` says), moments and n are host arrays of `count` device pointers / element counts (at most
+ * 2^31 - 1 each).  step: the count of this step, from 1 on.  lr_device (nullable): the rate as one float in device memory.
+ * corrections_device (nullable): the two numbers that adder_adamw_advance left, instead of step; both for callers that capture
+ * the step in a HIP graph.
+ *   adder_adamw_step: moments as floats, count <= ADDER_ADAMW_BATCH_MAX.
+ *   adder_adamw_step_8bit: moments as 8-bit codes, count <= ADDER_ADAMW_8BIT_BATCH_MAX.  ADDER_STATE_BLOCK neighbouring values
+ *     share a scale s, the largest magnitude among them: m = sign(q) s (q / 127)^2 with q in -127 .. 127 (signed char),
+ *     v = s (q / 255)^4 with q in 0 .. 255 (unsigned char), to the nearest in that root's scale; a second moment that is not
+ *     zero keeps a code that is not.  The parameter is updated with the moments before they are rounded.  A block with a
+ *     moment that is infinite or not a number becomes not a number as a whole.  Scales: ceil(n / ADDER_STATE_BLOCK) floats.
+ *   adder_adamw_advance: step_device[0] += 1, and corrections[0], [1] = 1 / (1 - beta1^step), 1 / sqrt(1 - beta2^step).
+ *   adder_state_values: the values that n codes (signed: of a first moment) and their scales stand for. */
+#define ADDER_ADAMW_BATCH_MAX 96
+#define ADDER_ADAMW_8BIT_BATCH_MAX 64
+#define ADDER_STATE_BLOCK 256
+ADDER_API int adder_adamw_step(int count, void *const *params, const void *const *grads, float *const *exp_avgs,
+                               float *const *exp_avg_sqs, const long *n, const float *lr_device, double lr, double beta1,
+                               double beta2, double eps, double weight_decay, long step, const float *corrections_device,
+                               int type, void *stream);
+ADDER_API int adder_adamw_step_8bit(int count, void *const *params, const void *const *grads, signed char *const *exp_avgs,
+                                    unsigned char *const *exp_avg_sqs, float *const *exp_avg_scales,
+                                    float *const *exp_avg_sq_scales, const long *n, const float *lr_device, double lr,
+                                    double beta1, double beta2, double eps, double weight_decay, long step,
+                                    const float *corrections_device, int type, void *stream);
+ADDER_API int adder_adamw_advance(float *step_device, double beta1, double beta2, float *corrections, void *stream);
+ADDER_API int adder_state_values(const void *codes, int is_signed, const float *scales, void *values, long n, int type,
+                                 void *stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,213 @@
+"""``addernetcuda_amd.linear`` against the formula in 64 bits: every type, activation, layout and size where the kernels can go wrong,
+with bounds that follow from the roundings (tests/layer_bounds.py)."""
+import pytest
+import torch
+
+from tests import layer_bounds as B
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.float32, torch.bfloat16]
+ACTS = ["none", "relu", "gelu", "silu"]
+
+
+def make(rows, k, n, dtype, seed=0, bias=True, residual=True):
+    g = torch.Generator().manual_seed(seed + 31 * rows + 7 * k + n)
+    t = lambda *s, scale=1.0: (torch.randn(*s, generator=g) * scale).to(dtype).cuda()
+    return (t(rows, k), t(n, k, scale=k ** -0.5), t(n, scale=0.3) if bias else None, t(rows, n) if residual else None, t(rows, n))
+
+
+def check(rows, k, n, dtype, act, seed=0, bias=True, residual=True):
+    from addernetcuda_amd.linear import linear_act
+    x, w, b, r, dy = make(rows, k, n, dtype, seed, bias, residual)
+    want = B.linear(x, w, b, r, dy, act)
+    with torch.no_grad():
+        B.within(linear_act(x, w, b, r, act), want["y"], "y without gradients")
+    leaves = [t.requires_grad_(True) for t in (x, w, b, r) if t is not None]
+    y = linear_act(x, w, b, r, act)
+    B.within(y, want["y"], "y")
+    got = torch.autograd.grad(y, leaves, dy)
+    names = ["gx", "gw"] + (["gb"] if bias else [])
+    for name, t in zip(names, got):
+        assert t.dtype == dtype
+        B.within(t, want[name], name)
+    if residual:
+        assert torch.equal(got[-1], dy)
+
+
+# one row up to many, widths below, at and beside the tiles' and chunks' sides, products that are split over k and that are not
+SIZES = [(1, 1, 1), (1, 8, 8), (1, 64, 16), (2, 7, 5), (3, 65, 33), (1, 4096, 256), (5, 1000, 130), (16, 512, 512), (17, 129, 100),
+         (33, 96, 1), (64, 64, 64), (65, 72, 80), (100, 1, 70), (128, 512, 512), (129, 520, 264), (130, 63, 257), (200, 2048, 40),
+         (256, 128, 384), (300, 515, 127), (512, 256, 256), (1031, 33, 129), (2000, 264, 520), (4099, 40, 24)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows,k,n", SIZES)
+def test_sizes(rows, k, n, dtype, gpu):
+    check(rows, k, n, dtype, ACTS[(rows + k + n) % 4])
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("bias,residual", [(False, False), (True, False), (False, True)])
+def test_epilogues(act, bias, residual, dtype, gpu):
+    check(37, 130, 75, dtype, act, bias=bias, residual=residual)
+    check(2, 264, 72, dtype, act, bias=bias, residual=residual)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+def test_large(dtype, gpu):
+    check(1024, 1024, 2048, dtype, "gelu", residual=False)
+    check(2500, 1032, 1000, dtype, "silu")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows,k,n", [(3, 40, 24), (130, 72, 136), (300, 100, 50)])
+def test_layouts(rows, k, n, dtype, gpu):
+    """Rows with gaps that hold NaN, bases off any alignment, transposed inputs, leading dimensions, expanded gradients and residuals."""
+    from addernetcuda_amd.linear import linear_act
+    x, w, b, r, dy = make(rows, k, n, dtype)
+    nan = float("nan")
+
+    def gap(t, more=5):   # the same values in rows that are `more` longer, one element off the allocation's start
+        big = torch.full((t.shape[0] * (t.shape[1] + more) + 1,), nan, dtype=dtype, device="cuda")
+        v = big[1:].view(t.shape[0], t.shape[1] + more)[:, :t.shape[1]]
+        v.copy_(t)
+        return v
+
+    want = B.linear(x, w, b, r, dy, "gelu")
+    across = lambda t: t.t().contiguous().t()
+    for lay_x, lay_r, lay_dy, lay_w in [(gap, gap, gap, gap), (across, across, across, across), (gap, across, gap, across)]:
+        leaves = [lay_x(x).detach().requires_grad_(True), lay_w(w).detach().requires_grad_(True), gap(b[None])[0].detach().requires_grad_(True)]
+        y = linear_act(leaves[0], leaves[1], leaves[2], lay_r(r), "gelu")
+        B.within(y, want["y"], "y")
+        for name, t in zip(("gx", "gw", "gb"), torch.autograd.grad(y, leaves, lay_dy(dy))):
+            B.within(t, want[name], name)
+    # three leading dimensions, a residual that is broadcast, a gradient that is one number expanded
+    xs = x[: rows // 3 * 3].view(3, rows // 3, k).requires_grad_(True)
+    row = r[0].clone().requires_grad_(True)
+    y = linear_act(xs, w, b, row, "silu")
+    assert y.shape == (3, rows // 3, n)
+    used = rows // 3 * 3
+    want = B.linear(xs.detach().view(used, k), w, b, row.detach().expand(used, n), torch.ones(used, n, dtype=dtype), "silu")
+    B.within(y.view(used, n), want["y"], "y")
+    gx, gr = torch.autograd.grad(y.sum(), (xs, row))
+    B.within(gx.view(used, k), want["gx"], "gx")
+    assert torch.equal(gr, torch.full_like(row, used))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+def test_rows_that_do_not_exist_and_single_gradients(dtype, gpu):
+    from addernetcuda_amd.linear import linear_act, LinearAct
+    x, w, b, _, _ = make(4, 24, 16, dtype)
+    none = x[:0].requires_grad_(True)
+    for t in (w, b):
+        t.requires_grad_(True)
+    y = linear_act(none, w, b, act="relu")
+    assert y.shape == (0, 16)
+    gx, gw, gb = torch.autograd.grad(y.sum(), (none, w, b))
+    assert gx.shape == (0, 24) and not gw.any() and not gb.any()
+    dy = torch.randn(4, 16, device="cuda").to(dtype)
+    want = B.linear(x, w, b, None, dy, "gelu")
+    for name, leaf in (("gw", w), ("gb", b)):
+        y = linear_act(x, w, b, act="gelu")
+        B.within(torch.autograd.grad(y, leaf, dy)[0], want[name], name)
+    xr = x.clone().requires_grad_(True)
+    y = linear_act(xr, w.detach(), None, act="gelu")
+    B.within(torch.autograd.grad(y, xr, dy)[0], B.linear(x, w, None, None, dy, "gelu")["gx"], "gx alone")
+    layer = LinearAct(24, 16, act="silu").cuda()   # float32 parameters; their gradients come back float32
+    y = layer(x, residual=dy)
+    y.float().square().sum().backward()
+    assert layer.weight.grad.dtype == torch.float32 and layer.bias.grad.dtype == torch.float32
+    ref = torch.nn.Linear(24, 16)
+    ref.load_state_dict(layer.state_dict())   # the same names
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows,k,n", [(3, 72, 40), (70, 130, 65), (300, 264, 264)])
+def test_infinite_and_nan_stay_where_they_are(rows, k, n, dtype, gpu):
+    """An infinite or not-a-number input reaches its own row only, and as the formula has it; so does one in the weights its column."""
+    from addernetcuda_amd.linear import linear_act
+    x, w, b, r, _ = make(rows, k, n, dtype)
+    x, w = x.abs() + 0.5, w.abs() + 0.01
+    clean = linear_act(x, w, b, r)
+    x[1, k - 1] = float("inf")
+    x[2, 0] = float("nan")
+    w[3, k // 2] = float("-inf")
+    y = linear_act(x, w, b, r).float()
+    assert torch.isnan(y[2]).all() and torch.isnan(y[1, 3])
+    keep = torch.ones(n, dtype=torch.bool, device="cuda")
+    keep[3] = False
+    assert (y[1][keep] == float("inf")).all()
+    rest = [i for i in range(rows) if i not in (1, 2)]
+    assert (y[rest][:, 3] == float("-inf")).all()
+    assert torch.equal(y[rest][:, keep], clean.float()[rest][:, keep])
+
+
+def test_gradients_against_differences(gpu):
+    """f(t + e d) - f(t - e d) = 2 e |grad f|^2 / |grad f| along d = grad f / |grad f|; float32 sums of 2^15 outputs carry 1e-5 of
+    their size at most, the step's third-order term less."""
+    from addernetcuda_amd.linear import linear_act
+    x, w, b, r, dy = (t.requires_grad_(True) for t in make(128, 96, 256, torch.float32))
+    f = lambda *t: (linear_act(*t, act="gelu").double() * dy.double()).sum().item()
+    args = [x, w, b, r]
+    grads = torch.autograd.grad(linear_act(*args, act="gelu"), args, dy)
+    with torch.no_grad():
+        for i, g in enumerate(grads):
+            size = g.norm().item()
+            d = g / size
+            e = 0.02 * args[i].norm().item() / args[i].numel() ** 0.5
+            up, down = ([a + s * e * d if j == i else a for j, a in enumerate(args)] for s in (1, -1))
+            assert abs((f(*up) - f(*down)) / (2 * e) - size) <= 5e-3 * size
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows,k,n", [(4, 512, 512), (128, 1024, 128), (1500, 264, 264)])
+def test_same_bits_every_time_and_on_other_streams(rows, k, n, dtype, gpu):
+    from addernetcuda_amd.linear import linear_act
+    x, w, b, r, dy = make(rows, k, n, dtype)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+
+    def once():
+        y = linear_act(x, w, b, r, "gelu")
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+
+    first = once()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        second = once()
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b_ in zip(first, second):
+        assert torch.equal(a, b_)
+
+
+def test_more_than_two_to_the_31_values(gpu):
+    from addernetcuda_amd.linear import linear_act
+    rows, k, n = (1 << 22) + 3, 520, 8
+    _, w, b, _, _ = make(1, k, n, torch.bfloat16)
+    x = torch.zeros(rows, k, dtype=torch.bfloat16, device="cuda")
+    x[-5:] = torch.randn(5, k, device="cuda").to(torch.bfloat16)
+    y = linear_act(x, w, b)
+    B.within(y[-5:], B.linear(x[-5:], w, b, None, None, "none")["y"], "last rows")
+    assert torch.equal(y[: rows - 5], b.expand(rows - 5, n))
+
+
+def test_refusals(gpu):
+    from addernetcuda_amd.linear import linear_act, LinearAct
+    x, w, b, r, _ = make(4, 24, 16, torch.float32)
+    with pytest.raises(ValueError, match="act must be one of"):
+        linear_act(x, w, act="tanh")
+    with pytest.raises(ValueError, match="act must be one of"):
+        LinearAct(4, 4, act="tanh")
+    with pytest.raises(RuntimeError, match="expects 24 features"):
+        linear_act(x[:, :23], w)
+    with pytest.raises(RuntimeError, match="two dimensions"):
+        linear_act(x, w[0])
+    with pytest.raises(RuntimeError, match="bias must have shape"):
+        linear_act(x, w, b[:3])
+    with pytest.raises(RuntimeError, match="the type of x"):
+        linear_act(x, w.bfloat16())
+    with pytest.raises(RuntimeError, match="same device"):
+        linear_act(x, w.cpu())
+    with pytest.raises(RuntimeError, match="does not broadcast"):
+        linear_act(x, w, b, r[:, :5])

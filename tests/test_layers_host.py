@@ -1,0 +1,124 @@
+"""The linear layer, layer normalisation and AdamW without a GPU: the C entry points refuse bad arguments before they touch one, and the
+modules run torch's own operators on the CPU."""
+import ctypes
+
+import pytest
+import torch
+
+P = ctypes.c_void_p
+A = [P(k << 32) for k in range(1, 10)]
+
+
+def size(call, *args):
+    n = ctypes.c_size_t(123)
+    return call(*args, ctypes.byref(n)), n.value
+
+
+def test_linear_refuses():
+    from addernetcuda_amd._lib import lib
+    f, b = lib.adder_linear_fwd, lib.adder_linear_bwd
+    fwd = lambda x=A[0], ldx=64, w=A[1], bias=None, r=None, ldr=0, y=A[2], pre=None, act=0, rows=8, k=64, n=32, t=0, ws=A[3], nb=1 << 30: \
+        f(x, ldx, w, bias, r, ldr, y, pre, act, rows, k, n, t, ws, nb, None)
+    for bad in ({"x": None}, {"w": None}, {"y": None}):
+        assert fwd(**bad) == -1
+    for bad in ({"rows": 0}, {"k": 0}, {"n": -1}, {"act": 4}, {"act": -1}, {"t": 2}, {"ldx": 63}, {"ldx": -64}, {"r": A[4], "ldr": 31}):
+        assert fwd(**bad) == -2
+    assert fwd(rows=1 << 40) == -3 and fwd(ldx=1 << 40) == -3 and fwd(rows=1 << 30, k=64, n=1 << 20) == -3
+    for bad in ({"y": A[0]}, {"y": A[1]}, {"pre": A[2]}, {"r": A[2], "ldr": 32}, {"bias": A[2]}):
+        assert fwd(**bad) == -6
+    bwd = lambda dy=A[0], ldd=32, pre=A[1], x=A[2], ldx=64, w=A[3], gx=A[4], gw=A[5], gb=A[6], act=2, rows=8, k=64, n=32, t=0, ws=A[7], nb=1 << 30: \
+        b(dy, ldd, pre, x, ldx, w, gx, gw, gb, act, rows, k, n, t, ws, nb, None)
+    for bad in ({"dy": None}, {"pre": None}, {"x": None}, {"w": None}, {"gx": None, "gw": None, "gb": None}):
+        assert bwd(**bad) == -1
+    for bad in ({"rows": 0}, {"ldd": 31}, {"ldx": 3}, {"act": 7}, {"t": -1}):
+        assert bwd(**bad) == -2
+    rc, need = size(lib.adder_linear_bwd_workspace_bytes, 8, 64, 32, 2, 0)
+    assert rc == 0 and need >= 8 * 32 * 4
+    for bad in ({"ws": None}, {"nb": need - 1}, {"ws": P((7 << 32) + 8)}):
+        assert bwd(**bad) == -4
+    for bad in ({"gx": A[0]}, {"gw": A[2]}, {"gb": A[3]}, {"gw": A[4]}, {"ws": A[1]}):
+        assert bwd(**bad) == -6
+    assert size(lib.adder_linear_fwd_workspace_bytes, 0, 64, 32, 0)[0] == -2
+    assert lib.adder_linear_fwd_workspace_bytes(8, 64, 32, 0, None) == -1
+    assert size(lib.adder_linear_bwd_workspace_bytes, 8, 64, 32, 9, 0)[0] == -2
+
+
+def test_layer_norm_refuses():
+    from addernetcuda_amd._lib import lib
+    f, b = lib.adder_layer_norm_fwd, lib.adder_layer_norm_bwd
+    fwd = lambda x=A[0], ldx=64, w=A[1], bias=A[2], y=A[3], m=A[4], r=A[5], eps=1e-5, rows=8, d=64, t=0, wt=0: f(x, ldx, w, bias, y, m, r, eps, rows, d, t, wt, None)
+    for bad in ({"x": None}, {"y": None}, {"m": None}, {"r": None}):
+        assert fwd(**bad) == -1
+    for bad in ({"rows": 0}, {"d": 0}, {"ldx": 10}, {"eps": -1.0}, {"eps": float("nan")}, {"t": 3}, {"wt": 3}):
+        assert fwd(**bad) == -2
+    assert fwd(wt=1) == -7 and fwd(rows=1 << 40) == -3
+    for bad in ({"y": A[0]}, {"m": A[3]}, {"r": A[4]}, {"w": A[3]}):
+        assert fwd(**bad) == -6
+    bwd = lambda dy=A[0], ldd=64, x=A[1], ldx=64, w=A[2], m=A[3], r=A[4], gx=A[5], gw=A[6], gb=A[7], rows=8, d=64, t=1, wt=0, ws=A[8], nb=1 << 30: \
+        b(dy, ldd, x, ldx, w, m, r, gx, gw, gb, rows, d, t, wt, ws, nb, None)
+    for bad in ({"dy": None}, {"x": None}, {"m": None}, {"r": None}, {"gx": None, "gw": None, "gb": None}):
+        assert bwd(**bad) == -1
+    for bad in ({"rows": -1}, {"ldd": 1}, {"ldx": 1}, {"t": 9}):
+        assert bwd(**bad) == -2
+    rc, need = size(lib.adder_layer_norm_bwd_workspace_bytes, 8, 64, 1)
+    assert rc == 0 and need >= 2 * 64 * 4
+    assert bwd(nb=need - 1) == -4 and bwd(ws=None) == -4 and bwd(t=0, wt=1) == -7
+    for bad in ({"gx": A[0]}, {"gw": A[1]}, {"gb": A[6]}, {"ws": A[2]}):
+        assert bwd(**bad) == -6
+
+
+def test_adamw_refuses():
+    from addernetcuda_amd._lib import lib
+    at = lambda *ks: (P * len(ks))(*[k << 32 for k in ks])
+    n1 = (ctypes.c_long * 2)(100, 300)
+
+    def step(count=2, p=at(1, 2), g=at(3, 4), m=at(5, 6), v=at(7, 8), n=n1, lr=0.1, b1=0.9, b2=0.99, eps=1e-8, wd=0.0, t=1, kind=0):
+        return lib.adder_adamw_step(count, p, g, m, v, n, None, lr, b1, b2, eps, wd, t, None, kind, None)
+
+    def step8(count=2, p=at(1, 2), g=at(3, 4), m=at(5, 6), v=at(7, 8), ms=at(9, 10), vs=at(11, 12), n=n1, t=1):
+        return lib.adder_adamw_step_8bit(count, p, g, m, v, ms, vs, n, None, 0.1, 0.9, 0.99, 1e-8, 0.0, t, None, 0, None)
+
+    for name in "pgmvn":
+        assert step(**{name: None}) == -1
+    assert step(p=(P * 2)(1 << 32, None)) == -1
+    nan = float("nan")
+    for bad in ({"count": 0}, {"count": 97}, {"lr": -0.1}, {"lr": nan}, {"b1": 1.0}, {"b2": -0.1}, {"b2": nan}, {"eps": -1.0}, {"wd": -1.0}, {"t": 0},
+                {"kind": 2}, {"n": (ctypes.c_long * 2)(100, 0)}):
+        assert step(**bad) == -2, bad
+    assert step(n=(ctypes.c_long * 2)(100, 1 << 31)) == -3
+    for bad in ({"g": at(1, 4)}, {"m": at(1, 6)}, {"v": at(5, 8)}):
+        assert step(**bad) == -6
+    for name in ("ms", "vs"):
+        assert step8(**{name: None}) == -1
+    assert step8(count=65) == -2 and step8(t=0) == -2
+    for bad in ({"ms": at(5, 10)}, {"vs": at(9, 12)}, {"m": at(3, 6)}):
+        assert step8(**bad) == -6
+    assert lib.adder_adamw_advance(None, 0.9, 0.99, A[0], None) == -1 and lib.adder_adamw_advance(A[0], 1.0, 0.99, A[1], None) == -2
+    assert lib.adder_adamw_advance(A[0], 0.9, 0.99, A[0], None) == -6
+    assert lib.adder_state_values(A[0], 1, A[1], None, 8, 0, None) == -1 and lib.adder_state_values(A[0], 1, A[1], A[2], 0, 0, None) == -2
+    assert lib.adder_state_values(A[0], 1, A[1], A[0], 8, 0, None) == -6
+
+
+@pytest.mark.parametrize("act,fn", [("none", lambda t: t), ("relu", torch.relu), ("gelu", torch.nn.functional.gelu), ("silu", torch.nn.functional.silu)])
+def test_cpu_tensors_take_torchs_operators(act, fn):
+    from addernetcuda_amd.linear import LinearAct
+    from addernetcuda_amd.layer_norm import LayerNorm
+    layer, norm = LinearAct(12, 7, act=act), LayerNorm(12)
+    x, r = torch.randn(3, 5, 12), torch.randn(7)
+    want = fn(torch.nn.functional.linear(torch.nn.functional.layer_norm(x, (12,), norm.weight, norm.bias), layer.weight, layer.bias)) + r
+    assert torch.allclose(layer(norm(x), residual=r), want)
+
+
+def test_adamw_on_the_cpu_is_torchs():
+    from addernetcuda_amd.optim import AdamW
+    a, b = (torch.nn.Parameter(torch.ones(5, 4)) for _ in range(2))
+    oa, ob = AdamW([a], lr=0.1), torch.optim.AdamW([b], lr=0.1)
+    for t in range(3):
+        for p in (a, b):
+            p.grad = torch.full((5, 4), 0.1 * (t + 1))
+        oa.step()
+        ob.step()
+    assert torch.allclose(a, b)
+    with pytest.raises(RuntimeError, match="state_bits=8"):
+        o8 = AdamW([a], state_bits=8)
+        o8.step()
