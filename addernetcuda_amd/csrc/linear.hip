@@ -14,53 +14,71 @@ __global__ __launch_bounds__(256) void product_join_kernel(const ProductArgs p) 
     const long m = i / groups, n = i % groups * 4;
     const int cnt = p.N - n < 4 ? (int)(p.N - n) : 4;
     float v[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < p.splits; ++s) {
-        const float *q = p.part + ((long)s * p.M + m) * p.N + n;
-        float t[4] = {0.f, 0.f, 0.f, 0.f};
-        if (cnt == 4) {
-            ld_strip<4>(q, t);
-        } else {
+    const float *q = p.part + m * p.N + n;
+    const long share = p.M * p.N;
+    int s = 0;
+    if (cnt == 4) {
+        for (; s + 4 <= p.splits; s += 4) {   // (four loads under way)
+            float t[4][4];
 #pragma unroll
-            for (int e = 0; e < 3; ++e)
-                if (e < cnt) t[e] = q[e];
+            for (int u = 0; u < 4; ++u) ld_strip<4>(q + (s + u) * share, t[u]);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] += t[u][e];
         }
+    }
+    for (; s < p.splits; ++s) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] += t[e];
+        for (int e = 0; e < 4; ++e) v[e] += e < cnt ? q[s * share + e] : 0.f;
     }
     finish<T>(p, m, n, cnt, v);
 }
 
 // ---- which kernel ---------------------------------------------------------------------------------------------------
-// A launch's time is estimated as rounds * (steps * step + tile) us for every shape and number of shares of k, and the least is
-// taken: rounds of as many workgroups as the card holds, steps of 64 (float32: 32) values of k a workgroup, `step` measured on a full
-// card (8192^3), `alone` where a compute unit has one workgroup only, `tile` the epilogue, the first loads and the start.  Shares of k
-// pay for their sums' way through memory (5 TB/s both ways) and the join's launch.
+// A launch's time is estimated for every shape of tile and number of shares of k, and the least is taken.  The workgroups run in rounds
+// of as many as the card holds, each steps * step + tile us: steps of 64 (float32: 32) values of k; `step` measured with every compute
+// unit full (8192 x 8192 x 1024 and 8192^3), less in proportion where fewer workgroups share one, but at least `alone` (1024^3); `tile` the first
+// loads, the epilogue and the start.  Shares of k pay for their sums' way through memory (5 TB/s both ways) and the join's launch.
+static constexpr int kCUs = 256;
 struct Shape { int bm, bn, per_cu; float step, alone, tile; };
-//                                     8192^3 in bfloat16 (float32), TFLOP/s
+//                                       8192^3, TFLOP/s
 static constexpr Shape kStreamShapes[] = {
-    {256, 256, 1, 1.6f, 1.6f, 8.f},    // 1320
-    {128, 256, 1, 0.93f, 0.93f, 4.5f}, // 1155
-    {128, 128, 2, 0.92f, 0.65f, 4.5f}, // 1155
+    {256, 256, 1, 1.55f, 1.55f, 8.f},    // 1320
+    {128, 256, 1, 0.9f, 0.9f, 4.f},      // 1155
+    {128, 128, 2, 0.87f, 0.5f, 3.5f},    // 1155
+    {64, 64, 2, 0.38f, 0.2f, 1.5f},      //  640
 };
 template <class T>
 static constexpr Shape kStagedShapes[] = {
-    {128, 128, 2, 1.1f, 0.9f, 5.f},    // 960
-    {64, 64, 4, 0.84f, 0.5f, 4.f},     // 636
+    {128, 128, 2, 1.f, 0.6f, 3.5f},      //  960
+    {64, 64, 4, 0.78f, 0.25f, 1.5f},     //  640
 };
 template <>
 constexpr Shape kStagedShapes<float>[] = {
-    {128, 128, 2, 2.8f, 2.0f, 6.f},    // (190)
-    {64, 64, 4, 1.75f, 0.8f, 5.f},     // (153)
+    {128, 128, 2, 2.3f, 1.9f, 3.5f},     //  220
+    {64, 64, 3, 1.25f, 0.65f, 1.5f},     //  155
+    {128, 128, 1, 1.25f, 1.25f, 3.5f},   //  200
 };
-static constexpr int kCUs = 256, kSplitMax = 16;
+static constexpr int kSplitMax = 16;
 
-struct ProductPlan { int shape, splits; long k_share; };
+struct ProductPlan { int shape, splits; long k_share; float us; };
+
+// The kernel for few rows likewise: workgroups of 16 columns and 16, 32 or 64 rows, whose waves take turns along k, 128 bytes of every
+// row at a time (us each, with the rows' share of the second-level caches: 4096 x 4096, full workgroups)
+template <class T>
+static float rows_us(long M, long N, long K) {
+    static constexpr float kTurn[2][3] = {{1.2f, 2.1f, 1.95f}, {1.75f, 2.5f, 2.2f}};
+    const int mt = M <= 16 ? 0 : M <= 32 ? 1 : 2;
+    const float groups = (float)ceil_div_l(N, 16) * (float)ceil_div_l(M, 16 << mt);
+    const long turns = ceil_div_l(ceil_div_l(K, 8 * Chunk<T>::n), mt == 2 ? 8 : 16);
+    return 3.f + ceilf(groups / kCUs) * (1.3f + turns * kTurn[sizeof(T) == 4][mt]);
+}
 
 template <int N>
 static ProductPlan plan_product(const Shape (&shapes)[N], int bk, long M, long N_, long K) {
     static constexpr int kSplits[] = {1, 2, 3, 4, 6, 8, 12, kSplitMax};
-    ProductPlan best{0, 1, K};
-    float least = 0.f;
+    ProductPlan best{0, 1, K, 0.f};
     const long steps = ceil_div_l(K, bk);
     for (int i = 0; i < N; ++i) {
         const Shape &h = shapes[i];
@@ -69,13 +87,16 @@ static ProductPlan plan_product(const Shape (&shapes)[N], int bk, long M, long N
             if (splits > steps || (splits > 1 && tiles * splits > 4.f * kCUs)) break;
             const long share = ceil_div_l(steps, splits);
             const float groups = tiles * splits;
-            const float rounds = ceilf(groups / (kCUs * h.per_cu));
-            float us = rounds * (share * (groups <= kCUs ? h.alone : h.step) + h.tile);
-            if (splits > 1) us += 4.f + (float)M * (float)N_ * splits * 8.f / 5e6f;
-            if (least == 0.f || us < least) {
-                least = us;
+            const float slots = (float)(kCUs * h.per_cu), whole = floorf(groups / slots), rest = groups - whole * slots;
+            float us = 3.f + whole * (share * h.step + h.tile);
+            if (rest > 0.f) {
+                const float shared = h.step * ceilf(rest / kCUs) / h.per_cu;
+                us += share * (shared > h.alone ? shared : h.alone) + h.tile;
+            }
+            if (splits > 1) us += 3.f + (float)M * (float)N_ * splits * 8.f / 5e6f;
+            if (best.us == 0.f || us < best.us) {
                 const int used = (int)ceil_div_l(steps, share);
-                best = ProductPlan{i, used, used > 1 ? share * bk : K};
+                best = ProductPlan{i, used, used > 1 ? share * bk : K, us};
             }
         }
     }
@@ -105,22 +126,26 @@ size_t product_workspace_bytes(long M, long N, long K) {
 template <class T>
 int launch_product(const Product &q, void *ws, hipStream_t s) {
     const bool stream = sizeof(T) == 2 && fits_stream(q.a, q.lda, q.a_across, q.K) && fits_stream(q.b, q.ldb, q.b_across, q.K);
-    const ProductPlan plan = stream ? plan_stream(q.M, q.N, q.K) : plan_staged<T>(q.M, q.N, q.K);
+    ProductPlan plan = stream ? plan_stream(q.M, q.N, q.K) : plan_staged<T>(q.M, q.N, q.K);
+    const bool rows = !q.a_across && !q.b_across && rows_us<T>(q.M, q.N, q.K) < plan.us;
+    if (rows) plan = ProductPlan{0, 1, q.K, 0.f};
     const ProductArgs p{q.a, q.b, q.bias, q.res, q.out, q.pre, static_cast<float *>(ws), q.lda, q.ldb, q.ldr, q.M, q.N, q.K, plan.k_share, 0, 0,
                         plan.splits, q.act};
-    const int rc = stream ? launch_product_stream(p, q.a_across, q.b_across, static_cast<StreamShape>(plan.shape), s)
-                          : launch_product_staged<T>(p, q.a_across, q.b_across, plan.shape == 1, s);
+    const int rc = rows ? launch_product_rows<T>(p, s)
+                 : stream ? launch_product_stream(p, q.a_across, q.b_across, static_cast<StreamShape>(plan.shape), s)
+                 : launch_product_staged<T>(p, q.a_across, q.b_across, static_cast<StagedShape>(plan.shape), s);
     if (rc || plan.splits == 1) return rc;
     hipLaunchKernelGGL(product_join_kernel<T>, dim3((unsigned)ceil_div_l(q.M * ((q.N + 3) / 4), 256)), dim3(256), 0, s, p);
     return check_launch();
 }
 
 // ---- the activation's derivative and the bias's gradient ---------------------------------------------------------------
-// A workgroup takes 64 lanes' chunks of columns and a share of the rows: its four waves walk over the rows, and their column
-// sums are added through LDS into one slab per share.
-template <class T>
+// A workgroup takes 64 lanes' chunks of columns and a share of the rows: its four waves walk over the rows, kActRows of them under way,
+// and their column sums are added through LDS into one slab a share.
+static constexpr int kActRows = 4;
+template <class T, Act ACT>
 __global__ __launch_bounds__(256) void act_bwd_kernel(const T *__restrict__ dy, long dy_stride, const T *__restrict__ z,
-                                                      T *__restrict__ dz, float *__restrict__ part, Act act, long rows, long N) {
+                                                      T *__restrict__ dz, float *__restrict__ part, long rows, long N) {
     constexpr int V = Chunk<T>::n;
     __shared__ float lds[4][64 * V];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -129,17 +154,31 @@ __global__ __launch_bounds__(256) void act_bwd_kernel(const T *__restrict__ dy, 
     float sum[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) sum[e] = 0.f;
-    for (long m = (long)blockIdx.y * 4 + wave; m < rows; m += (long)gridDim.y * 4) {
-        float g[V], v[V];
-        load_part(dy + m * dy_stride + n, left, g);
-        if (act != Act::none) {
-            load_part(z + m * N + n, left, v);
+    const long ahead = (long)gridDim.y * 4;   // rows from one of a wave's to the next
+    for (long m0 = (long)blockIdx.y * 4 + wave; m0 < rows; m0 += kActRows * ahead) {
+        uint4 g[kActRows], v[kActRows];
 #pragma unroll
-            for (int e = 0; e < V; ++e) g[e] *= slope<kExactAct<T>>(v[e], act);
-            if (dz) store_part(dz + m * N + n, left, g);
+        for (int r = 0; r < kActRows; ++r) {
+            const long m = m0 + r * ahead;
+            const int valid = m < rows ? left : 0;
+            g[r] = load_raw_part(dy + m * dy_stride + n, valid);
+            if constexpr (ACT != Act::none) v[r] = load_raw_part(z + m * N + n, valid);
         }
 #pragma unroll
-        for (int e = 0; e < V; ++e) sum[e] += g[e];
+        for (int r = 0; r < kActRows; ++r) {
+            const long m = m0 + r * ahead;
+            float d[V];
+            unpack(g[r], d);
+            if constexpr (ACT != Act::none) {
+                float w[V];
+                unpack(v[r], w);
+#pragma unroll
+                for (int e = 0; e < V; ++e) d[e] *= slope<kExactAct<T>>(w[e], ACT);
+                if (dz) store_part(dz + m * N + n, m < rows ? left : 0, d);
+            }
+#pragma unroll
+            for (int e = 0; e < V; ++e) sum[e] += d[e];   // (rows that do not exist: dy of zero times the slope at zero)
+        }
     }
     if (!part) return;
 #pragma unroll
@@ -155,15 +194,21 @@ __global__ __launch_bounds__(256) void act_bwd_kernel(const T *__restrict__ dy, 
     }
 }
 
+// Shares of the rows: enough workgroups for eight a compute unit, and at least kActRows rows a wave
 int act_bwd_parts(long rows, long N) {
-    const long columns = ceil_div_l(N, 256), need = ceil_div_l(rows, 16), most = ceil_div_l(1024, columns);
+    const long columns = ceil_div_l(N, 512), need = ceil_div_l(rows, 4 * kActRows), most = ceil_div_l(2048, columns);
     return (int)(need < most ? need : most);
 }
 
 template <class T>
 int launch_act_bwd(const T *dy, long dy_stride, const T *z, T *dz, float *part, Act act, long rows, long N, hipStream_t s) {
-    hipLaunchKernelGGL(act_bwd_kernel<T>, dim3((unsigned)ceil_div_l(N, 64 * Chunk<T>::n), act_bwd_parts(rows, N)), dim3(256), 0, s, dy,
-                       dy_stride, z, dz, part, act, rows, N);
+    const dim3 grid((unsigned)ceil_div_l(N, 64 * Chunk<T>::n), act_bwd_parts(rows, N)), threads(256);
+    switch (act) {
+        case Act::relu: hipLaunchKernelGGL((act_bwd_kernel<T, Act::relu>), grid, threads, 0, s, dy, dy_stride, z, dz, part, rows, N); break;
+        case Act::gelu: hipLaunchKernelGGL((act_bwd_kernel<T, Act::gelu>), grid, threads, 0, s, dy, dy_stride, z, dz, part, rows, N); break;
+        case Act::silu: hipLaunchKernelGGL((act_bwd_kernel<T, Act::silu>), grid, threads, 0, s, dy, dy_stride, z, dz, part, rows, N); break;
+        default: hipLaunchKernelGGL((act_bwd_kernel<T, Act::none>), grid, threads, 0, s, dy, dy_stride, z, dz, part, rows, N);
+    }
     return check_launch();
 }
 

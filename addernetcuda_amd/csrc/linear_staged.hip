@@ -13,7 +13,6 @@ namespace adder {
 // them the six that matter, hi hi, hi mid, mid hi, mid mid, hi lo and lo hi, are summed in 32 bits: what is left out is 2^-26 of a
 // product.  An operand that is infinite, not a number, or rounds up to infinity gives a sum that is not finite; a wave that finds some
 // computes those again, in float32.
-static constexpr int kStagedThreads = 256;
 template <class T>
 static constexpr int kStagedPlanes = sizeof(T) == 4 ? 3 : 1;
 template <class T>
@@ -30,40 +29,80 @@ __device__ __forceinline__ void split(float x, float y, uint32_t (&o)[3]) {
     o[2] = pack_bf16(x - low_f32(o[1]), y - high_f32(o[1]));
 }
 
-// One operand's tile: loads of 16 bytes, of 4 floats or 8 bfloat16 that lie side by side
-template <class T, int R, bool ACROSS>
+// One operand's tile: loads of 16 bytes, of 4 floats or 8 bfloat16 that lie side by side.  The loads of the main loop have no branch
+// around them (a wait behind one would have to be for all that is under way): rows and columns that do not exist are other ones
+// again, whose results are not stored; with k across the rows, a chunk that ends beyond the last column is read value by value (EDGE).
+// Only the last tile of a k that is no whole number of tiles holds zeros, and is read on its own.
+template <class T, int R, bool ACROSS, int THREADS>
 struct Staged {
     static constexpr int E = Chunk<T>::n, BK = kStagedK<T>, P = kStagedPlanes<T>;
     typedef LdsTile<R, BK, ACROSS> Tile;
-    static constexpr int row_loads = Tile::row_chunks * 8 / E, per = R * BK / E / kStagedThreads;
-    uint4 v[per];
+    static constexpr int row_loads = Tile::row_chunks * 8 / E, per = R * BK / E / THREADS;
+    struct Values { uint4 v[per]; };
+    const T *at[per];   // of the next tile
+    int most[per];      // across: a chunk's last column that exists, counted from its first
+    long step;
 
-    __device__ __forceinline__ void load(const T *p, long ld, long rows, long k_end, long row0, long k0) {
+    // chunk i of this thread: its row (across: of k) and its first column (along: of k) in the tile
+    static __device__ __forceinline__ int row_of(int i) { return (threadIdx.x + i * THREADS) / row_loads; }
+    static __device__ __forceinline__ int column_of(int i) { return (threadIdx.x + i * THREADS) % row_loads * E; }
+    static __device__ __forceinline__ bool edge(long all, long row0) { return ACROSS && row0 + R > all; }
+
+    __device__ __forceinline__ void setup(const T *p, long ld, long all, long row0, long k_begin) {
+        step = ACROSS ? BK * ld : BK;
 #pragma unroll
         for (int i = 0; i < per; ++i) {
-            const int u = threadIdx.x + i * kStagedThreads, c = u % row_loads, r = u / row_loads;
-            long left;
-            const T *q;
+            const int r = row_of(i), c = column_of(i);
             if constexpr (ACROSS) {
-                left = k0 + r < k_end ? rows - row0 - c * E : 0;
-                q = p + (k0 + r) * ld + row0 + c * E;
+                const long col = row0 + c < all ? row0 + c : all - 1, left = all - 1 - col;
+                at[i] = p + (k_begin + r) * ld + col;
+                most[i] = left < E - 1 ? (int)left : E - 1;
             } else {
-                left = row0 + r < rows ? k_end - k0 - c * E : 0;
-                q = p + (row0 + r) * ld + k0 + c * E;
+                at[i] = p + (row0 + r < all ? row0 + r : all - 1) * ld + k_begin + c;
             }
-            v[i] = load_raw_part(q, left < 0 ? 0 : left < E ? (int)left : E);
         }
     }
-    __device__ __forceinline__ void store(char *tile) const {
+    template <bool EDGE>
+    __device__ __forceinline__ void load(Values &t, bool more) {
 #pragma unroll
         for (int i = 0; i < per; ++i) {
-            const int u = threadIdx.x + i * kStagedThreads, c = u % row_loads, r = u / row_loads;
+            if constexpr (EDGE && ACROSS) {
+                uint32_t w[4];
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const T *q = at[i] + (e < most[i] ? e : most[i]);
+                    if constexpr (E == 4) w[e] = __float_as_uint(*q);
+                    else w[e / 2] = e & 1 ? w[e / 2] | (uint32_t)*q << 16 : *q;
+                }
+                t.v[i] = make_uint4(w[0], w[1], w[2], w[3]);
+            } else {
+                t.v[i] = load_raw(at[i]);
+            }
+        }
+        const long go = more ? step : 0;   // (past the last whole tile: that one again, unused)
+#pragma unroll
+        for (int i = 0; i < per; ++i) at[i] += go;
+    }
+    // the tile from k on, of which `left` values of k exist
+    static __device__ __forceinline__ void load_last(Values &t, const T *p, long ld, long all, long row0, long k, int left) {
+#pragma unroll
+        for (int i = 0; i < per; ++i) {
+            const int r = row_of(i), c = column_of(i);
+            const long rows = all - row0 - (ACROSS ? c : r);
+            if constexpr (ACROSS) t.v[i] = load_raw_part(p + (k + r) * ld + row0 + c, r >= left || rows <= 0 ? 0 : rows < E ? (int)rows : E);
+            else t.v[i] = load_raw_part(p + (row0 + r) * ld + k + c, rows <= 0 ? 0 : left - c);
+        }
+    }
+    static __device__ __forceinline__ void store(char *tile, const Values &t) {
+#pragma unroll
+        for (int i = 0; i < per; ++i) {
+            const int r = row_of(i), c = column_of(i) / E;
             if constexpr (P == 1) {
-                *reinterpret_cast<uint4 *>(tile + r * Tile::row_bytes + (Tile::place(r, c) << 4)) = v[i];
+                *reinterpret_cast<uint4 *>(tile + r * Tile::row_bytes + (Tile::place(r, c) << 4)) = t.v[i];
             } else {
                 uint32_t a[3], b[3];
-                split(__uint_as_float(v[i].x), __uint_as_float(v[i].y), a);
-                split(__uint_as_float(v[i].z), __uint_as_float(v[i].w), b);
+                split(__uint_as_float(t.v[i].x), __uint_as_float(t.v[i].y), a);
+                split(__uint_as_float(t.v[i].z), __uint_as_float(t.v[i].w), b);
                 char *q = tile + r * Tile::row_bytes + (Tile::place(r, c >> 1) << 4) + ((c & 1) << 3);
 #pragma unroll
                 for (int k = 0; k < 3; ++k) *reinterpret_cast<uint2 *>(q + k * Tile::bytes) = make_uint2(a[k], b[k]);
@@ -111,16 +150,17 @@ __device__ __forceinline__ void sum_again(const ProductArgs &p, f32x4 (&acc)[TM]
             for (int e = 0; e < 4; ++e) acc[i][j][e] = fabsf(acc[i][j][e]) < __builtin_inff() ? acc[i][j][e] : again[i][j][e];
 }
 
-// AHEAD: tiles in registers or on their way there.  Small tiles are multiplied faster than the next arrives.
-template <class T, int TM, int TN, bool AA, bool BA>
-__global__ __launch_bounds__(kStagedThreads, 2) void product_staged_kernel(const ProductArgs p) {
-    constexpr int BM = TM * 32, BN = TN * 32, BK = kStagedK<T>, P = kStagedPlanes<T>, AHEAD = TM * TN <= 4 ? 3 : 1;
-    typedef Staged<T, BM, AA> SA;
-    typedef Staged<T, BN, BA> SB;
-    __shared__ __align__(16) char lds[P * (SA::Tile::bytes + SB::Tile::bytes)];
-    char *ta = lds, *tb = lds + P * SA::Tile::bytes;
+// WM x WN waves of TM x TN tiles of 16 x 16.  AHEAD: tiles of k in registers or on their way there (small ones are multiplied faster than the
+// next arrives).  BUFFERS = 2: one barrier a tile, and the next is split and stored while this one is multiplied.
+template <class T, int WM, int WN, int TM, int TN, int AHEAD, int BUFFERS, bool AA, bool BA>
+__global__ __launch_bounds__(WM *WN * 64, 2) void product_staged_kernel(const ProductArgs p) {
+    constexpr int BM = WM * TM * 16, BN = WN * TN * 16, BK = kStagedK<T>, P = kStagedPlanes<T>, THREADS = WM * WN * 64;
+    typedef Staged<T, BM, AA, THREADS> SA;
+    typedef Staged<T, BN, BA, THREADS> SB;
+    constexpr int BYTES = P * (SA::Tile::bytes + SB::Tile::bytes);
+    extern __shared__ __align__(16) char lds[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wm = (wave & 1) * (TM * 16), wn = (wave >> 1) * (TN * 16);
+    const int wm = (wave % WM) * (TM * 16), wn = (wave / WM) * (TN * 16);
     int tm, tn;
     tile_of(blockIdx.x, p.tiles_m, p.tiles_n, tm, tn);
     const long m0 = (long)tm * BM, n0 = (long)tn * BN;
@@ -131,47 +171,96 @@ __global__ __launch_bounds__(kStagedThreads, 2) void product_staged_kernel(const
     for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    SA sa[AHEAD];
-    SB sb[AHEAD];
-#pragma unroll
-    for (int d = 0; d < AHEAD; ++d) {
-        sa[d].load(a, p.lda, p.M, k_end, m0, k_begin + d * BK);
-        sb[d].load(b, p.ldb, p.N, k_end, n0, k_begin + d * BK);
-    }
-    auto step = [&](long k0, SA &na, SB &nb) {
-        __syncthreads();
-        na.store(ta);
-        nb.store(tb);
-        __syncthreads();
-        if (k0 + AHEAD * BK < k_end) {
-            na.load(a, p.lda, p.M, k_end, m0, k0 + AHEAD * BK);
-            nb.load(b, p.ldb, p.N, k_end, n0, k0 + AHEAD * BK);
-        }
+    // One tile: `between` runs once the first operands have been asked for
+    auto multiply = [&](const char *ta, auto between) {
+        const char *tb = ta + P * SA::Tile::bytes;
 #pragma unroll
         for (int k = 0; k < BK; k += 32) {
-            bf16x8 fb[P][TN];
+            bf16x8 fb[P][TN], fa[2][P];
+            auto read = [&](int i) {
+#pragma unroll
+                for (int q = 0; q < P; ++q) fa[i & 1][q] = SA::Tile::fragment(ta + q * SA::Tile::bytes, wm + i * 16, k, lane);
+            };
 #pragma unroll
             for (int q = 0; q < P; ++q)
 #pragma unroll
                 for (int j = 0; j < TN; ++j) fb[q][j] = SB::Tile::fragment(tb + q * SB::Tile::bytes, wn + j * 16, k, lane);
+            read(0);
 #pragma unroll
             for (int i = 0; i < TM; ++i) {
-                bf16x8 fa[P];
-#pragma unroll
-                for (int q = 0; q < P; ++q) fa[q] = SA::Tile::fragment(ta + q * SA::Tile::bytes, wm + i * 16, k, lane);
+                if (i + 1 < TM) read(i + 1);
+                if (k == 0 && i == 0) between();
 #pragma unroll
                 for (int u = P == 3 ? 2 : 0; u >= 0; --u)   // (the small products first)
 #pragma unroll
                     for (int q = 0; q <= u; ++q)
 #pragma unroll
-                        for (int j = 0; j < TN; ++j) acc[i][j] = mfma(fb[u - q][j], fa[q], acc[i][j]);
+                        for (int j = 0; j < TN; ++j) acc[i][j] = mfma(fb[u - q][j], fa[i & 1][q], acc[i][j]);
             }
         }
     };
-    for (long k0 = k_begin; k0 < k_end; k0 += AHEAD * BK)
+    const int full = (int)((k_end - k_begin) / BK), left = (int)(k_end - k_begin - (long)full * BK);
+    auto walk = [&](auto edge) {   // over the whole tiles of k
+        constexpr bool EDGE = decltype(edge)::value;
+        SA sa;
+        SB sb;
+        sa.setup(a, p.lda, p.M, m0, k_begin);
+        sb.setup(b, p.ldb, p.N, n0, k_begin);
+        typename SA::Values va[AHEAD];
+        typename SB::Values vb[AHEAD];
+        int next = 0;
+        auto load = [&](int d) {
+            ++next;
+            sa.template load<EDGE>(va[d], next < full);
+            sb.template load<EDGE>(vb[d], next < full);
+        };
+        auto store = [&](char *tile, int d) {
+            SA::store(tile, va[d]);
+            SB::store(tile + P * SA::Tile::bytes, vb[d]);
+        };
 #pragma unroll
-        for (int d = 0; d < AHEAD; ++d)
-            if (k0 + d * BK < k_end) step(k0 + d * BK, sa[d], sb[d]);
+        for (int d = 0; d < AHEAD; ++d) load(d);
+        if constexpr (BUFFERS == 2) {
+            store(lds, 0);
+            load(0);
+            int buf = 0;
+            for (int t = 0; t < full; t += AHEAD)
+#pragma unroll
+                for (int d = 0; d < AHEAD; ++d) {
+                    if (t + d >= full) break;
+                    __syncthreads();   // this tile is there; the other buffer has been read
+                    multiply(lds + buf * BYTES, [&]() {
+                        store(lds + (buf ^ 1) * BYTES, (d + 1) % AHEAD);
+                        load((d + 1) % AHEAD);
+                    });
+                    buf ^= 1;
+                }
+        } else {
+            for (int t = 0; t < full; ++t) {
+                __syncthreads();
+                store(lds, 0);
+                __syncthreads();
+                load(0);
+                multiply(lds, [] {});
+            }
+        }
+    };
+    if (full) {
+        if (SA::edge(p.M, m0) || SB::edge(p.N, n0)) walk(Flag<true>{});
+        else walk(Flag<false>{});
+    }
+    if (left) {
+        typename SA::Values va;
+        typename SB::Values vb;
+        const long k = k_begin + (long)full * BK;
+        SA::load_last(va, a, p.lda, p.M, m0, k, left);
+        SB::load_last(vb, b, p.ldb, p.N, n0, k, left);
+        __syncthreads();
+        SA::store(lds, va);
+        SB::store(lds + P * SA::Tile::bytes, vb);
+        __syncthreads();
+        multiply(lds, [] {});
+    }
     if constexpr (P == 3) {
         bool finite = true;
 #pragma unroll
@@ -185,21 +274,34 @@ __global__ __launch_bounds__(kStagedThreads, 2) void product_staged_kernel(const
     finish_wave<T, TM, TN>(p, acc, m0 + wm, n0 + wn, lane);
 }
 
-template <class T, int TM, int TN>
-static int launch_staged(ProductArgs p, bool a_across, bool b_across, hipStream_t s) {
-    p.tiles_m = (int)ceil_div_l(p.M, TM * 32);
-    p.tiles_n = (int)ceil_div_l(p.N, TN * 32);
-    const dim3 grid((unsigned)p.tiles_m * p.tiles_n, p.splits), threads(kStagedThreads);
-    if (!a_across && !b_across) hipLaunchKernelGGL((product_staged_kernel<T, TM, TN, false, false>), grid, threads, 0, s, p);
-    else if (!a_across) hipLaunchKernelGGL((product_staged_kernel<T, TM, TN, false, true>), grid, threads, 0, s, p);
-    else hipLaunchKernelGGL((product_staged_kernel<T, TM, TN, true, true>), grid, threads, 0, s, p);
+template <class T, int WM, int WN, int TM, int TN, int AHEAD, int BUFFERS, bool AA, bool BA>
+static int launch_staged_layout(ProductArgs p, hipStream_t s) {
+    constexpr int BM = WM * TM * 16, BN = WN * TN * 16, bytes = BUFFERS * kStagedPlanes<T> * (BM + BN) * kStagedK<T> * 2;
+    p.tiles_m = (int)ceil_div_l(p.M, BM);
+    p.tiles_n = (int)ceil_div_l(p.N, BN);
+    if (int rc = allow_dynamic_lds<&product_staged_kernel<T, WM, WN, TM, TN, AHEAD, BUFFERS, AA, BA>>(bytes)) return rc;
+    hipLaunchKernelGGL((product_staged_kernel<T, WM, WN, TM, TN, AHEAD, BUFFERS, AA, BA>), dim3((unsigned)p.tiles_m * p.tiles_n, p.splits),
+                       dim3(WM * WN * 64), bytes, s, p);
     return check_launch();
 }
-template <class T>
-int launch_product_staged(ProductArgs p, bool a_across, bool b_across, bool small, hipStream_t s) {
-    return small ? launch_staged<T, 2, 2>(p, a_across, b_across, s) : launch_staged<T, 4, 4>(p, a_across, b_across, s);
+template <class T, int WM, int WN, int TM, int TN, int AHEAD, int BUFFERS>
+static int launch_staged(const ProductArgs &p, bool a_across, bool b_across, hipStream_t s) {
+    if (a_across) return launch_staged_layout<T, WM, WN, TM, TN, AHEAD, BUFFERS, true, true>(p, s);
+    return b_across ? launch_staged_layout<T, WM, WN, TM, TN, AHEAD, BUFFERS, false, true>(p, s)
+                    : launch_staged_layout<T, WM, WN, TM, TN, AHEAD, BUFFERS, false, false>(p, s);
 }
-template int launch_product_staged<float>(ProductArgs, bool, bool, bool, hipStream_t);
-template int launch_product_staged<bf16_t>(ProductArgs, bool, bool, bool, hipStream_t);
+template <>
+int launch_product_staged<float>(const ProductArgs &p, bool a_across, bool b_across, StagedShape shape, hipStream_t s) {
+    switch (shape) {
+        case StagedShape::large: return launch_staged<float, 2, 2, 4, 4, 1, 1>(p, a_across, b_across, s);
+        case StagedShape::small: return launch_staged<float, 2, 2, 2, 2, 3, 2>(p, a_across, b_across, s);
+        default: return launch_staged<float, 2, 4, 4, 2, 1, 2>(p, a_across, b_across, s);
+    }
+}
+template <>
+int launch_product_staged<bf16_t>(const ProductArgs &p, bool a_across, bool b_across, StagedShape shape, hipStream_t s) {
+    return shape == StagedShape::large ? launch_staged<bf16_t, 2, 2, 4, 4, 1, 1>(p, a_across, b_across, s)
+                                       : launch_staged<bf16_t, 2, 2, 2, 2, 3, 2>(p, a_across, b_across, s);
+}
 
 }  // namespace adder

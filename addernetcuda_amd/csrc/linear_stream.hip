@@ -56,9 +56,6 @@ __device__ __forceinline__ bf16x8 keep_first(const bf16x8 &v, int valid) {
     return __builtin_bit_cast(bf16x8, u);
 }
 
-template <bool V>
-struct Flag { static constexpr bool value = V; };
-
 template <int WM, int WN, int TM, int TN, int BK, int STAGES, bool AA, bool BA, int OCC>
 __global__ __launch_bounds__(WM *WN * 64, OCC) void product_stream_kernel(const ProductArgs p) {
     constexpr int WAVES = WM * WN, BM = WM * TM * 16, BN = WN * TN * 16;
@@ -157,7 +154,8 @@ static int launch_stream_shape(const ProductArgs &p, StreamShape shape, hipStrea
     switch (shape) {
         case StreamShape::big: return launch_stream<2, 4, 8, 4, 64, 2, AA, BA>(p, s);
         case StreamShape::wide: return launch_stream<2, 4, 4, 4, 64, 3, AA, BA>(p, s);
-        default: return launch_stream<2, 2, 4, 4, 64, 2, AA, BA>(p, s);
+        case StreamShape::mid: return launch_stream<2, 2, 4, 4, 64, 2, AA, BA>(p, s);
+        default: return launch_stream<2, 2, 2, 2, 64, 4, AA, BA>(p, s);
     }
 }
 int launch_product_stream(ProductArgs p, bool a_across, bool b_across, StreamShape shape, hipStream_t s) {

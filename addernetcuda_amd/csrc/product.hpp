@@ -225,6 +225,9 @@ __device__ __forceinline__ void finish_wave(const ProductArgs &p, const f32x4 (&
     }
 }
 
+template <bool V>
+struct Flag { static constexpr bool value = V; };
+
 // ---- operands in LDS -------------------------------------------------------------------------------------------------
 // A tile of R rows (or columns, with k across the rows) by BK values of k in bfloat16.  Where rows lie a power of two apart, a bank
 // conflict is avoided by the order of their 16-byte chunks:
@@ -266,9 +269,13 @@ __device__ __forceinline__ void tile_of(int id, int tiles_m, int tiles_n, int &t
 }
 
 // Launches of the tiled kernels; p has everything but its tiles
-enum class StreamShape { big, wide, mid };   // 256 x 256, 128 x 256, 128 x 128 results a workgroup
+enum class StreamShape { big, wide, mid, small };   // 256 x 256, 128 x 256, 128 x 128, 64 x 64 results a workgroup
 int launch_product_stream(ProductArgs p, bool a_across, bool b_across, StreamShape shape, hipStream_t s);
+// 128 x 128, 64 x 64, and (float32) 128 x 128 by twice as many waves, for launches that leave a compute unit one workgroup
+enum class StagedShape { large, small, alone };
 template <class T>
-int launch_product_staged(ProductArgs p, bool a_across, bool b_across, bool small, hipStream_t s);
+int launch_product_staged(const ProductArgs &p, bool a_across, bool b_across, StagedShape shape, hipStream_t s);
+template <class T>
+int launch_product_rows(const ProductArgs &p, hipStream_t s);   // both along; few rows
 
 }  // namespace adder
