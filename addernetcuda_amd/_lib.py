@@ -114,6 +114,13 @@ class BnLinks(ctypes.Structure):
                 ("out_dbeta", ctypes.c_void_p)]
 
 
+if not os.path.exists(os.path.join(_HERE, "_nodes.so")):
+    raise ImportError(f"{os.path.join(_HERE, '_nodes.so')} is missing: build it with `python addernetcuda_amd/build.py`.")
+from . import _nodes as nodes   # noqa: E402  (csrc/nodes.cpp: runs on the library that is loaded here)
+
+nodes.bind({_name: ctypes.cast(getattr(lib, _name), ctypes.c_void_p).value for _name in _SIGNATURES})
+
+
 def check(status, what):
     """Turn a negative adder_status into the RuntimeError the reference's AT_ASSERTM would raise."""
     if status != 0:
@@ -176,6 +183,19 @@ def plain_call(x):
     return (type(x) is torch.Tensor and not torch.is_grad_enabled() and not _functorch_stack()
             and _forward_ad._current_level < 0 and not _dispatch_modes() and (not _function_modes() or _only_default_device())
             and not _is_tracing() and not _is_compiling())
+
+
+_PLAIN = frozenset((torch.Tensor, torch.nn.Parameter, type(None)))
+
+
+def plain_tensors(x, *rest):
+    """Whether these (or None) are ordinary tensors in an ordinary call: nothing but autograd's reverse mode records, transforms or traces it."""
+    if type(x) not in _PLAIN or _functorch_stack() or _dispatch_modes() or _forward_ad._current_level >= 0 or _is_tracing() or _is_compiling():
+        return False
+    for t in rest:
+        if type(t) not in _PLAIN:
+            return False
+    return not _function_modes() or _only_default_device()
 
 
 def _only_default_device():

@@ -14,7 +14,7 @@ import ctypes
 
 import torch
 
-from ._lib import lib, check, stream_ptr, on_device
+from ._lib import lib, check, nodes, stream_ptr, on_device
 
 _MAX = 96   # ADDER_SGD_BATCH_MAX
 
@@ -86,8 +86,8 @@ class SGD(torch.optim.SGD):
         return loss
 
 
-_ADAMW_MAX, _ADAMW8_MAX, STATE_BLOCK = 96, 64, 256   # ADDER_ADAMW_BATCH_MAX, ADDER_ADAMW_8BIT_BATCH_MAX, ADDER_STATE_BLOCK
-_PIECE = 1 << 30                                     # values of one entry of the kernel's table; longer tensors take several
+STATE_BLOCK = 256   # ADDER_STATE_BLOCK
+_PIECE = 1 << 30    # values of one entry of the kernel's table; longer tensors take several
 _CODES = {"exp_avg": torch.int8, "exp_avg_sq": torch.uint8}
 
 
@@ -141,7 +141,7 @@ class AdamW(torch.optim.AdamW):
         self.state_bits, self.min_8bit_size = state_bits, min_8bit_size
 
     @staticmethod
-    def _kernel_takes(group, params, grads):
+    def _kernel_takes(group, params):
         if group["amsgrad"] or group["maximize"]:
             return False
         lr = group["lr"]
@@ -149,11 +149,13 @@ class AdamW(torch.optim.AdamW):
             return False
         if any(isinstance(b, torch.Tensor) for b in group["betas"]):
             return False
-        both = params + grads
-        types = list(map(_dtype, params))
-        return (set(map(_layout, both)) == {torch.strided} and set(map(_device, both)) == {params[0].device} and params[0].is_cuda
-                and set(types) <= _ADAMW_TYPES.keys() and types == list(map(_dtype, grads)) and all(map(_contiguous, both))
-                and list(map(_numel, params)) == list(map(_numel, grads)))
+        dev = params[0].device
+        for p in params:
+            g = p.grad
+            if not (p.is_cuda and p.device == dev and g.device == dev and p.dtype in _ADAMW_TYPES and g.dtype == p.dtype
+                    and p.layout == g.layout == torch.strided and p.is_contiguous() and g.is_contiguous()):
+                return False
+        return True
 
     def _new_state(self, p, step):
         state = self.state[p]
@@ -199,9 +201,12 @@ class AdamW(torch.optim.AdamW):
             params = [p for p in group["params"] if p.grad is not None]
             if not params:
                 continue
-            grads = [p.grad for p in params]
-            if self._kernel_takes(group, params, grads):
-                self._kernel_step(group, params, grads)
+            if self._kernel_step(group, params):
+                continue
+            if self._kernel_takes(group, params):
+                self._make_states(group, params)
+                if not self._kernel_step(group, params):
+                    raise RuntimeError("AdamW: the state does not fit its parameters")
             elif self.state_bits == 8:
                 raise RuntimeError("state_bits=8 needs contiguous float32 or bfloat16 GPU parameters with gradients of their type, on one device")
             else:
@@ -222,90 +227,45 @@ class AdamW(torch.optim.AdamW):
                 self.param_groups = kept
         return loss
 
-    def _counted(self, group, params):
-        """The states of ``params`` with their step counts as the kernel wants them: an int or, with ``capturable``, a tensor on the
-        device that the parameters of one count share (one tiny launch counts them all)."""
-        of, capturable = self.state, group["capturable"]
+    def _make_states(self, group, params):
+        """The states of ``params`` as the kernel wants them: moments as float32 or codes, and the step count as an int or, with
+        ``capturable``, as a tensor on the device that the parameters of one count share (one tiny launch counts them all)."""
+        of, capturable, dev = self.state, group["capturable"], params[0].device
+        fresh = torch.zeros((), dtype=torch.float32, device=dev) if capturable else 0
+        for p in params:
+            state = of[p] or self._new_state(p, fresh)
+            step = state["step"]
+            if not capturable:
+                state["step"] = int(step)
+            elif not (isinstance(step, torch.Tensor) and step.is_cuda and step.dtype == torch.float32):
+                state["step"] = torch.tensor(float(step), dtype=torch.float32, device=dev)
+            for name in _CODES:   # (what torch.optim.AdamW made for a group that it had to take before)
+                if state[name].dtype not in (torch.float32, _CODES[name]):
+                    state[name] = state[name].float()
+        if capturable:   # parameters without a gradient now do not count on with the others
+            used = {id(of[p]["step"]) for p in params}
+            for p in group["params"]:
+                if p.grad is None and of.get(p) and id(of[p]["step"]) in used:
+                    of[p]["step"] = of[p]["step"].clone()
+
+    def _kernel_step(self, group, params):
+        """The launches of one step, by csrc/nodes.cpp: False, and nothing done, where something is not as the kernels want it."""
+        lr, capturable, of = group["lr"], group["capturable"], self.state
+        if group["amsgrad"] or group["maximize"]:
+            return False
         states = [of[p] for p in params]
         if not all(states):
-            fresh = torch.zeros((), dtype=torch.float32, device=params[0].device) if capturable else 0
-            states = [state or self._new_state(p, fresh) for p, state in zip(params, states)]
-        if capturable:
-            for state in states:
-                if not (isinstance(state["step"], torch.Tensor) and state["step"].is_cuda and state["step"].dtype == torch.float32):
-                    state["step"] = torch.tensor(float(state["step"]), dtype=torch.float32, device=params[0].device)
-            if len(params) < len(group["params"]):   # parameters without a gradient now do not count on with the others
-                used = {id(state["step"]) for state in states}
-                for p in group["params"]:
-                    if p.grad is None and of.get(p) and id(of[p]["step"]) in used:
-                        of[p]["step"] = of[p]["step"].clone()
-        else:
-            for state in states:
-                if type(state["step"]) is not int:
-                    state["step"] = int(state["step"])
-        return states
-
-    def _kernel_step(self, group, params, grads):
-        capturable, dev = group["capturable"], params[0].device
-        states = self._counted(group, params)
-        batches = {}   # one launch per step count and storage type of the parameter and of its state: almost always one
-        for p, g, state in zip(params, grads, states):
-            step, m = state["step"], state["exp_avg"]
-            if m.dtype not in _STATE_TYPES:   # what torch.optim.AdamW made for a group that it had to take before
-                for name in _CODES:
-                    state[name] = state[name].float()
-                m = state["exp_avg"]
-            batches.setdefault((id(step) if capturable else step, p.dtype, m.dtype), []).append((p, g, state))
-        lr = group["lr"]
-        lr_ptr, lr_val = (lr.data_ptr(), 0.0) if isinstance(lr, torch.Tensor) else (None, float(lr))
+            return False
+        if capturable and len(params) < len(group["params"]):
+            used = {id(state["step"]) for state in states}
+            if any(p.grad is None and of.get(p) and id(of[p]["step"]) in used for p in group["params"]):
+                return False
+        rate, rate_at = lr, 0
+        if isinstance(lr, torch.Tensor):
+            if not (lr.is_cuda and lr.dtype == torch.float32 and lr.numel() == 1 and lr.device == params[0].device):
+                return False
+            rate, rate_at = 0.0, lr.data_ptr()
         b1, b2 = group["betas"]
-        with on_device(dev):
-            stream = stream_ptr(dev)
-            advanced = {}
-            for (_, dtype, kept), batch in batches.items():
-                corr, count, step = None, 0, batch[0][2]["step"]
-                if capturable:
-                    if id(step) not in advanced:
-                        corr = advanced[id(step)] = torch.empty(2, dtype=torch.float32, device=dev)
-                        check(lib.adder_adamw_advance(step.data_ptr(), b1, b2, corr.data_ptr(), stream), "adder_adamw_advance")
-                    corr = advanced[id(step)].data_ptr()
-                else:
-                    count = step + 1
-                _adamw_launches(batch, kept == torch.int8,
-                                (lr_ptr, lr_val, b1, b2, group["eps"], group["weight_decay"], count, corr, _ADAMW_TYPES[dtype], stream))
-                if not capturable:
-                    for _, _, state in batch:
-                        state["step"] = count
-
-
-_dtype, _device, _layout = torch.Tensor.dtype.__get__, torch.Tensor.device.__get__, torch.Tensor.layout.__get__
-_numel, _contiguous, _data_ptr = torch.Tensor.numel, torch.Tensor.is_contiguous, torch.Tensor.data_ptr
-_STATE_TYPES = (torch.float32, torch.int8)
-
-
-def _adamw_launches(batch, coded, tail):
-    params, grads, states = zip(*batch)
-    call, most, what = ((lib.adder_adamw_step_8bit, _ADAMW8_MAX, "adder_adamw_step_8bit") if coded
-                        else (lib.adder_adamw_step, _ADAMW_MAX, "adder_adamw_step"))
-    sizes = list(map(_numel, params))
-    moments = [[state["exp_avg"] for state in states], [state["exp_avg_sq"] for state in states]]
-    fits, types = [sizes, sizes], list(_CODES.values()) if coded else [torch.float32, torch.float32]
-    if coded:
-        moments += [[state["exp_avg_scale"] for state in states], [state["exp_avg_sq_scale"] for state in states]]
-        fits += [[-(-n // STATE_BLOCK) for n in sizes]] * 2
-        types += [torch.float32, torch.float32]
-    for tensors, fit, dtype in zip(moments, fits, types):   # (a state that was set by hand, or a parameter that was replaced)
-        if not (list(map(_numel, tensors)) == fit and set(map(_dtype, tensors)) == {dtype} and all(map(_contiguous, tensors))
-                and set(map(_device, tensors)) == {params[0].device}):
-            raise RuntimeError(f"{what}: the state does not fit its parameter")
-    columns = [list(map(_data_ptr, c)) for c in (params, grads, *moments)]
-    if min(sizes) == 0 or max(sizes) > _PIECE:   # empty tensors have no entry, long ones several
-        e = params[0].element_size()
-        widths = [e, e, 1, 1, 4 / STATE_BLOCK, 4 / STATE_BLOCK] if coded else [e, e, 4, 4]
-        cut = [(t, at) for t, n in enumerate(sizes) for at in range(0, n, _PIECE)]
-        columns = [[c[t] + int(at * w) for t, at in cut] for c, w in zip(columns, widths)]
-        sizes = [min(_PIECE, sizes[t] - at) for t, at in cut]
-    for i in range(0, len(sizes), most):
-        k = min(most, len(sizes) - i)
-        pointers, longs = ctypes.c_void_p * k, ctypes.c_long * k
-        check(call(k, *[pointers(*c[i:i + k]) for c in columns], longs(*sizes[i:i + k]), *tail), what)
+        if isinstance(b1, torch.Tensor) or isinstance(b2, torch.Tensor):
+            return False
+        return nodes.adamw_step(params, states, capturable, rate, rate_at, b1, b2, group["eps"], group["weight_decay"], _PIECE)
