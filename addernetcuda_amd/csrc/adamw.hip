@@ -47,11 +47,14 @@ __device__ __forceinline__ int tensor_of(const B &b, int count) {
     return lo;
 }
 
+// The root and the reciprocal are the plain instructions (one unit in the last place of the update each).  The root's takes moments below
+// the smallest normal float for zero; beside an eps of less than a root of those it is the exact one.
 __device__ __forceinline__ float adamw_value(float p, float g, float &m, float &v, const AdamWArgs &a, const Corrections &c,
                                              float rate, float decay) {
     m = fmaf(a.b1, m, a.one_b1 * g);
     v = fmaf(a.b2, v, a.one_b2 * g * g);
-    return fmaf(-rate * c.c1, m / fmaf(sqrtf(v), c.c2, a.eps), p * decay);
+    const float root = a.eps < 1e-12f ? sqrtf(v) : __builtin_amdgcn_sqrtf(v);
+    return fmaf(-rate * c.c1, m * __builtin_amdgcn_rcpf(fmaf(root, c.c2, a.eps)), p * decay);
 }
 
 static constexpr int kAdamWThreads = 256, kAdamWChunk = 4 * kAdamWThreads;
@@ -119,27 +122,22 @@ __global__ __launch_bounds__(kAdamWThreads) void adamw_kernel(const AdamWBatch b
     st4(v, left, vv);
 }
 
-// Largest of the 64 lanes' values; not a number where one of them is none (or infinite).
-__device__ __forceinline__ float wave_scale(float v) {
-    const bool bad = !(v < __builtin_inff());
-    float t = v;
-    t = fmaxf(t, dpp_row_move<0xB1>(t));
-    t = fmaxf(t, dpp_row_move<0x4E>(t));
-    t = fmaxf(t, dpp_row_move<0x141>(t));
-    t = fmaxf(t, dpp_row_move<0x140>(t));
-    t = fmaxf(t, __shfl_xor(t, 16, 64));
-    t = fmaxf(t, __shfl_xor(t, 32, 64));
-    return __any(bad) ? __builtin_nanf("") : t;
+// The larger of two values, not a number where one of them is none (fmaxf passes over it)
+__device__ __forceinline__ float maximum(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+// Largest of the 64 lanes' values; not a number where one of them is none or infinite.
+__device__ __forceinline__ float wave_scale(float t) {
+    t = maximum(t, dpp_row_move<0xB1>(t));
+    t = maximum(t, dpp_row_move<0x4E>(t));
+    t = maximum(t, dpp_row_move<0x141>(t));
+    t = maximum(t, dpp_row_move<0x140>(t));
+    t = maximum(t, __shfl_xor(t, 16, 64));
+    t = maximum(t, __shfl_xor(t, 32, 64));
+    return t < __builtin_inff() ? t : __builtin_nanf("");
 }
 
-// What divides by a scale: up * inv * value is value / scale, where 1 / scale on its own may be infinite.  A scale of zero, or
-// one that is not a number, gives codes of zero.
-struct Inverse { float up, inv; };
-__device__ __forceinline__ Inverse inverse(float scale) {
-    const float up = scale < 0x1p-64f ? 0x1p64f : 1.f;
-    const float s = scale * up;
-    return Inverse{up, s > 0.f ? 1.f / s : 0.f};
-}
+// What a value is multiplied with towards its code.  Scales of zero, below the smallest normal float, or not a number: codes of zero.
+__device__ __forceinline__ float inverse(float scale) { return scale >= 0x1p-126f ? 1.f / scale : 0.f; }
 
 __device__ __forceinline__ float first_moment(int q, float s) {
     const float r = (float)q;
@@ -168,31 +166,25 @@ __global__ __launch_bounds__(kAdamWThreads) void adamw_8bit_kernel(const AdamW8B
     ld4(g, left, gv);
     uint32_t mq = ld_codes(b.m[t] + i, left), vq = ld_codes(b.v[t] + i, left);
     float mtop = 0.f, vtop = 0.f;
-    bool bad_m = false, bad_v = false;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < 4; ++e) {   // (beside the tensor: zeros)
         mv[e] = first_moment((int8_t)(mq >> (8 * e)), ms);
         vv[e] = second_moment((vq >> (8 * e)) & 255u, vs);
         pv[e] = adamw_value(pv[e], gv[e], mv[e], vv[e], a, c, rate, decay);
-        if (e < left) {
-            mtop = fmaxf(mtop, fabsf(mv[e]));
-            vtop = fmaxf(vtop, vv[e]);
-            bad_m = bad_m || mv[e] != mv[e];   // (fmaxf passes over what is not a number)
-            bad_v = bad_v || vv[e] != vv[e];
-        }
+        mtop = maximum(mtop, fabsf(mv[e]));
+        vtop = maximum(vtop, vv[e]);
     }
     st4(p, left, pv);
-    const float nan = __builtin_nanf("");
-    const float ns = wave_scale(bad_m ? nan : mtop), ws = wave_scale(bad_v ? nan : vtop);
-    const Inverse im = inverse(ns), iv = inverse(ws);
+    const float ns = wave_scale(mtop), ws = wave_scale(vtop);
+    const float im = inverse(ns), iv = inverse(ws);
     mq = vq = 0;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const float rm = rintf(127.f * sqrtf(fabsf(mv[e]) * im.up * im.inv));
-        const float rv = rintf(255.f * sqrtf(sqrtf(vv[e] * iv.up * iv.inv)));
-        const int qm = (int)fminf(rm, 127.f), qv = (int)fminf(fmaxf(rv, vv[e] > 0.f ? 1.f : 0.f), 255.f);
-        mq |= (uint32_t)((mv[e] < 0.f ? -qm : qm) & 255) << (8 * e);
-        vq |= (uint32_t)qv << (8 * e);
+        // (the plain root instruction, one unit in the last place: of a number from 0 to 1, towards a code)
+        const float rm = copysignf(rintf(127.f * __builtin_amdgcn_sqrtf(fabsf(mv[e]) * im)), mv[e]);
+        const float rv = rintf(255.f * __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(vv[e] * iv)));
+        mq = __builtin_amdgcn_cvt_pk_u8_f32(rm < 0.f ? rm + 256.f : rm, e, mq);   // (two's complement)
+        vq = __builtin_amdgcn_cvt_pk_u8_f32(fmaxf(rv, vv[e] > 0.f ? 1.f : 0.f), e, vq);
     }
     st_codes(b.m[t] + i, left, mq);
     st_codes(b.v[t] + i, left, vq);

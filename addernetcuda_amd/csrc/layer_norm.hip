@@ -86,15 +86,16 @@ __global__ __launch_bounds__(G > kNormFwdThreads ? G : kNormFwdThreads) void lay
 }
 
 // The workgroups walk over the rows and keep the columns' sums of dy * h and dy of their rows in registers; at the end the
-// groups of a workgroup add theirs through LDS and it writes one slab of 2 D floats, which launch_fold_columns adds up: no
-// atomics, the same bits every run.
+// lanes of a wave that hold the same columns add theirs, then the waves through LDS, and the workgroup writes one slab of 2 D
+// floats, which launch_fold_columns adds up: no atomics, the same bits every run.
 template <class T, class W, int G>
 __global__ __launch_bounds__(G > kNormBwdThreads ? G : kNormBwdThreads) void layer_norm_bwd_kernel(
     const T *__restrict__ dy, long dy_stride, const T *__restrict__ x, long x_stride, const W *__restrict__ w,
     const float *__restrict__ mean, const float *__restrict__ rstd, T *__restrict__ gx, float *__restrict__ part, long rows, int D) {
     constexpr int V = Chunk<T>::n, C = kNormChunks<T>, THREADS = G > kNormBwdThreads ? G : kNormBwdThreads, PER = THREADS / G;
     __shared__ float lds[16];
-    __shared__ __align__(16) float fold[PER > 1 ? THREADS * 8 : 4];
+    constexpr int LANES = G < 64 ? G : 64, SHARE = G < 64 ? THREADS / 64 : PER;   // lanes of a wave with columns of their own; LDS copies of the columns
+    __shared__ __align__(16) float fold[SHARE > 1 ? SHARE * G * kNormValues : 4];
     const int lane = threadIdx.x % G;
     const float inv = 1.f / (float)D;
     float wv[C][V], sw[C][V], sb[C][V];
@@ -144,28 +145,40 @@ __global__ __launch_bounds__(G > kNormBwdThreads ? G : kNormBwdThreads) void lay
     float *slab = part + (size_t)blockIdx.x * 2 * D;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
+        float (&t)[C][V] = k ? sb : sw;
 #pragma unroll
         for (int c = 0; c < C; ++c)
 #pragma unroll
-            for (int q = 0; q < V; q += 4) {   // four columns of every lane at a time
-                const int at = (lane + c * G) * V + q;
-                float t[4];
+            for (int e = 0; e < V; ++e)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) t[e] = k ? sb[c][q + e] : sw[c][q + e];
-                if constexpr (PER > 1) {
-                    __syncthreads();
-                    *reinterpret_cast<float4 *>(fold + threadIdx.x * 4) = make_float4(t[0], t[1], t[2], t[3]);
-                    __syncthreads();
-                    if (threadIdx.x < G) {
-#pragma unroll 4
-                        for (int i = 1; i < PER; ++i) {
-                            const float4 o = *reinterpret_cast<const float4 *>(fold + (threadIdx.x + i * G) * 4);
-                            t[0] += o.x; t[1] += o.y; t[2] += o.z; t[3] += o.w;
-                        }
-                    }
+                for (int off = LANES; off < 64; off *= 2) t[c][e] += __shfl_xor(t[c][e], off, 64);
+        if constexpr (SHARE == 1) {
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int q = 0; q < V; q += 4) {
+                    const float u[4] = {t[c][q], t[c][q + 1], t[c][q + 2], t[c][q + 3]};
+                    const int at = (lane + c * G) * V + q;
+                    store_part(slab + (size_t)k * D + at, D - at, u);
                 }
-                if (threadIdx.x < G) store_part(slab + (size_t)k * D + at, D - at, t);
+        } else {
+            const int copy = threadIdx.x / (G < 64 ? 64 : G);
+            if (k) __syncthreads();
+            if ((threadIdx.x & 63) < LANES)
+#pragma unroll
+                for (int c = 0; c < C; ++c)
+#pragma unroll
+                    for (int q = 0; q < V; q += 4)
+                        *reinterpret_cast<float4 *>(fold + copy * (G * kNormValues) + (lane + c * G) * V + q) =
+                            make_float4(t[c][q], t[c][q + 1], t[c][q + 2], t[c][q + 3]);
+            __syncthreads();
+            for (int i = threadIdx.x; i < D; i += THREADS) {
+                float u = fold[i];
+#pragma unroll
+                for (int r = 1; r < SHARE; ++r) u += fold[r * (G * kNormValues) + i];
+                slab[(size_t)k * D + i] = u;
             }
+        }
     }
 }
 
@@ -243,8 +256,8 @@ __global__ __launch_bounds__(256) void layer_norm_wide_columns_kernel(const T *_
     slab[(size_t)D + i] = sb;
 }
 
-// 64 columns and up to sixteen shares of the slabs a workgroup
-static constexpr int kFoldColumns = 64, kFoldShares = 16;
+// 32 columns and 32 shares of the slabs a workgroup
+static constexpr int kFoldColumns = 32, kFoldShares = 32;
 template <class T>
 __global__ __launch_bounds__(kFoldColumns *kFoldShares) void fold_columns_kernel(const float *__restrict__ part, int parts, int K,
                                                                                  long cols, const FoldOut out) {
@@ -291,7 +304,7 @@ int layer_norm_bwd_parts(long rows, int D, int type) {
     (void)type;
     if (D > kNormRegisterWidth) return (int)(rows < 64 ? rows : 64);
     const int G = norm_lanes(D);
-    const long per = G > kNormBwdThreads ? 1 : kNormBwdThreads / G, need = ceil_div_l(rows, per), most = 512;
+    const long per = G > kNormBwdThreads ? 1 : kNormBwdThreads / G, need = ceil_div_l(rows, per), most = 256;
     return (int)(need < most ? need : most);
 }
 

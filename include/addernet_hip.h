@@ -537,8 +537,9 @@ ADDER_API int adder_layer_norm_bwd(const void *dy, long dy_row_stride, const voi
  *   adder_adamw_step_8bit: moments as 8-bit codes, count <= ADDER_ADAMW_8BIT_BATCH_MAX.  ADDER_STATE_BLOCK neighbouring values
  *     share a scale s, the largest magnitude among them: m = sign(q) s (q / 127)^2 with q in -127 .. 127 (signed char),
  *     v = s (q / 255)^4 with q in 0 .. 255 (unsigned char), to the nearest in that root's scale; a second moment that is not
- *     zero keeps a code that is not.  The parameter is updated with the moments before they are rounded.  A block with a
- *     moment that is infinite or not a number becomes not a number as a whole.  Scales: ceil(n / ADDER_STATE_BLOCK) floats.
+ *     zero keeps a code that is not, and scales below the smallest normal float have codes of zero otherwise.  The parameter is
+ *     updated with the moments before they are rounded.  A block with a moment that is infinite or not a number becomes not a
+ *     number as a whole.  Scales: ceil(n / ADDER_STATE_BLOCK) floats.
  *   adder_adamw_advance: step_device[0] += 1, and corrections[0], [1] = 1 / (1 - beta1^step), 1 / sqrt(1 - beta2^step).
  *   adder_state_values: the values that n codes (signed: of a first moment) and their scales stand for. */
 #define ADDER_ADAMW_BATCH_MAX 96
