@@ -39,14 +39,14 @@ __global__ __launch_bounds__(256) void product_join_kernel(const ProductArgs p) 
 // A launch's time is estimated for every shape of tile and number of shares of k, and the least is taken.  The workgroups run in rounds
 // of as many as the card holds, each steps * step + tile us: steps of 64 (float32: 32) values of k; `step` measured with every compute
 // unit full (8192 x 8192 x 1024 and 8192^3), less in proportion where fewer workgroups share one, but at least `alone` (1024^3); `tile` the first
-// loads, the epilogue and the start.  Shares of k pay for their sums' way through memory (5 TB/s both ways) and the join's launch.
+// loads, the epilogue and the start, once more where a second output is written.  Shares of k pay for their sums' way through memory (5 TB/s both ways) and the join's launch.
 static constexpr int kCUs = 256;
 struct Shape { int bm, bn, per_cu; float step, alone, tile; };
 //                                       8192^3, TFLOP/s
 static constexpr Shape kStreamShapes[] = {
-    {256, 256, 1, 1.55f, 1.55f, 8.f},    // 1320
+    {256, 256, 1, 1.55f, 1.55f, 10.f},   // 1320
     {128, 256, 1, 0.9f, 0.9f, 4.f},      // 1155
-    {128, 128, 2, 0.87f, 0.5f, 3.5f},    // 1155
+    {128, 128, 2, 0.87f, 0.65f, 3.5f},   // 1155
     {64, 64, 2, 0.38f, 0.2f, 1.5f},      //  640
 };
 template <class T>
@@ -59,6 +59,7 @@ constexpr Shape kStagedShapes<float>[] = {
     {128, 128, 2, 2.3f, 1.9f, 3.5f},     //  220
     {64, 64, 3, 1.25f, 0.65f, 1.5f},     //  155
     {128, 128, 1, 1.25f, 1.25f, 3.5f},   //  200
+    {64, 64, 1, 0.53f, 0.53f, 2.5f},     //  145
 };
 static constexpr int kSplitMax = 16;
 
@@ -76,7 +77,7 @@ static float rows_us(long M, long N, long K) {
 }
 
 template <int N>
-static ProductPlan plan_product(const Shape (&shapes)[N], int bk, long M, long N_, long K) {
+static ProductPlan plan_product(const Shape (&shapes)[N], int bk, long M, long N_, long K, int outputs) {
     static constexpr int kSplits[] = {1, 2, 3, 4, 6, 8, 12, kSplitMax};
     ProductPlan best{0, 1, K, 0.f};
     const long steps = ceil_div_l(K, bk);
@@ -88,10 +89,10 @@ static ProductPlan plan_product(const Shape (&shapes)[N], int bk, long M, long N
             const long share = ceil_div_l(steps, splits);
             const float groups = tiles * splits;
             const float slots = (float)(kCUs * h.per_cu), whole = floorf(groups / slots), rest = groups - whole * slots;
-            float us = 3.f + whole * (share * h.step + h.tile);
+            float us = 3.f + whole * (share * h.step + h.tile * outputs);
             if (rest > 0.f) {
                 const float shared = h.step * ceilf(rest / kCUs) / h.per_cu;
-                us += share * (shared > h.alone ? shared : h.alone) + h.tile;
+                us += share * (shared > h.alone ? shared : h.alone) + h.tile * outputs;
             }
             if (splits > 1) us += 3.f + (float)M * (float)N_ * splits * 8.f / 5e6f;
             if (best.us == 0.f || us < best.us) {
@@ -103,8 +104,8 @@ static ProductPlan plan_product(const Shape (&shapes)[N], int bk, long M, long N
     return best;
 }
 template <class T>
-static ProductPlan plan_staged(long M, long N, long K) { return plan_product(kStagedShapes<T>, sizeof(T) == 4 ? 32 : 64, M, N, K); }
-static ProductPlan plan_stream(long M, long N, long K) { return plan_product(kStreamShapes, 64, M, N, K); }
+static ProductPlan plan_staged(long M, long N, long K, int outputs) { return plan_product(kStagedShapes<T>, sizeof(T) == 4 ? 32 : 64, M, N, K, outputs); }
+static ProductPlan plan_stream(long M, long N, long K, int outputs) { return plan_product(kStreamShapes, 64, M, N, K, outputs); }
 
 // Loads of 16 aligned bytes fit a bfloat16 operand: base and rows begin at multiples of them, and what a tile's last load brings
 // beside the operand it can be told from by k alone (k along: rows of whole loads) or is never stored (k across).  A tile's rows
@@ -117,16 +118,20 @@ static size_t split_bytes(const ProductPlan &p, long M, long N) { return p.split
 
 template <class T>
 size_t product_workspace_bytes(long M, long N, long K) {
-    const size_t staged = split_bytes(plan_staged<T>(M, N, K), M, N);
-    if (sizeof(T) == 4) return staged;
-    const size_t stream = split_bytes(plan_stream(M, N, K), M, N);
-    return stream > staged ? stream : staged;
+    size_t most = 0;   // whichever kernel strides and alignments leave, with and without a second output
+    for (int outputs = 1; outputs <= 2; ++outputs) {
+        const size_t staged = split_bytes(plan_staged<T>(M, N, K, outputs), M, N), stream = sizeof(T) == 2 ? split_bytes(plan_stream(M, N, K, outputs), M, N) : 0;
+        if (staged > most) most = staged;
+        if (stream > most) most = stream;
+    }
+    return most;
 }
 
 template <class T>
 int launch_product(const Product &q, void *ws, hipStream_t s) {
     const bool stream = sizeof(T) == 2 && fits_stream(q.a, q.lda, q.a_across, q.K) && fits_stream(q.b, q.ldb, q.b_across, q.K);
-    ProductPlan plan = stream ? plan_stream(q.M, q.N, q.K) : plan_staged<T>(q.M, q.N, q.K);
+    const int outputs = q.pre ? 2 : 1;
+    ProductPlan plan = stream ? plan_stream(q.M, q.N, q.K, outputs) : plan_staged<T>(q.M, q.N, q.K, outputs);
     const bool rows = !q.a_across && !q.b_across && rows_us<T>(q.M, q.N, q.K) < plan.us;
     if (rows) plan = ProductPlan{0, 1, q.K, 0.f};
     const ProductArgs p{q.a, q.b, q.bias, q.res, q.out, q.pre, static_cast<float *>(ws), q.lda, q.ldb, q.ldr, q.M, q.N, q.K, plan.k_share, 0, 0,

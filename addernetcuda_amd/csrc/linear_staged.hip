@@ -44,8 +44,8 @@ struct Staged {
     long step;
 
     // chunk i of this thread: its row (across: of k) and its first column (along: of k) in the tile
-    static __device__ __forceinline__ int row_of(int i) { return (threadIdx.x + i * THREADS) / row_loads; }
-    static __device__ __forceinline__ int column_of(int i) { return (threadIdx.x + i * THREADS) % row_loads * E; }
+    static __device__ __forceinline__ int row_of(int i) { return (threadIdx.x % THREADS + i * THREADS) / row_loads; }
+    static __device__ __forceinline__ int column_of(int i) { return (threadIdx.x % THREADS + i * THREADS) % row_loads * E; }
     static __device__ __forceinline__ bool edge(long all, long row0) { return ACROSS && row0 + R > all; }
 
     __device__ __forceinline__ void setup(const T *p, long ld, long all, long row0, long k_begin) {
@@ -151,15 +151,17 @@ __device__ __forceinline__ void sum_again(const ProductArgs &p, f32x4 (&acc)[TM]
 }
 
 // WM x WN waves of TM x TN tiles of 16 x 16.  AHEAD: tiles of k in registers or on their way there (small ones are multiplied faster than the
-// next arrives).  BUFFERS = 2: one barrier a tile, and the next is split and stored while this one is multiplied.
-template <class T, int WM, int WN, int TM, int TN, int AHEAD, int BUFFERS, bool AA, bool BA>
-__global__ __launch_bounds__(WM *WN * 64, 2) void product_staged_kernel(const ProductArgs p) {
+// next arrives).  BUFFERS = 2: one barrier a tile, and the next is split and stored while this one is multiplied.  KG: groups of so many
+// waves that share the tiles of k, each with buffers of its own; their sums are added through LDS.
+template <class T, int WM, int WN, int TM, int TN, int AHEAD, int BUFFERS, int KG, bool AA, bool BA>
+__global__ __launch_bounds__(WM *WN * 64 * KG, KG == 1 ? 2 : 1) void product_staged_kernel(const ProductArgs p) {
     constexpr int BM = WM * TM * 16, BN = WN * TN * 16, BK = kStagedK<T>, P = kStagedPlanes<T>, THREADS = WM * WN * 64;
     typedef Staged<T, BM, AA, THREADS> SA;
     typedef Staged<T, BN, BA, THREADS> SB;
     constexpr int BYTES = P * (SA::Tile::bytes + SB::Tile::bytes);
-    extern __shared__ __align__(16) char lds[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    extern __shared__ __align__(16) char all_lds[];
+    const int lane = threadIdx.x & 63, wave = (threadIdx.x % THREADS) >> 6, group = __builtin_amdgcn_readfirstlane(threadIdx.x / THREADS);
+    char *lds = all_lds + group * (BUFFERS * BYTES);
     const int wm = (wave % WM) * (TM * 16), wn = (wave / WM) * (TN * 16);
     int tm, tn;
     tile_of(blockIdx.x, p.tiles_m, p.tiles_n, tm, tn);
@@ -200,19 +202,22 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void product_staged_kernel(const Pr
         }
     };
     const int full = (int)((k_end - k_begin) / BK), left = (int)(k_end - k_begin - (long)full * BK);
+    // this group's whole tiles: `mine` of them from `first` on, in `turns` turns of all groups
+    const int turns = (full + KG - 1) / KG, first = group * turns < full ? group * turns : full - 1;
+    const int mine = full - group * turns < 0 ? 0 : full - group * turns < turns ? full - group * turns : turns;
     auto walk = [&](auto edge) {   // over the whole tiles of k
         constexpr bool EDGE = decltype(edge)::value;
         SA sa;
         SB sb;
-        sa.setup(a, p.lda, p.M, m0, k_begin);
-        sb.setup(b, p.ldb, p.N, n0, k_begin);
+        sa.setup(a, p.lda, p.M, m0, k_begin + (long)first * BK);
+        sb.setup(b, p.ldb, p.N, n0, k_begin + (long)first * BK);
         typename SA::Values va[AHEAD];
         typename SB::Values vb[AHEAD];
         int next = 0;
         auto load = [&](int d) {
             ++next;
-            sa.template load<EDGE>(va[d], next < full);
-            sb.template load<EDGE>(vb[d], next < full);
+            sa.template load<EDGE>(va[d], next < mine);
+            sb.template load<EDGE>(vb[d], next < mine);
         };
         auto store = [&](char *tile, int d) {
             SA::store(tile, va[d]);
@@ -224,19 +229,20 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void product_staged_kernel(const Pr
             store(lds, 0);
             load(0);
             int buf = 0;
-            for (int t = 0; t < full; t += AHEAD)
+            for (int t = 0; t < turns; t += AHEAD)
 #pragma unroll
                 for (int d = 0; d < AHEAD; ++d) {
-                    if (t + d >= full) break;
+                    if (t + d >= turns) break;
                     __syncthreads();   // this tile is there; the other buffer has been read
-                    multiply(lds + buf * BYTES, [&]() {
-                        store(lds + (buf ^ 1) * BYTES, (d + 1) % AHEAD);
-                        load((d + 1) % AHEAD);
-                    });
+                    if (KG == 1 || t + d < mine)
+                        multiply(lds + buf * BYTES, [&]() {
+                            store(lds + (buf ^ 1) * BYTES, (d + 1) % AHEAD);
+                            load((d + 1) % AHEAD);
+                        });
                     buf ^= 1;
                 }
         } else {
-            for (int t = 0; t < full; ++t) {
+            for (int t = 0; t < turns; ++t) {
                 __syncthreads();
                 store(lds, 0);
                 __syncthreads();
@@ -249,17 +255,40 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void product_staged_kernel(const Pr
         if (SA::edge(p.M, m0) || SB::edge(p.N, n0)) walk(Flag<true>{});
         else walk(Flag<false>{});
     }
-    if (left) {
+    if (left) {   // (by the last group)
         typename SA::Values va;
         typename SB::Values vb;
         const long k = k_begin + (long)full * BK;
-        SA::load_last(va, a, p.lda, p.M, m0, k, left);
-        SB::load_last(vb, b, p.ldb, p.N, n0, k, left);
+        if (group == KG - 1) {
+            SA::load_last(va, a, p.lda, p.M, m0, k, left);
+            SB::load_last(vb, b, p.ldb, p.N, n0, k, left);
+        }
         __syncthreads();
-        SA::store(lds, va);
-        SB::store(lds + P * SA::Tile::bytes, vb);
+        if (group == KG - 1) {
+            SA::store(lds, va);
+            SB::store(lds + P * SA::Tile::bytes, vb);
+        }
         __syncthreads();
-        multiply(lds, [] {});
+        if (group == KG - 1) multiply(lds, [] {});
+    }
+    if constexpr (KG > 1) {
+        static_assert((KG - 1) * WM * WN * TM * TN * 64 * sizeof(f32x4) <= KG * BUFFERS * BYTES, "the groups' sums fit");
+        f32x4 *sums = reinterpret_cast<f32x4 *>(all_lds) + ((group - 1) * WM * WN + wave) * (TM * TN * 64) + lane;
+        __syncthreads();
+        if (group > 0) {
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) sums[(i * TN + j) * 64] = acc[i][j];
+        }
+        __syncthreads();
+        if (group > 0) return;
+#pragma unroll
+        for (int g = 1; g < KG; ++g)
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] += sums[(g * WM * WN * TM * TN + i * TN + j) * 64];
     }
     if constexpr (P == 3) {
         bool finite = true;
@@ -274,28 +303,29 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void product_staged_kernel(const Pr
     finish_wave<T, TM, TN>(p, acc, m0 + wm, n0 + wn, lane);
 }
 
-template <class T, int WM, int WN, int TM, int TN, int AHEAD, int BUFFERS, bool AA, bool BA>
+template <class T, int WM, int WN, int TM, int TN, int AHEAD, int BUFFERS, int KG, bool AA, bool BA>
 static int launch_staged_layout(ProductArgs p, hipStream_t s) {
-    constexpr int BM = WM * TM * 16, BN = WN * TN * 16, bytes = BUFFERS * kStagedPlanes<T> * (BM + BN) * kStagedK<T> * 2;
+    constexpr int BM = WM * TM * 16, BN = WN * TN * 16, bytes = KG * BUFFERS * kStagedPlanes<T> * (BM + BN) * kStagedK<T> * 2;
     p.tiles_m = (int)ceil_div_l(p.M, BM);
     p.tiles_n = (int)ceil_div_l(p.N, BN);
-    if (int rc = allow_dynamic_lds<&product_staged_kernel<T, WM, WN, TM, TN, AHEAD, BUFFERS, AA, BA>>(bytes)) return rc;
-    hipLaunchKernelGGL((product_staged_kernel<T, WM, WN, TM, TN, AHEAD, BUFFERS, AA, BA>), dim3((unsigned)p.tiles_m * p.tiles_n, p.splits),
-                       dim3(WM * WN * 64), bytes, s, p);
+    if (int rc = allow_dynamic_lds<&product_staged_kernel<T, WM, WN, TM, TN, AHEAD, BUFFERS, KG, AA, BA>>(bytes)) return rc;
+    hipLaunchKernelGGL((product_staged_kernel<T, WM, WN, TM, TN, AHEAD, BUFFERS, KG, AA, BA>), dim3((unsigned)p.tiles_m * p.tiles_n, p.splits),
+                       dim3(WM * WN * 64 * KG), bytes, s, p);
     return check_launch();
 }
-template <class T, int WM, int WN, int TM, int TN, int AHEAD, int BUFFERS>
+template <class T, int WM, int WN, int TM, int TN, int AHEAD, int BUFFERS, int KG = 1>
 static int launch_staged(const ProductArgs &p, bool a_across, bool b_across, hipStream_t s) {
-    if (a_across) return launch_staged_layout<T, WM, WN, TM, TN, AHEAD, BUFFERS, true, true>(p, s);
-    return b_across ? launch_staged_layout<T, WM, WN, TM, TN, AHEAD, BUFFERS, false, true>(p, s)
-                    : launch_staged_layout<T, WM, WN, TM, TN, AHEAD, BUFFERS, false, false>(p, s);
+    if (a_across) return launch_staged_layout<T, WM, WN, TM, TN, AHEAD, BUFFERS, KG, true, true>(p, s);
+    return b_across ? launch_staged_layout<T, WM, WN, TM, TN, AHEAD, BUFFERS, KG, false, true>(p, s)
+                    : launch_staged_layout<T, WM, WN, TM, TN, AHEAD, BUFFERS, KG, false, false>(p, s);
 }
 template <>
 int launch_product_staged<float>(const ProductArgs &p, bool a_across, bool b_across, StagedShape shape, hipStream_t s) {
     switch (shape) {
         case StagedShape::large: return launch_staged<float, 2, 2, 4, 4, 1, 1>(p, a_across, b_across, s);
         case StagedShape::small: return launch_staged<float, 2, 2, 2, 2, 3, 2>(p, a_across, b_across, s);
-        default: return launch_staged<float, 2, 4, 4, 2, 1, 2>(p, a_across, b_across, s);
+        case StagedShape::alone: return launch_staged<float, 2, 4, 4, 2, 1, 2>(p, a_across, b_across, s);
+        default: return launch_staged<float, 2, 2, 2, 2, 3, 2, 2>(p, a_across, b_across, s);
     }
 }
 template <>

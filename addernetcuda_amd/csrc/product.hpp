@@ -271,8 +271,8 @@ __device__ __forceinline__ void tile_of(int id, int tiles_m, int tiles_n, int &t
 // Launches of the tiled kernels; p has everything but its tiles
 enum class StreamShape { big, wide, mid, small };   // 256 x 256, 128 x 256, 128 x 128, 64 x 64 results a workgroup
 int launch_product_stream(ProductArgs p, bool a_across, bool b_across, StreamShape shape, hipStream_t s);
-// 128 x 128, 64 x 64, and (float32) 128 x 128 by twice as many waves, for launches that leave a compute unit one workgroup
-enum class StagedShape { large, small, alone };
+// 128 x 128, 64 x 64, and (float32) both by twice as many waves, for launches that leave a compute unit one workgroup
+enum class StagedShape { large, small, alone, pair };
 template <class T>
 int launch_product_staged(const ProductArgs &p, bool a_across, bool b_across, StagedShape shape, hipStream_t s);
 template <class T>
