@@ -31,8 +31,9 @@ __device__ __forceinline__ void split(float x, float y, uint32_t (&o)[3]) {
 
 // One operand's tile: loads of 16 bytes, of 4 floats or 8 bfloat16 that lie side by side.  The loads of the main loop have no branch
 // around them (a wait behind one would have to be for all that is under way): rows and columns that do not exist are other ones
-// again, whose results are not stored; with k across the rows, a chunk that ends beyond the last column is read value by value (EDGE).
-// Only the last tile of a k that is no whole number of tiles holds zeros, and is read on its own.
+// again, whose results are not stored; with k across the rows, the chunk that ends beyond the last column is read as the last whole
+// chunk and shifted on its way to LDS (EDGE; below a chunk's columns: NARROW, no main loop).  Only the last tile of a k that is no whole
+// number of tiles holds zeros, and is read on its own.
 template <class T, int R, bool ACROSS, int THREADS>
 struct Staged {
     static constexpr int E = Chunk<T>::n, BK = kStagedK<T>, P = kStagedPlanes<T>;
@@ -40,13 +41,14 @@ struct Staged {
     static constexpr int row_loads = Tile::row_chunks * 8 / E, per = R * BK / E / THREADS;
     struct Values { uint4 v[per]; };
     const T *at[per];   // of the next tile
-    int most[per];      // across: a chunk's last column that exists, counted from its first
+    int shift[per];     // across: how many columns before its place a chunk was read
     long step;
 
     // chunk i of this thread: its row (across: of k) and its first column (along: of k) in the tile
     static __device__ __forceinline__ int row_of(int i) { return (threadIdx.x % THREADS + i * THREADS) / row_loads; }
     static __device__ __forceinline__ int column_of(int i) { return (threadIdx.x % THREADS + i * THREADS) % row_loads * E; }
     static __device__ __forceinline__ bool edge(long all, long row0) { return ACROSS && row0 + R > all; }
+    static __device__ __forceinline__ bool narrow(long all) { return ACROSS && all < E; }
 
     __device__ __forceinline__ void setup(const T *p, long ld, long all, long row0, long k_begin) {
         step = ACROSS ? BK * ld : BK;
@@ -54,31 +56,17 @@ struct Staged {
         for (int i = 0; i < per; ++i) {
             const int r = row_of(i), c = column_of(i);
             if constexpr (ACROSS) {
-                const long col = row0 + c < all ? row0 + c : all - 1, left = all - 1 - col;
+                const long col = row0 + c + E <= all ? row0 + c : all - E;
                 at[i] = p + (k_begin + r) * ld + col;
-                most[i] = left < E - 1 ? (int)left : E - 1;
+                shift[i] = row0 + c < all ? (int)(row0 + c - col) : 0;
             } else {
                 at[i] = p + (row0 + r < all ? row0 + r : all - 1) * ld + k_begin + c;
             }
         }
     }
-    template <bool EDGE>
     __device__ __forceinline__ void load(Values &t, bool more) {
 #pragma unroll
-        for (int i = 0; i < per; ++i) {
-            if constexpr (EDGE && ACROSS) {
-                uint32_t w[4];
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const T *q = at[i] + (e < most[i] ? e : most[i]);
-                    if constexpr (E == 4) w[e] = __float_as_uint(*q);
-                    else w[e / 2] = e & 1 ? w[e / 2] | (uint32_t)*q << 16 : *q;
-                }
-                t.v[i] = make_uint4(w[0], w[1], w[2], w[3]);
-            } else {
-                t.v[i] = load_raw(at[i]);
-            }
-        }
+        for (int i = 0; i < per; ++i) t.v[i] = load_raw(at[i]);
         const long go = more ? step : 0;   // (past the last whole tile: that one again, unused)
 #pragma unroll
         for (int i = 0; i < per; ++i) at[i] += go;
@@ -93,7 +81,26 @@ struct Staged {
             else t.v[i] = load_raw_part(p + (row0 + r) * ld + k + c, rows <= 0 ? 0 : left - c);
         }
     }
-    static __device__ __forceinline__ void store(char *tile, const Values &t) {
+    static __device__ __forceinline__ uint4 shifted(uint4 v, int by) {   // values by.. in the first places
+        if constexpr (E == 8) {
+            v.x = by & 1 ? (v.x >> 16) | (v.y << 16) : v.x;
+            v.y = by & 1 ? (v.y >> 16) | (v.z << 16) : v.y;
+            v.z = by & 1 ? (v.z >> 16) | (v.w << 16) : v.z;
+            v.w = by & 1 ? v.w >> 16 : v.w;
+            by >>= 1;
+        }
+        if (by & 1) v = make_uint4(v.y, v.z, v.w, v.w);
+        if (by & 2) v = make_uint4(v.z, v.w, v.w, v.w);
+        return v;
+    }
+    template <bool EDGE>
+    __device__ __forceinline__ void store(char *tile, Values t) const {
+        if constexpr (EDGE && ACROSS)
+#pragma unroll
+            for (int i = 0; i < per; ++i) t.v[i] = shifted(t.v[i], shift[i]);
+        put(tile, t);
+    }
+    static __device__ __forceinline__ void put(char *tile, const Values &t) {
 #pragma unroll
         for (int i = 0; i < per; ++i) {
             const int r = row_of(i), c = column_of(i) / E;
@@ -216,18 +223,22 @@ __global__ __launch_bounds__(WM *WN * 64 * KG, KG == 1 ? 2 : 1) void product_sta
         int next = 0;
         auto load = [&](int d) {
             ++next;
-            sa.template load<EDGE>(va[d], next < mine);
-            sb.template load<EDGE>(vb[d], next < mine);
+            sa.load(va[d], next < mine);
+            sb.load(vb[d], next < mine);
         };
         auto store = [&](char *tile, int d) {
-            SA::store(tile, va[d]);
-            SB::store(tile + P * SA::Tile::bytes, vb[d]);
+            sa.template store<EDGE>(tile, va[d]);
+            sb.template store<EDGE>(tile + P * SA::Tile::bytes, vb[d]);
         };
 #pragma unroll
-        for (int d = 0; d < AHEAD; ++d) load(d);
+        for (int d = 0; d < AHEAD; ++d) {
+            load(d);
+            asm volatile("" ::: "memory");   // (in this order: the loop waits for the oldest)
+        }
         if constexpr (BUFFERS == 2) {
             store(lds, 0);
             load(0);
+            asm volatile("" ::: "memory");
             int buf = 0;
             for (int t = 0; t < turns; t += AHEAD)
 #pragma unroll
@@ -251,26 +262,28 @@ __global__ __launch_bounds__(WM *WN * 64 * KG, KG == 1 ? 2 : 1) void product_sta
             }
         }
     };
-    if (full) {
-        if (SA::edge(p.M, m0) || SB::edge(p.N, n0)) walk(Flag<true>{});
-        else walk(Flag<false>{});
-    }
-    if (left) {   // (by the last group)
+    auto single = [&](long k, int left) {   // one tile on its own, by the last group
         typename SA::Values va;
         typename SB::Values vb;
-        const long k = k_begin + (long)full * BK;
         if (group == KG - 1) {
             SA::load_last(va, a, p.lda, p.M, m0, k, left);
             SB::load_last(vb, b, p.ldb, p.N, n0, k, left);
         }
         __syncthreads();
         if (group == KG - 1) {
-            SA::store(lds, va);
-            SB::store(lds + P * SA::Tile::bytes, vb);
+            SA::put(lds, va);
+            SB::put(lds + P * SA::Tile::bytes, vb);
         }
         __syncthreads();
         if (group == KG - 1) multiply(lds, [] {});
+    };
+    if (SA::narrow(p.M) || SB::narrow(p.N)) {
+        for (int t = 0; t < full; ++t) single(k_begin + (long)t * BK, BK);
+    } else if (full) {
+        if (SA::edge(p.M, m0) || SB::edge(p.N, n0)) walk(Flag<true>{});
+        else walk(Flag<false>{});
     }
+    if (left) single(k_begin + (long)full * BK, left);
     if constexpr (KG > 1) {
         static_assert((KG - 1) * WM * WN * TM * TN * 64 * sizeof(f32x4) <= KG * BUFFERS * BYTES, "the groups' sums fit");
         f32x4 *sums = reinterpret_cast<f32x4 *>(all_lds) + ((group - 1) * WM * WN + wave) * (TM * TN * 64) + lane;
