@@ -9,6 +9,7 @@ namespace adder {
 
 static const long kMaxElems = 0x7fffffffL;          // of a tensor that one kernel index of 32 bits walks over
 static const double kMaxWide = 1099511627776.0;     // of the others: 2^40
+static const int kMaxWidth = 1 << 26;               // of a row: the folds of columns are launches of 32 threads a column
 
 static bool known(int type) { return type == ADDER_TYPE_F32 || type == ADDER_TYPE_BF16; }
 static size_t size_of(int type) { return type == ADDER_TYPE_BF16 ? 2 : 4; }
@@ -24,7 +25,7 @@ static int check_workspace(const void *ws, size_t have, size_t need) {
 
 static int check_linear(long rows, int in, int out, int type) {
     if (rows <= 0 || in <= 0 || out <= 0 || !known(type)) return ADDER_ERR_BAD_SHAPE;
-    if (wide(rows, in) || wide(rows, out) || wide(in, out)) return ADDER_ERR_TOO_LARGE;
+    if (wide(rows, in) || wide(rows, out) || wide(in, out) || in > kMaxWidth || out > kMaxWidth) return ADDER_ERR_TOO_LARGE;
     // (workgroups of 256 threads and at least 64 x 64 results; a launch has at most 2^32 threads)
     const double r = rows / 64 + 1, i = in / 64 + 1, o = out / 64 + 1, most = 16777216.0;
     return r * o > most || r * i > most || i * o > most ? ADDER_ERR_TOO_LARGE : ADDER_OK;
@@ -168,7 +169,7 @@ int adder_layer_norm_fwd(const void *x, long x_row_stride, const void *weight, c
     if (rows <= 0 || width <= 0 || !known(type) || !known(weight_type) || !(eps >= 0.f) || bad_stride(x_row_stride, rows, width))
         return ADDER_ERR_BAD_SHAPE;
     if (type == ADDER_TYPE_F32 && weight_type != type) return ADDER_ERR_UNSUPPORTED;
-    if (wide(rows, width) || wide(rows, x_row_stride)) return ADDER_ERR_TOO_LARGE;
+    if (width > kMaxWidth || wide(rows, width) || wide(rows, x_row_stride)) return ADDER_ERR_TOO_LARGE;
     const size_t nw = size_of(weight_type) * (size_t)width, nr = sizeof(float) * (size_t)rows;
     const Span outs[] = {{y, size_of(type) * (size_t)rows * width}, {save_mean, nr}, {save_rstd, nr}};
     const Span ins[] = {{x, span(rows, x_row_stride, width, type)}, {weight, nw}, {bias, nw}};
@@ -187,7 +188,7 @@ int adder_layer_norm_fwd(const void *x, long x_row_stride, const void *weight, c
 int adder_layer_norm_bwd_workspace_bytes(long rows, int width, int type, size_t *bytes) {
     if (!bytes) return ADDER_ERR_NULL_POINTER;
     if (rows <= 0 || width <= 0 || !known(type)) return ADDER_ERR_BAD_SHAPE;
-    if (wide(rows, width)) return ADDER_ERR_TOO_LARGE;
+    if (width > kMaxWidth || wide(rows, width)) return ADDER_ERR_TOO_LARGE;
     *bytes = whole(sizeof(float) * 2 * (size_t)layer_norm_bwd_parts(rows, width, type) * width);
     return ADDER_OK;
 }
@@ -200,7 +201,7 @@ int adder_layer_norm_bwd(const void *dy, long dy_row_stride, const void *x, long
         bad_stride(dy_row_stride, rows, width))
         return ADDER_ERR_BAD_SHAPE;
     if (type == ADDER_TYPE_F32 && weight_type != type) return ADDER_ERR_UNSUPPORTED;
-    if (wide(rows, width) || wide(rows, x_row_stride) || wide(rows, dy_row_stride)) return ADDER_ERR_TOO_LARGE;
+    if (width > kMaxWidth || wide(rows, width) || wide(rows, x_row_stride) || wide(rows, dy_row_stride)) return ADDER_ERR_TOO_LARGE;
     const bool sums = gweight || gbias;
     size_t need = 0;
     if (int rc = adder_layer_norm_bwd_workspace_bytes(rows, width, type, &need)) return rc;

@@ -67,6 +67,7 @@ struct ProductPlan { int shape, splits; long k_share; float us; };
 
 // The kernel for few rows likewise: workgroups of 16 columns and 16, 32 or 64 rows, whose waves take turns along k, 128 bytes of every
 // row at a time (us each, with the rows' share of the second-level caches: 4096 x 4096, full workgroups)
+static constexpr long kRowsMost = 1024, kRowsColumns = 1L << 25;   // within which the estimate finds it the fastest, and its launch has few enough threads
 template <class T>
 static float rows_us(long M, long N, long K) {
     static constexpr float kTurn[2][3] = {{1.2f, 2.1f, 1.95f}, {1.75f, 2.5f, 2.2f}};
@@ -132,7 +133,7 @@ int launch_product(const Product &q, void *ws, hipStream_t s) {
     const bool stream = sizeof(T) == 2 && fits_stream(q.a, q.lda, q.a_across, q.K) && fits_stream(q.b, q.ldb, q.b_across, q.K);
     const int outputs = q.pre ? 2 : 1;
     ProductPlan plan = stream ? plan_stream(q.M, q.N, q.K, outputs) : plan_staged<T>(q.M, q.N, q.K, outputs);
-    const bool rows = !q.a_across && !q.b_across && rows_us<T>(q.M, q.N, q.K) < plan.us;
+    const bool rows = !q.a_across && !q.b_across && q.M <= kRowsMost && q.N <= kRowsColumns && rows_us<T>(q.M, q.N, q.K) < plan.us;
     if (rows) plan = ProductPlan{0, 1, q.K, 0.f};
     const ProductArgs p{q.a, q.b, q.bias, q.res, q.out, q.pre, static_cast<float *>(ws), q.lda, q.ldb, q.ldr, q.M, q.N, q.K, plan.k_share, 0, 0,
                         plan.splits, q.act};

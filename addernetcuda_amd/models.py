@@ -22,6 +22,10 @@ concatenated in front of the input, densenet.py:9-21), transitions of BatchNorm 
 channels - 2x2 average pooling (densenet.py:24-33), BatchNorm - ReLU - 4x4 average pooling - linear classifier
 (densenet.py:67-68, 92-95).  Its layers have channel counts that are multiples of 12, not of 16.
 
+``token_mlp`` is no network of the reference: a small one that shows linear layers beside adder layers.  An adder layer cuts a 32x32
+image into 64 patches; blocks of two residual MLPs (layer norm - linear with GELU - linear with the shortcut), over the
+patches and over the channels, follow.  ``fused=False`` builds the same from torch's ``nn.LayerNorm`` and ``nn.Linear``.
+
 All take ``adder2d_cls`` to build the same network around another implementation of the layer (the tests do
 this with their CPU reference), and ``fused=False`` to build it from stock ``nn.BatchNorm2d`` / ``nn.ReLU``
 modules exactly as the reference's model files do -- the adder layers are then the only thing that differs
@@ -36,6 +40,8 @@ import torch.nn.functional as F
 
 from . import adder as _adder
 from .bn_act import BatchNormAct2d
+from .layer_norm import LayerNorm
+from .linear import LinearAct
 from .unit import adder_bn_act
 from .resnet20 import StemConv2d   # nn.Conv2d with the same parameters; forward and weight gradient through the tiled kernels
 
@@ -363,3 +369,47 @@ def DenseNet201(**kwargs):
 def DenseNet161(**kwargs):
     """densenet.py:105-106."""
     return DenseNet((6, 12, 36, 24), growth_rate=48, **kwargs)
+
+
+# ---- linear layers beside adder layers --------------------------------------------------------------------
+class ResidualMLP(nn.Module):
+    """``x + fc2(gelu(fc1(norm(x))))`` over the last dimension: three kernels (the shortcut rides on the second product)."""
+
+    def __init__(self, width, hidden, fused=True):
+        super().__init__()
+        self.fused = fused
+        self.norm = LayerNorm(width) if fused else nn.LayerNorm(width)
+        self.fc1 = LinearAct(width, hidden, act="gelu") if fused else nn.Linear(width, hidden)
+        self.fc2 = LinearAct(hidden, width) if fused else nn.Linear(hidden, width)
+
+    def forward(self, x):
+        if self.fused:
+            return self.fc2(self.fc1(self.norm(x)), residual=x)
+        return x + self.fc2(F.gelu(self.fc1(self.norm(x))))
+
+
+class TokenMLP(nn.Module):
+    """An adder layer (``patch`` x ``patch`` taps, stride ``patch``) and BatchNorm, then ``layers`` pairs of residual MLPs, over the
+    patches and over the channels; layer norm, the patches' mean, a linear classifier.  For 32x32 images."""
+
+    def __init__(self, width=128, layers=4, patch=4, num_classes=10, image=32, adder2d_cls=None, fused=True, **adder_kw):
+        super().__init__()
+        make = adder2d_cls or _adder.adder2d
+        tokens = (image // patch) ** 2
+        self.stem = make(3, width, kernel_size=patch, stride=patch, padding=0, bias=False, **adder_kw)
+        self.bn = _bn(width, False, fused)
+        self.over_tokens = nn.ModuleList([ResidualMLP(tokens, 2 * tokens, fused) for _ in range(layers)])
+        self.over_channels = nn.ModuleList([ResidualMLP(width, 4 * width, fused) for _ in range(layers)])
+        self.norm = LayerNorm(width) if fused else nn.LayerNorm(width)
+        self.classifier = LinearAct(width, num_classes) if fused else nn.Linear(width, num_classes)
+
+    def forward(self, x):
+        x = self.bn(self.stem(x)).flatten(2)   # (images, channels, patches)
+        for tokens, channels in zip(self.over_tokens, self.over_channels):
+            x = channels(tokens(x).transpose(1, 2)).transpose(1, 2)
+        return self.classifier(self.norm(x.transpose(1, 2)).mean(1))
+
+
+def token_mlp(**kwargs):
+    """``TokenMLP`` with its defaults: 128 channels, 64 patches, four pairs of MLPs."""
+    return TokenMLP(**kwargs)

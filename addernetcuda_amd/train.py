@@ -15,6 +15,7 @@ processes are needed.  What it adds: the training step of a full batch runs as o
     python -m addernetcuda_amd.train --synthetic 4096 --epochs 2
     python -m addernetcuda_amd.train --data cifar10.npz --epochs 400 --output-dir models/
     python -m addernetcuda_amd.train --data cifar10.npz --resume models/addernet.pt --eval-only
+    python -m addernetcuda_amd.train --arch token_mlp --optimizer adamw8bit --lr 0.002 --weight-decay 0.05
     (npz keys: x_train (N,32,32,3) or (N,3,32,32) uint8, y_train (N,), x_test, y_test)
 """
 import argparse
@@ -165,12 +166,13 @@ def train_one_epoch(net, opt, x_u8, y, batch, generator=None, graphed=None, bf16
     return torch.stack(losses).mean().item()
 
 
-ARCHS = ("resnet20", "vgg_small", "densenet_cifar", "resnet50")
+ARCHS = ("resnet20", "vgg_small", "densenet_cifar", "resnet50", "token_mlp")
+OPTIMIZERS = ("sgd", "adamw", "adamw8bit")
 
 
 def build_network(arch, eta, num_classes=10):
     """The reference's networks for 32x32 inputs (main.py:66 builds resnet20; vgg.py, densenet.py and resnet50.py
-    are its other model files)."""
+    are its other model files), and ``token_mlp``: an adder layer with residual MLPs behind it."""
     if arch == "resnet20":
         from addernetcuda_amd.resnet20 import resnet20
         return resnet20(eta=eta, num_classes=num_classes)
@@ -178,6 +180,18 @@ def build_network(arch, eta, num_classes=10):
         raise ValueError(f"unknown architecture {arch!r}: one of {ARCHS}")
     from addernetcuda_amd import models
     return getattr(models, arch)(eta=eta, num_classes=num_classes)
+
+
+def build_optimizer(name, params, lr, weight_decay=None):
+    """main.py:67's SGD by default (torch.optim.SGD's rule and state, all parameters in one launch), or AdamW with its moments in 32 or in
+    8 bits; the counts of its steps live on the device, for the captured step."""
+    from addernetcuda_amd.optim import SGD, AdamW
+    if name == "sgd":
+        return SGD(params, lr=lr, momentum=0.9, weight_decay=5e-4 if weight_decay is None else weight_decay)
+    if name not in OPTIMIZERS:
+        raise ValueError(f"unknown optimizer {name!r}: one of {OPTIMIZERS}")
+    return AdamW(params, lr=lr, weight_decay=1e-2 if weight_decay is None else weight_decay, capturable=True,
+                 state_bits=8 if name == "adamw8bit" else 32)
 
 
 def run(args):
@@ -191,8 +205,7 @@ def run(args):
         net.load_state_dict(torch.load(args.resume, map_location=dev, weights_only=True))
     # the learning rate lives on the device so that the captured step sees each epoch's value
     lr_now = torch.tensor(float(args.lr), device=dev)
-    from addernetcuda_amd.optim import SGD   # torch.optim.SGD's rule and state, all parameters in one launch
-    opt = SGD(net.parameters(), lr=lr_now, momentum=0.9, weight_decay=5e-4)
+    opt = build_optimizer(args.optimizer, net.parameters(), lr_now, args.weight_decay)
     if args.eval_only:   # the reference's test.py: load a checkpoint, one pass over the test split
         test_loss, acc = evaluate(net, *data["test"], args.test_batch_size, args.bf16_activations)
         print(f"test loss {test_loss:.4f}  accuracy {acc:.4f}", flush=True)
@@ -240,6 +253,8 @@ def parse_args(argv=None):
                    help="optional mode: activations stored as bfloat16 between the layers (float32 weights, float32 / "
                         "float64 accumulation in the adder kernels); the default, like the reference, is float32 throughout")
     p.add_argument("--seed", type=int, default=0)
+    p.add_argument("--optimizer", choices=OPTIMIZERS, default="sgd", help="sgd as in main.py:67, or AdamW with its state in 32 or 8 bits")
+    p.add_argument("--weight-decay", type=float, default=None, help="5e-4 for sgd (main.py:67), 1e-2 for adamw")
     p.add_argument("--arch", choices=ARCHS, default="resnet20", help="network (main.py:66 trains resnet20)")
     return p.parse_args(argv)
 

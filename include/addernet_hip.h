@@ -489,8 +489,8 @@ ADDER_API int adder_sgd_momentum_step_f32(int count, float *const *params, const
  * [layers] Layers beside the adder layers.  No counterpart in the reference, which leaves its Linear layers (vgg.py) and its
  * optimizer to the framework.
  * `type` says how the tensors given as void * are stored; sums, statistics and moments are 32 bits in either.  Matrices are
- * rows of neighbouring values; a row stride (in values) is 0, or at least the row's width.  Any alignment.  Tensors may have
- * more than 2^31 - 1 elements.  Nothing depends on the order in which workgroups run: the same bits every time.
+ * rows of neighbouring values, 2^26 at most; a row stride (in values) is 0, or at least the row's width.  Any alignment.  Tensors
+ * may have more than 2^31 - 1 elements.  Nothing depends on the order in which workgroups run: the same bits every time.
  * ---------------------------------------------------------------------- */
 typedef enum adder_type { ADDER_TYPE_F32 = 0, ADDER_TYPE_BF16 = 1 } adder_type;
 

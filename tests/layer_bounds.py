@@ -97,6 +97,8 @@ def within(actual, expected, what):
     a = actual.detach().double().cpu()
     assert a.shape == value.shape, f"{what}: shape {tuple(a.shape)}, expected {tuple(value.shape)}"
     far = (a - value).abs()
+    beyond = value.abs() > torch.finfo(actual.dtype).max   # (what the type cannot hold is infinite)
+    far = torch.where(beyond & (a == value.sign() * float("inf")), torch.zeros_like(far), far)
     bad = ~(far <= off + 1e-30)
     if bad.any():
         at = tuple(torch.nonzero(bad)[0].tolist())

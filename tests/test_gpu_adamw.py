@@ -275,6 +275,17 @@ def test_more_than_one_piece(gpu, monkeypatch):
             assert torch.equal(a, b)
 
 
+def test_a_step_is_a_change_in_place(gpu):
+    from addernetcuda_amd.optim import AdamW
+    p = torch.nn.Parameter(torch.ones(8, device="cuda"))
+    opt = AdamW([p], lr=0.1)
+    (p * p).sum().backward()
+    y = (p * p).sum()
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
 def test_refusals(gpu):
     from addernetcuda_amd import optim
     p = torch.nn.Parameter(torch.ones(5000, device="cuda"))

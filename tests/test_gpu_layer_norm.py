@@ -129,6 +129,18 @@ def test_gradients_against_differences(gpu):
 
 
 @pytest.mark.parametrize("kind", KINDS, ids=IDS)
+def test_second_derivatives_are_an_error_and_vmap_works(kind, gpu):
+    from addernetcuda_amd.layer_norm import layer_norm
+    x, w, b, _ = make(6, 40, kind)
+    x.requires_grad_(True)
+    gx, = torch.autograd.grad(layer_norm(x, w, b).float().square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiate twice"):
+        gx.sum().backward()
+    if kind[0] == torch.float32:
+        assert torch.allclose(torch.func.vmap(lambda t: layer_norm(t, w, b))(x.detach()), layer_norm(x.detach(), w, b), atol=1e-5)
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=IDS)
 def test_same_bits_every_time_and_on_other_streams(kind, gpu):
     from addernetcuda_amd.layer_norm import layer_norm
     x, w, b, dy = make(3000, 264, kind)

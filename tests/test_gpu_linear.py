@@ -143,6 +143,48 @@ def test_infinite_and_nan_stay_where_they_are(rows, k, n, dtype, gpu):
     assert torch.equal(y[rest][:, keep], clean.float()[rest][:, keep])
 
 
+@pytest.mark.parametrize("rows,k,n", [(2, 40, 33), (200, 72, 64), (300, 300, 300)])
+def test_float32_over_its_whole_range(rows, k, n, gpu):
+    """Values that round up to infinity in bfloat16, products of the largest with the smallest, values whose parts lie below the smallest
+    normal number: as good as in the middle of the range."""
+    from addernetcuda_amd.linear import linear_act
+    x, w, b, _, dy = make(rows, k, n, torch.float32)
+    for sx, sw in ((2.0 ** 100, 2.0 ** -100), (2.0 ** -60, 2.0 ** 50), (2.0 ** -115, 2.0 ** 110)):
+        xs, ws, bs = x * sx, w * sw, b * (sx * sw)
+        if sx > 1:
+            xs[0, 0], ws[:, 0] = 3.4e38, 2.0 ** -130
+        want = B.linear(xs, ws, bs, None, dy, "none")
+        leaves = [t.requires_grad_(True) for t in (xs, ws, bs)]
+        y = linear_act(*leaves)
+        names = ("gx", "gw", "gb")
+        # (what is lost below the smallest normal float, 2^-126 a term at most)
+        for name, t, terms in zip(("y",) + names, (y,) + torch.autograd.grad(y, leaves, dy), (k, n, rows, rows)):
+            value, off = want[name]
+            size = {"y": 1, "gx": float(dy.abs().max()), "gw": float(dy.abs().max()), "gb": 1}[name]
+            big = {"y": max(sx, sw), "gx": 1, "gw": 1, "gb": 1}[name]
+            B.within(t, (value, off + terms * 2.0 ** -126 * max(1.0, size) * max(1.0, big) * 4), name)
+
+
+def test_what_torch_does_with_calls_it_does_with_these(gpu):
+    """A gradient of a gradient is an error, vmap and autocast work, a parameter that changes between forward and backward is noticed."""
+    from addernetcuda_amd.linear import linear_act, LinearAct
+    x, w, b, r, dy = make(6, 24, 16, torch.float32)
+    x.requires_grad_(True)
+    gx, = torch.autograd.grad(linear_act(x, w, b, act="gelu").square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiate twice"):
+        gx.sum().backward()
+    each = torch.func.vmap(lambda t: linear_act(t, w, b, act="silu"))(x.detach().view(3, 2, 24))
+    assert torch.allclose(each.view(6, 16), linear_act(x.detach(), w, b, act="silu"), atol=1e-5)
+    layer = LinearAct(24, 16, act="relu").cuda()
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        assert layer(x.detach().bfloat16()).dtype == torch.bfloat16
+    y = layer(x)
+    with torch.no_grad():
+        layer.weight.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
 def test_gradients_against_differences(gpu):
     """f(t + e d) - f(t - e d) = 2 e |grad f|^2 / |grad f| along d = grad f / |grad f|; float32 sums of 2^15 outputs carry 1e-5 of
     their size at most, the step's third-order term less."""

@@ -23,7 +23,7 @@ def test_linear_refuses():
         assert fwd(**bad) == -1
     for bad in ({"rows": 0}, {"k": 0}, {"n": -1}, {"act": 4}, {"act": -1}, {"t": 2}, {"ldx": 63}, {"ldx": -64}, {"r": A[4], "ldr": 31}):
         assert fwd(**bad) == -2
-    assert fwd(rows=1 << 40) == -3 and fwd(ldx=1 << 40) == -3 and fwd(rows=1 << 30, k=64, n=1 << 20) == -3
+    assert fwd(rows=1 << 40) == -3 and fwd(ldx=1 << 40) == -3 and fwd(rows=1 << 30, k=64, n=1 << 20) == -3 and fwd(n=(1 << 26) + 1) == -3
     for bad in ({"y": A[0]}, {"y": A[1]}, {"pre": A[2]}, {"r": A[2], "ldr": 32}, {"bias": A[2]}):
         assert fwd(**bad) == -6
     bwd = lambda dy=A[0], ldd=32, pre=A[1], x=A[2], ldx=64, w=A[3], gx=A[4], gw=A[5], gb=A[6], act=2, rows=8, k=64, n=32, t=0, ws=A[7], nb=1 << 30: \
@@ -122,3 +122,33 @@ def test_adamw_on_the_cpu_is_torchs():
     with pytest.raises(RuntimeError, match="state_bits=8"):
         o8 = AdamW([a], state_bits=8)
         o8.step()
+
+
+def test_token_mlp_on_the_cpu_is_the_network_of_torchs_modules():
+    from addernetcuda_amd.models import token_mlp
+    stem = lambda i, o, kernel_size, stride, padding, bias: torch.nn.Conv2d(i, o, kernel_size, stride, padding, bias=bias)
+    a, b = (token_mlp(width=32, layers=1, adder2d_cls=stem, fused=fused) for fused in (True, False))
+    b.load_state_dict(a.state_dict())
+    x = torch.randn(4, 3, 32, 32)
+    assert torch.allclose(a.eval()(x), b.eval()(x), atol=1e-6)
+
+
+def test_optimizers_of_the_training_script():
+    from addernetcuda_amd import optim, train
+    p = [torch.nn.Parameter(torch.ones(3))]
+    assert isinstance(train.build_optimizer("sgd", p, 0.1), optim.SGD) and train.build_optimizer("sgd", p, 0.1).defaults["weight_decay"] == 5e-4
+    assert train.build_optimizer("adamw8bit", p, 0.1, 0.3).state_bits == 8 and train.build_optimizer("adamw", p, 0.1).state_bits == 32
+    with pytest.raises(ValueError, match="unknown optimizer"):
+        train.build_optimizer("adam", p, 0.1)
+
+
+def test_wrapped_and_transformed_calls_take_torchs_operators():
+    """vmap, forward-mode derivatives, tracing and second derivatives are torch's business (here on the CPU)."""
+    from addernetcuda_amd.linear import linear_act
+    from addernetcuda_amd.layer_norm import layer_norm
+    x, w, b = torch.randn(4, 3, 8, dtype=torch.float64), torch.randn(5, 8, dtype=torch.float64), torch.randn(5, dtype=torch.float64)
+    f = lambda t: linear_act(t, w, b, act="silu")
+    assert torch.allclose(torch.func.vmap(f)(x), f(x))
+    _, tangent = torch.func.jvp(f, (x,), (torch.ones_like(x),))
+    assert tangent.shape == (4, 3, 5)
+    assert torch.autograd.gradgradcheck(lambda t: layer_norm(t, torch.ones(8, dtype=torch.float64)), (x[0].requires_grad_(True),))
