@@ -121,8 +121,11 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
     static Variable forward(AutogradContext *ctx, const Variable &x, const Variable &w, const Maybe &has_bias, const Maybe &has_residual, int64_t act) {
         const Tensor bias = has_bias.value_or(Tensor()), residual = has_residual.value_or(Tensor());
         const bool wx = x.requires_grad(), ww = w.requires_grad(), wb = bias.defined() && bias.requires_grad();
+        // what the activation's derivative is taken from: the values before it, or ReLU's own result where nothing was added to it
+        const bool keep = act != ADDER_ACT_NONE && (wx || ww || wb), own = act == ADDER_ACT_RELU && !residual.defined();
         Tensor pre;
-        const Tensor y = linear_forward(x, w, bias, residual, act, act != ADDER_ACT_NONE && (wx || ww || wb) ? &pre : nullptr);
+        const Tensor y = linear_forward(x, w, bias, residual, act, keep && !own ? &pre : nullptr);
+        if (keep && own) pre = y;
         ctx->save_for_backward({ww ? x : Variable(), wx ? w : Variable(), pre});
         ctx->saved_data["act"] = act;
         ctx->saved_data["x"] = x.sizes().vec();

@@ -37,7 +37,8 @@ def _torch_linear_act(x, weight, bias, residual, act):
 def linear_act(x, weight, bias=None, residual=None, act="none"):
     """``act(x @ weight.T + bias) + residual`` with ``x`` (..., in_features), ``weight`` (out_features, in_features), ``bias``
     (out_features) or None, ``residual`` None or of any shape that broadcasts to the result's, and ``act`` one of "none", "relu",
-    "gelu" (by the error function) and "silu"."""
+    "gelu" (by the error function) and "silu".  As with torch's, the backward of "relu" without a residual reads the result: it is not
+    to be edited in place before that."""
     code = ACTS.get(act)
     if code is None:
         raise ValueError(f"act must be one of {tuple(ACTS)}, got {act!r}")

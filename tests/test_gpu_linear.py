@@ -253,3 +253,21 @@ def test_refusals(gpu):
         linear_act(x, w.cpu())
     with pytest.raises(RuntimeError, match="does not broadcast"):
         linear_act(x, w, b, r[:, :5])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,k,n", [(1, 5, 3), (33, 24, 17), (256, 128, 64)])
+def test_relu_reads_its_own_result(gpu, rows, k, n, dtype):
+    """Its gradients are those of the plain product for dy where the result is not zero: the same launches of the same numbers
+    (where the result is no number, dy's; torch's does the same).  An edit of the result is noticed."""
+    from addernetcuda_amd.linear import linear_act
+    x, w, b, _, dy = make(rows, k, n, dtype)
+    x[0, 0] = float("nan")
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    own, product = linear_act(*leaves, act="relu"), linear_act(*leaves)
+    dz = torch.where(own.detach() == 0, torch.zeros_like(dy), dy)
+    for g, h in zip(torch.autograd.grad(own, leaves, dy, retain_graph=True), torch.autograd.grad(product, leaves, dz)):
+        assert torch.equal(g.nan_to_num(7), h.nan_to_num(7))
+    own.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        own.sum().backward()
