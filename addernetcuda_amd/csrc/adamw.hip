@@ -125,14 +125,15 @@ __global__ __launch_bounds__(kAdamWThreads) void adamw_kernel(const AdamWBatch b
 // The larger of two values, not a number where one of them is none (fmaxf passes over it)
 __device__ __forceinline__ float maximum(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
-// Largest of the 64 lanes' values; not a number where one of them is none or infinite.
-__device__ __forceinline__ float wave_scale(float t) {
+// Largest of G neighbouring lanes' values (32 or 64); not a number where one of them is none or infinite.
+template <int G>
+__device__ __forceinline__ float lanes_scale(float t) {
     t = maximum(t, dpp_row_move<0xB1>(t));
     t = maximum(t, dpp_row_move<0x4E>(t));
     t = maximum(t, dpp_row_move<0x141>(t));
     t = maximum(t, dpp_row_move<0x140>(t));
     t = maximum(t, __shfl_xor(t, 16, 64));
-    t = maximum(t, __shfl_xor(t, 32, 64));
+    if constexpr (G == 64) t = maximum(t, __shfl_xor(t, 32, 64));
     return t < __builtin_inff() ? t : __builtin_nanf("");
 }
 
@@ -148,47 +149,59 @@ __device__ __forceinline__ float second_moment(unsigned q, float s) {
     return r2 * r2 * (1.f / (255.f * 255.f * 255.f * 255.f)) * s;
 }
 
-// A wave takes a block of the state at a time, four values a lane.
+// A lane takes a chunk of 16 bytes of the parameter: a wave one block of the state in float32, two in bfloat16.
+template <class T>
+static constexpr int kAdamW8Chunk = Chunk<T>::n * kAdamWThreads;
 template <class T>
 __global__ __launch_bounds__(kAdamWThreads) void adamw_8bit_kernel(const AdamW8Batch b, int count, const AdamWArgs a) {
-    static_assert(kStateBlock == 256, "four values a lane");
-    const int t = tensor_of(b, count), lane = threadIdx.x & 63;
-    const int block = ((int)blockIdx.x - b.first_block[t]) * (kAdamWThreads / 64) + (int)(threadIdx.x >> 6);
-    const int i = block * kStateBlock + lane * 4, left = b.n[t] - i;
-    if (b.n[t] - block * kStateBlock <= 0) return;   // (the whole wave)
+    constexpr int V = Chunk<T>::n, LANES = kStateBlock / V;
+    static_assert(LANES == 64 || LANES == 32, "whole waves or halves");
+    const int t = tensor_of(b, count);
+    const int i = ((int)blockIdx.x - b.first_block[t]) * kAdamW8Chunk<T> + (int)threadIdx.x * V, left = b.n[t] - i;
+    if (__all(left <= 0)) return;
     T *p = static_cast<T *>(b.p[t]) + i;
     const T *g = static_cast<const T *>(b.g[t]) + i;
+    const int block = (left > 0 ? i : b.n[t] - 1) / kStateBlock;   // (lanes beside the tensor: the last one, of which they read and write no value)
     const Corrections c = corrections(a);
     const float rate = a.lr_ptr ? *a.lr_ptr : a.lr, decay = a.lr_ptr ? 1.f - rate * a.weight_decay : a.decay;
     const float ms = b.ms[t][block], vs = b.vs[t][block];
-    float pv[4], gv[4], mv[4], vv[4];
-    ld4(p, left, pv);
-    ld4(g, left, gv);
-    uint32_t mq = ld_codes(b.m[t] + i, left), vq = ld_codes(b.v[t] + i, left);
+    float pv[V], gv[V], mv[V], vv[V];
+    load_part(p, left, pv);
+    load_part(g, left, gv);
+    uint32_t mq[V / 4], vq[V / 4];
+#pragma unroll
+    for (int h = 0; h < V / 4; ++h) {
+        mq[h] = ld_codes(b.m[t] + i + 4 * h, left - 4 * h);
+        vq[h] = ld_codes(b.v[t] + i + 4 * h, left - 4 * h);
+    }
     float mtop = 0.f, vtop = 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {   // (beside the tensor: zeros)
-        mv[e] = first_moment((int8_t)(mq >> (8 * e)), ms);
-        vv[e] = second_moment((vq >> (8 * e)) & 255u, vs);
+    for (int e = 0; e < V; ++e) {   // (beside the tensor: zeros)
+        mv[e] = first_moment((int8_t)(mq[e / 4] >> (8 * (e & 3))), ms);
+        vv[e] = second_moment((vq[e / 4] >> (8 * (e & 3))) & 255u, vs);
         pv[e] = adamw_value(pv[e], gv[e], mv[e], vv[e], a, c, rate, decay);
         mtop = maximum(mtop, fabsf(mv[e]));
         vtop = maximum(vtop, vv[e]);
     }
-    st4(p, left, pv);
-    const float ns = wave_scale(mtop), ws = wave_scale(vtop);
+    store_part(p, left, pv);
+    const float ns = lanes_scale<LANES>(mtop), ws = lanes_scale<LANES>(vtop);
     const float im = inverse(ns), iv = inverse(ws);
-    mq = vq = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        // (the plain root instruction, one unit in the last place: of a number from 0 to 1, towards a code)
-        const float rm = copysignf(rintf(127.f * __builtin_amdgcn_sqrtf(fabsf(mv[e]) * im)), mv[e]);
-        const float rv = rintf(255.f * __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(vv[e] * iv)));
-        mq = __builtin_amdgcn_cvt_pk_u8_f32(rm < 0.f ? rm + 256.f : rm, e, mq);   // (two's complement)
-        vq = __builtin_amdgcn_cvt_pk_u8_f32(fmaxf(rv, vv[e] > 0.f ? 1.f : 0.f), e, vq);
+    for (int h = 0; h < V / 4; ++h) {
+        mq[h] = vq[h] = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float m = mv[4 * h + e], v = vv[4 * h + e];
+            // (the plain root instruction, one unit in the last place: of a number from 0 to 1, towards a code)
+            const float rm = copysignf(rintf(127.f * __builtin_amdgcn_sqrtf(fabsf(m) * im)), m);
+            const float rv = rintf(255.f * __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(v * iv)));
+            mq[h] = __builtin_amdgcn_cvt_pk_u8_f32(rm < 0.f ? rm + 256.f : rm, e, mq[h]);   // (two's complement)
+            vq[h] = __builtin_amdgcn_cvt_pk_u8_f32(fmaxf(rv, v > 0.f ? 1.f : 0.f), e, vq[h]);
+        }
+        st_codes(b.m[t] + i + 4 * h, left - 4 * h, mq[h]);
+        st_codes(b.v[t] + i + 4 * h, left - 4 * h, vq[h]);
     }
-    st_codes(b.m[t] + i, left, mq);
-    st_codes(b.v[t] + i, left, vq);
-    if (lane == 0) {
+    if ((threadIdx.x & (LANES - 1)) == 0 && left > 0) {
         b.ms[t][block] = ns;
         b.vs[t][block] = ws;
     }
@@ -234,12 +247,12 @@ __global__ __launch_bounds__(256) void state_values_kernel(const void *codes, in
 }
 
 template <class B, class F>
-static int fill_blocks(B &b, int count, const long *n, F more) {
+static int fill_blocks(B &b, int count, const long *n, int chunk, F more) {
     int blocks = 0;
     for (int t = 0; t < count; ++t) {
         b.n[t] = (int)n[t];
         b.first_block[t] = blocks;
-        blocks += (int)ceil_div_l(n[t], kAdamWChunk);
+        blocks += (int)ceil_div_l(n[t], chunk);
         more(t);
     }
     b.first_block[count] = blocks;
@@ -250,7 +263,7 @@ template <class T>
 int launch_adamw(int count, void *const *p, const void *const *g, float *const *m, float *const *v, const long *n, const AdamWArgs &a,
                  hipStream_t s) {
     AdamWBatch b;
-    const int blocks = fill_blocks(b, count, n, [&](int t) {
+    const int blocks = fill_blocks(b, count, n, kAdamWChunk, [&](int t) {
         b.p[t] = p[t]; b.g[t] = g[t]; b.m[t] = m[t]; b.v[t] = v[t];
     });
     hipLaunchKernelGGL(adamw_kernel<T>, dim3(blocks), dim3(kAdamWThreads), 0, s, b, count, a);
@@ -261,7 +274,7 @@ template <class T>
 int launch_adamw_8bit(int count, void *const *p, const void *const *g, int8_t *const *m, uint8_t *const *v, float *const *ms,
                       float *const *vs, const long *n, const AdamWArgs &a, hipStream_t s) {
     AdamW8Batch b;
-    const int blocks = fill_blocks(b, count, n, [&](int t) {
+    const int blocks = fill_blocks(b, count, n, kAdamW8Chunk<T>, [&](int t) {
         b.p[t] = p[t]; b.g[t] = g[t]; b.m[t] = m[t]; b.v[t] = v[t]; b.ms[t] = ms[t]; b.vs[t] = vs[t];
     });
     hipLaunchKernelGGL(adamw_8bit_kernel<T>, dim3(blocks), dim3(kAdamWThreads), 0, s, b, count, a);

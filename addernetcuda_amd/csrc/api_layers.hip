@@ -189,7 +189,7 @@ int adder_layer_norm_bwd_workspace_bytes(long rows, int width, int type, size_t 
     if (!bytes) return ADDER_ERR_NULL_POINTER;
     if (rows <= 0 || width <= 0 || !known(type)) return ADDER_ERR_BAD_SHAPE;
     if (width > kMaxWidth || wide(rows, width)) return ADDER_ERR_TOO_LARGE;
-    *bytes = whole(sizeof(float) * 2 * (size_t)layer_norm_bwd_parts(rows, width, type) * width);
+    *bytes = whole(sizeof(float) * 2 * (size_t)layer_norm_bwd_parts(rows, width) * width);
     return ADDER_OK;
 }
 

@@ -300,8 +300,7 @@ static int norm_fwd_blocks(long rows, int G) {
     return (int)(need < most ? need : most);
 }
 
-int layer_norm_bwd_parts(long rows, int D, int type) {
-    (void)type;
+int layer_norm_bwd_parts(long rows, int D) {
     if (D > kNormRegisterWidth) return (int)(rows < 64 ? rows : 64);
     const int G = norm_lanes(D);
     const long per = G > kNormBwdThreads ? 1 : kNormBwdThreads / G, need = ceil_div_l(rows, per), most = 256;
@@ -340,7 +339,7 @@ int launch_layer_norm_fwd(const T *x, long x_stride, const W *w, const W *b, T *
 template <class T, class W>
 int launch_layer_norm_bwd(const T *dy, long dy_stride, const T *x, long x_stride, const W *w, const float *mean, const float *rstd,
                           T *gx, W *gw, W *gb, long rows, int D, float *part, hipStream_t s) {
-    const int parts = layer_norm_bwd_parts(rows, D, 0);
+    const int parts = layer_norm_bwd_parts(rows, D);
     float *sums = gw || gb ? part : nullptr;
     if (D > kNormRegisterWidth) {
         if (gx) {

@@ -141,7 +141,7 @@ int launch_layer_norm_fwd(const T *x, long x_stride, const W *w, const W *b, T *
 template <class T, class W>
 int launch_layer_norm_bwd(const T *dy, long dy_stride, const T *x, long x_stride, const W *w, const float *mean, const float *rstd,
                           T *gx, W *gw, W *gb, long rows, int D, float *part, hipStream_t s);
-int layer_norm_bwd_parts(long rows, int D, int type);   // slabs of 2 D floats that the backward's workspace holds
+int layer_norm_bwd_parts(long rows, int D);   // slabs of 2 D floats that the backward's workspace holds
 
 // the AdamW step (adamw.hip)
 static constexpr int kAdamWBatchMax = ADDER_ADAMW_BATCH_MAX, kAdamW8BatchMax = ADDER_ADAMW_8BIT_BATCH_MAX;
