@@ -232,12 +232,14 @@ struct Flag { static constexpr bool value = V; };
 // A tile of R rows (or columns, with k across the rows) by BK values of k in bfloat16.  Where rows lie a power of two apart, a bank
 // conflict is avoided by the order of their 16-byte chunks:
 //   k along the rows:   row r has BK / 8 chunks; chunk c at place c ^ (r & 7) (rows of 128 bytes) or c ^ (r / 2 & 3) (64 bytes)
-//   k across the rows:  row k has R / 8 chunks; chunk c at place c ^ 2 (k & 7), below 128 columns 2 (k & 3)
+//   k across the rows:  row k has R / 8 chunks, read in pairs by 32 lanes at once: rows 0 to 3 and 8 to 11 of sixteen, or 4 to 7 and 12 to
+//                       15.  Chunk c at place c ^ 2 (k & 3 | k / 8 & 1 << 2), below 128 columns, where two rows lie beside each other in
+//                       the 64 banks, c ^ 2 (k / 2 & 1 | k / 8 & 1 << 1)
 template <int R, int BK, bool ACROSS>
 struct LdsTile {
     static constexpr int bytes = R * BK * 2, row_bytes = ACROSS ? R * 2 : BK * 2, row_chunks = row_bytes / 16;
     static __device__ __forceinline__ int place(int row, int chunk) {
-        if constexpr (ACROSS) return chunk ^ ((row & (R >= 128 ? 7 : 3)) << 1);
+        if constexpr (ACROSS) return chunk ^ (R >= 128 ? (row & 3) << 1 | (row & 8) : (row & 2) | (row & 8) >> 1);
         else return BK == 64 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3);
     }
     // values k + 8 (lane / 16) .. + 7 of row (column) at + lane % 16, a matrix instruction's operand.  With k across the rows:
@@ -246,9 +248,9 @@ struct LdsTile {
         if constexpr (ACROSS) {
             typedef __attribute__((address_space(3))) s16x4 *lds_ptr;
             const int i = lane & 15, row = k + (lane >> 4) * 8 + (i >> 2), c = at / 8 + ((i & 3) >> 1);
-            const char *q = tile + row * row_bytes + ((i & 1) << 3);
-            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(q + (place(row, c) << 4)));
-            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(q + 4 * row_bytes + (place(row + 4, c) << 4)));
+            const char *q = tile + row * row_bytes + (place(row, c) << 4) + ((i & 1) << 3);   // (four rows on: the same place)
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)q);
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(q + 4 * row_bytes));
             struct Both { s16x4 lo, hi; };
             return __builtin_bit_cast(bf16x8, Both{lo, hi});
         } else {
