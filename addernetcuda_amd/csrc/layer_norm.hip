@@ -296,7 +296,7 @@ static int norm_lanes(int D) {
 }
 
 static int norm_fwd_blocks(long rows, int G) {
-    const long per = G > kNormFwdThreads ? 1 : kNormFwdThreads / G, need = ceil_div_l(rows, per), most = 2048;
+    const long per = G > kNormFwdThreads ? 1 : kNormFwdThreads / G, need = ceil_div_l(rows, per), most = 768;
     return (int)(need < most ? need : most);
 }
 

@@ -146,9 +146,11 @@ int launch_product(const Product &q, void *ws, hipStream_t s) {
 }
 
 // ---- the activation's derivative and the bias's gradient ---------------------------------------------------------------
-// A workgroup takes 64 lanes' chunks of columns and a share of the rows: its four waves walk over the rows, kActRows of them under way,
-// and their column sums are added through LDS into one slab a share.
-static constexpr int kActRows = 4;
+// Memory decides: dy and z are read and dz is written, 41 us for 8192 x 4096 in bfloat16 with a GELU (4.9 TB/s).  A workgroup takes 64 lanes'
+// chunks of columns and a share of the rows; its four waves walk over the rows, and their column sums are added through LDS into
+// one slab a share.  A row at a time and up to four workgroups a compute unit: two or four rows under way in a wave are no faster where there
+// are many (53 us with what follows, all three) and leave waves out where there are few (128 x 512: 9.9 and 10.8 us instead of 9.5);
+// 2048 workgroups leave more slabs to fold (16384 x 512: 23.4 us instead of 21.1).
 template <class T, Act ACT>
 __global__ __launch_bounds__(256) void act_bwd_kernel(const T *__restrict__ dy, long dy_stride, const T *__restrict__ z,
                                                       T *__restrict__ dz, float *__restrict__ part, long rows, long N) {
@@ -160,31 +162,18 @@ __global__ __launch_bounds__(256) void act_bwd_kernel(const T *__restrict__ dy, 
     float sum[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) sum[e] = 0.f;
-    const long ahead = (long)gridDim.y * 4;   // rows from one of a wave's to the next
-    for (long m0 = (long)blockIdx.y * 4 + wave; m0 < rows; m0 += kActRows * ahead) {
-        uint4 g[kActRows], v[kActRows];
+    for (long m = (long)blockIdx.y * 4 + wave; m < rows; m += (long)gridDim.y * 4) {
+        float d[V];
+        load_part(dy + m * dy_stride + n, left, d);
+        if constexpr (ACT != Act::none) {
+            float w[V];
+            load_part(z + m * N + n, left, w);
 #pragma unroll
-        for (int r = 0; r < kActRows; ++r) {
-            const long m = m0 + r * ahead;
-            const int valid = m < rows ? left : 0;
-            g[r] = load_raw_part(dy + m * dy_stride + n, valid);
-            if constexpr (ACT != Act::none) v[r] = load_raw_part(z + m * N + n, valid);
+            for (int e = 0; e < V; ++e) d[e] *= slope<kExactAct<T>>(w[e], ACT);
+            if (dz) store_part(dz + m * N + n, left, d);
         }
 #pragma unroll
-        for (int r = 0; r < kActRows; ++r) {
-            const long m = m0 + r * ahead;
-            float d[V];
-            unpack(g[r], d);
-            if constexpr (ACT != Act::none) {
-                float w[V];
-                unpack(v[r], w);
-#pragma unroll
-                for (int e = 0; e < V; ++e) d[e] *= slope<kExactAct<T>>(w[e], ACT);
-                if (dz) store_part(dz + m * N + n, m < rows ? left : 0, d);
-            }
-#pragma unroll
-            for (int e = 0; e < V; ++e) sum[e] += d[e];   // (rows that do not exist: dy of zero times the slope at zero)
-        }
+        for (int e = 0; e < V; ++e) sum[e] += d[e];   // (columns that do not exist: dy of zero times the slope at zero)
     }
     if (!part) return;
 #pragma unroll
@@ -200,9 +189,9 @@ __global__ __launch_bounds__(256) void act_bwd_kernel(const T *__restrict__ dy, 
     }
 }
 
-// Shares of the rows: enough workgroups for eight a compute unit, and at least kActRows rows a wave
+// Shares of the rows: a row a wave, as long as there are no more workgroups than four a compute unit
 int act_bwd_parts(long rows, long N) {
-    const long columns = ceil_div_l(N, 512), need = ceil_div_l(rows, 4 * kActRows), most = ceil_div_l(2048, columns);
+    const long columns = ceil_div_l(N, 512), need = ceil_div_l(rows, 4), most = ceil_div_l(4 * kCUs, columns);
     return (int)(need < most ? need : most);
 }
 
