@@ -6,7 +6,8 @@ matrix cores and bias, activation and shortcut on its way out, so that the produ
 is one pass for ``dy * act'(z)`` and the bias's gradient, then the two products.  Arguments, outputs and the autograd node are
 csrc/nodes.cpp.
 
-float32 and bfloat16, all tensors of a call alike (the module rounds float32 parameters for a bfloat16 input).  CPU tensors, other
+float32 and bfloat16, all tensors of a call alike (the module rounds float32 parameters for a bfloat16 input, ``torch.autocast`` all
+that the product reads).  CPU tensors, other
 types, tensor subclasses and calls that something records, traces or transforms go through torch's own operators.
 """
 import torch
@@ -19,19 +20,32 @@ ACTS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}   # adder_act
 TYPES = {torch.float32: 0, torch.bfloat16: 1}         # adder_type
 
 
+def _plus(y, residual):
+    try:
+        residual = residual.expand(y.shape)
+    except RuntimeError:
+        raise RuntimeError(f"residual of shape {tuple(residual.shape)} does not broadcast to {tuple(y.shape)}") from None
+    return y + residual
+
+
 def _torch_linear_act(x, weight, bias, residual, act):
     if weight.dim() != 2:
         raise RuntimeError(f"weight must have two dimensions, got {tuple(weight.shape)}")
     y = F.linear(x, weight, bias)
     if act != "none":
         y = {"relu": F.relu, "gelu": F.gelu, "silu": F.silu}[act](y)
-    if residual is None:
-        return y
-    try:
-        residual = residual.expand(y.shape)
-    except RuntimeError:
-        raise RuntimeError(f"residual of shape {tuple(residual.shape)} does not broadcast to {tuple(y.shape)}") from None
-    return y + residual
+    return y if residual is None else _plus(y, residual)
+
+
+def _autocast_linear_act(x, weight, bias, residual, act):
+    """Inside ``torch.autocast``: the product in its type, as ``F.linear``'s there; a residual of another type is added behind it."""
+    dtype = torch.get_autocast_dtype("cuda")
+    if dtype not in TYPES or any(t is not None and t.dtype not in TYPES for t in (x, weight, bias)):
+        return _torch_linear_act(x, weight, bias, residual, act)
+    own = residual is None or residual.dtype == dtype
+    with torch.autocast("cuda", enabled=False):
+        y = linear_act(x.to(dtype), weight.to(dtype), None if bias is None else bias.to(dtype), residual if own else None, act)
+        return y if own else _plus(y, residual)
 
 
 def linear_act(x, weight, bias=None, residual=None, act="none"):
@@ -42,8 +56,11 @@ def linear_act(x, weight, bias=None, residual=None, act="none"):
     code = ACTS.get(act)
     if code is None:
         raise ValueError(f"act must be one of {tuple(ACTS)}, got {act!r}")
-    if plain_tensors(x, weight, bias, residual) and x.is_cuda and x.dtype in TYPES and weight.numel():
-        return nodes.linear_act(x, weight, bias, residual, code)
+    if plain_tensors(x, weight, bias, residual) and x.is_cuda:
+        if torch.is_autocast_enabled("cuda"):
+            return _autocast_linear_act(x, weight, bias, residual, act)
+        if x.dtype in TYPES and weight.numel():
+            return nodes.linear_act(x, weight, bias, residual, code)
     return _torch_linear_act(x, weight, bias, residual, act)
 
 

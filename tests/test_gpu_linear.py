@@ -271,3 +271,27 @@ def test_relu_reads_its_own_result(gpu, rows, k, n, dtype):
     own.add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         own.sum().backward()
+
+
+def test_autocast_as_torch_linear(gpu):
+    """The product in autocast's type, a residual of another type added in the wider one, gradients of the leaves' own type; a type that
+    has no kernel goes through torch."""
+    from addernetcuda_amd.linear import linear_act, LinearAct
+    x, w, b, r, dy = make(40, 72, 56, torch.float32)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        y = linear_act(x.requires_grad_(True), w.requires_grad_(True), b, act="gelu")
+        wide = linear_act(x, w, b, r, act="gelu")
+        with pytest.raises(RuntimeError, match="does not broadcast"):
+            linear_act(x, w, b, r[:, :3], act="gelu")
+    half = [t.detach().bfloat16() for t in (x, w, b)]
+    assert y.dtype == torch.bfloat16 and torch.equal(y, linear_act(*half, act="gelu"))
+    assert wide.dtype == torch.float32 and torch.equal(wide, y.float() + r)
+    own = [t.requires_grad_(True) for t in half[:2]]
+    want = torch.autograd.grad(linear_act(*own, half[2], act="gelu"), own, dy.bfloat16())
+    for g, h in zip(torch.autograd.grad(y, (x, w), dy.bfloat16()), want):
+        assert g.dtype == torch.float32 and torch.equal(g, h.float())
+    layer = LinearAct(72, 56, act="silu").cuda()
+    with torch.autocast("cuda", dtype=torch.float16):
+        assert layer(x).dtype == torch.float16
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        assert layer(x).dtype == torch.bfloat16 and linear_act(x.double().detach(), w.double().detach()).dtype == torch.float64
