@@ -7,8 +7,10 @@
 // The roots give small values more codes than a straight scale would (the second moment reaches down to 2e-10 of the block's
 // largest), and they need no table.  Codes go to the nearest; a second moment that is not zero keeps a code that is not zero,
 // since its root divides.  The parameter is updated with the moments before they are rounded.
-// Memory decides: 28 bytes a float parameter with moments of 32 bits, 16 with moments of 8.  The table of tensors travels by
-// value in the kernel arguments, as that of the SGD step does.
+// Memory decides: 28 bytes a float parameter with moments of 32 bits, 16 with moments of 8.  67 million float values: 340 us (5.5 TB/s)
+// and 192 us (5.6 TB/s); in bfloat16 264 us (22 bytes, 5.6 TB/s) and 147 us (10 bytes, 4.6 TB/s: the roots and roundings of the codes
+// begin to count).  65 small tensors, 272 000 values: 4.9 us.  The table of tensors travels by value in the kernel arguments, as
+// that of the SGD step does.
 #include "layers.hpp"
 
 namespace adder {
@@ -149,7 +151,8 @@ __device__ __forceinline__ float second_moment(unsigned q, float s) {
     return r2 * r2 * (1.f / (255.f * 255.f * 255.f * 255.f)) * s;
 }
 
-// A lane takes a chunk of 16 bytes of the parameter: a wave one block of the state in float32, two in bfloat16.
+// A lane takes a chunk of 16 bytes of the parameter: a wave one block of the state in float32, two in bfloat16 (one: 165 us instead of 147
+// for 64M values).  The block's largest moments are known only behind the update of all its values, so both stay in registers.
 template <class T>
 static constexpr int kAdamW8Chunk = Chunk<T>::n * kAdamWThreads;
 template <class T>

@@ -4,6 +4,8 @@
 // Memory decides: the forward has to read x and write y, the backward to read x and dy and write gx.  A row stays in registers
 // from its one load on (G lanes with at most 16 values each), so the variance is that of the differences from the mean, with
 // no second read and none of the cancellation of E[x^2] - mean^2.  All sums are 32 bits.
+// 16384 x 1024 in bfloat16: forward 14.9 us (4.5 TB/s; a copy of as much takes 10), backward 19.2 us (5.2 TB/s) and 3.8 us for the
+// fold of the columns; 3001 x 777 in float32 8.1, 9 and 3 us; 8 x 512 3.2 us, a launch.
 #include "layers.hpp"
 
 namespace adder {
@@ -182,7 +184,7 @@ __global__ __launch_bounds__(G > kNormBwdThreads ? G : kNormBwdThreads) void lay
     }
 }
 
-// Rows longer than kNormRegisterWidth: one workgroup a row, which reads it again for each of the sums.
+// Rows longer than kNormRegisterWidth: one workgroup a row, which reads it again (from its L2, as long as that holds it) for each of the sums.
 static constexpr int kNormWide = 1024;
 template <class T, class W>
 __global__ __launch_bounds__(kNormWide) void layer_norm_wide_fwd_kernel(const T *__restrict__ x, long x_stride,
@@ -256,7 +258,7 @@ __global__ __launch_bounds__(256) void layer_norm_wide_columns_kernel(const T *_
     slab[(size_t)D + i] = sb;
 }
 
-// 32 columns and 32 shares of the slabs a workgroup
+// 32 columns and 32 shares of the slabs a workgroup: 2.5 to 5 us, half of it the launch
 static constexpr int kFoldColumns = 32, kFoldShares = 32;
 template <class T>
 __global__ __launch_bounds__(kFoldColumns *kFoldShares) void fold_columns_kernel(const float *__restrict__ part, int parts, int K,
@@ -295,11 +297,15 @@ static int norm_lanes(int D) {
     return g;
 }
 
+// At most three workgroups a compute unit, which walk over the rows with the weight in registers: 512 workgroups take 15.5 us for 16384 x 1024 in
+// bfloat16 instead of 13.6, 2048 take 17.9 us for 2048 x 8192 instead of 15.6 and 8.0 for 32768 x 256 instead of 6.9
 static int norm_fwd_blocks(long rows, int G) {
     const long per = G > kNormFwdThreads ? 1 : kNormFwdThreads / G, need = ceil_div_l(rows, per), most = 768;
     return (int)(need < most ? need : most);
 }
 
+// One workgroup of eight waves a compute unit, each with a slab: 128 take 25.8 us with the fold for 16384 x 1024 in bfloat16 instead of
+// 19.2 and 512 take 17.6, but 30.5 for 2048 x 8192 instead of 25.1, whose slabs are as large as its tensors
 int layer_norm_bwd_parts(long rows, int D) {
     if (D > kNormRegisterWidth) return (int)(rows < 64 ? rows : 64);
     const int G = norm_lanes(D);

@@ -7,7 +7,8 @@ namespace adder {
 // A workgroup takes sixteen rows of w (columns of the output) and up to 16 MT rows of x.  Its waves take turns along k, 128
 // bytes of every row at a time, straight from memory into the matrix instructions' operands -- a lane 32 of a row's 128
 // bytes, so that lines are used whole -- and add their sums through LDS.  No tile of w is read twice by a workgroup, nothing waits
-// for a barrier before the end, and no second launch joins anything.  float32 stays float32: the matrix cores' rate for it is enough
+// for a barrier before the end, and no second launch joins anything.  One row, 4096 x 4096 in bfloat16: 7.4 us in a graph (4.5 TB/s)
+// with everything around it; 64 rows 11.5 us; one float32 row 14 us.  float32 stays float32: the matrix cores' rate for it is enough
 // beside the loads.
 template <int MT>
 static constexpr int kRowsWaves = MT == 4 ? 8 : 16;   // (four tiles of x and what arrives behind them take more than 128 registers)

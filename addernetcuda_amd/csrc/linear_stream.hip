@@ -9,6 +9,11 @@ namespace adder {
 // stage, the barrier makes that every wave's, and behind it the buffer read last is free for the next loads.  One barrier a
 // stage, and no wait for loads that are under way.
 //
+// The matrix cores decide, with what the LDS reads leave them: 8192 x 4096 to 1024 values and a residual 62.9 us, 1093 TFLOP/s, the matrix
+// cores busy for 61 % of the cycles (the rates of all shapes stand beside the choice among them).  8192 x 1024 to 4096 with a GELU and the
+// values before it as a second output takes 97 us: 51 for the products, the rest for 17 vector instructions a result and 134 MB of
+// stores, which two workgroups a compute unit overlap in part; to start them apart from each other changed nothing.
+//
 // A load instruction of a wave fills 1024 consecutive bytes of LDS, 16 a lane: the lanes fetch the chunks in the order in which the
 // tile keeps them.  Loads past a tensor's end return nothing: the buffer descriptor ends with the tensor.  What lies past a row's
 // end (k beyond K in the last tile) is masked in registers, results of rows past M or N are not stored.
