@@ -168,7 +168,9 @@ __global__ __launch_bounds__(256) void act_bwd_kernel(const T *__restrict__ dy, 
         load_part(dy + m * dy_stride + n, left, d);
         if constexpr (ACT != Act::none) {
             float w[V];
-            load_part(z + m * N + n, left, w);
+            const uint4 u = load_raw_part(z + m * N + n, left);
+            if constexpr (keeps_half(sizeof(T), ACT)) unpack_half(u, w);
+            else unpack(u, w);
 #pragma unroll
             for (int e = 0; e < V; ++e) d[e] *= slope<kExactAct<T>>(w[e], ACT);
             if (dz) store_part(dz + m * N + n, left, d);

@@ -24,7 +24,7 @@ __device__ __forceinline__ i32x4 descriptor(const char *p, long left) {
 }
 // 16 bytes a lane from base + offset to the 1024 bytes of LDS at `to` (a wave's); no register is written
 __device__ __forceinline__ void stream(const i32x4 &d, unsigned offset, unsigned to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(d) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(d) : "memory", "m0");
 }
 // All but the `N` newest loads of this wave done, and its LDS reads; then the workgroup's waves meet.
 template <int N>

@@ -62,6 +62,20 @@ __device__ __forceinline__ float slope(float z, Act act) {
 template <class T>
 static constexpr bool kExactAct = sizeof(T) == 4;
 
+// z as it is kept for the backward.  In bfloat16 a GELU's or SiLU's is an IEEE half, of 11 bits instead of 8: a derivative from z in
+// bfloat16 alone would be 6e-4 off, beside the 1.6e-3 of rounding dz.  Rounded toward zero (v_cvt_pkrtz_f16_f32), so that no finite z
+// becomes infinite: beyond 65504 the derivative is a constant.  A ReLU's has z's sign, in the layer's type.
+__host__ __device__ constexpr bool keeps_half(size_t size, Act act) { return size == 2 && (act == Act::gelu || act == Act::silu); }
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(lo, hi)); }
+__device__ __forceinline__ uint4 pack_half(const float (&v)[8]) {
+    return make_uint4(pack_half(v[0], v[1]), pack_half(v[2], v[3]), pack_half(v[4], v[5]), pack_half(v[6], v[7]));
+}
+__device__ __forceinline__ void unpack_half(const uint4 &u, float (&v)[8]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[e / 2] >> (16 * (e & 1))));
+}
+
 // ---- products ------------------------------------------------------------------------------------------------------
 struct ProductArgs {
     const void *a, *b, *bias, *res;
@@ -71,6 +85,15 @@ struct ProductArgs {
     int tiles_m, tiles_n, splits;
     Act act;
 };
+
+__device__ __forceinline__ void keep(float *p, float z, Act) { *p = z; }
+__device__ __forceinline__ void keep(bf16_t *p, float z, Act act) { *p = keeps_half(2, act) ? (bf16_t)pack_half(z, 0.f) : round_bf16(z); }
+__device__ __forceinline__ void keep4(float *p, const float (&z)[4], Act) { put4(p, z); }
+__device__ __forceinline__ void keep4(bf16_t *p, const float (&z)[4], Act act) {
+    if (!keeps_half(2, act)) return put4(p, z);
+    const uint32_t lo = pack_half(z[0], z[1]), hi = pack_half(z[2], z[3]);
+    *reinterpret_cast<u16x4_any *>(p) = u16x4_any{(uint16_t)lo, (uint16_t)(lo >> 16), (uint16_t)hi, (uint16_t)(hi >> 16)};
+}
 
 // `cnt` <= 4 neighbouring sums of row m from column n on: the epilogue
 template <class T>
@@ -112,13 +135,13 @@ __device__ __forceinline__ void finish(const ProductArgs &p, long m, long n, int
     for (int e = 0; e < 4; ++e) y[e] += r[e];
     if (cnt == 4) {
         put4(out + at, y);
-        if (pre) put4(pre + at, z);
+        if (pre) keep4(pre + at, z, p.act);
     } else {
 #pragma unroll
         for (int e = 0; e < 3; ++e)
             if (e < cnt) {
                 put(out + at + e, y[e]);
-                if (pre) put(pre + at + e, z[e]);
+                if (pre) keep(pre + at + e, z[e], p.act);
             }
     }
 }
@@ -179,7 +202,9 @@ __device__ __forceinline__ void finish_tile(const ProductArgs &p, const f32x4 (&
             exchange(o);
             store_raw(out + m * p.N + at + j * 16, o);
             if (pre) {
-                uint4 q = pack(z);
+                uint4 q;
+                if constexpr (keeps_half(sizeof(T), ACT)) q = pack_half(z);
+                else q = pack(z);
                 exchange(q);
                 store_raw(pre + m * p.N + at + j * 16, q);
             }

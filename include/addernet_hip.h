@@ -497,8 +497,9 @@ typedef enum adder_type { ADDER_TYPE_F32 = 0, ADDER_TYPE_BF16 = 1 } adder_type;
 /* Linear layer: z = x w' + bias, y = act(z) + residual; x (rows, in_features), w (out_features, in_features) dense,
  * bias (out_features), residual and y (rows, out_features).
  *   act: none, relu, gelu (z Phi(z), by the error function) or silu (z / (1 + exp(-z))).
- *   adder_linear_fwd: bias and residual nullable.  pre (nullable): receives z (rows, out_features), which the backward of every
- *     act but none needs (relu's takes y just as well where there was no residual).
+ *   adder_linear_fwd: bias and residual nullable.  pre (nullable): receives what the backward of every act but none needs of z, rows x
+ *     out_features values of the type's size: z itself, but for gelu and silu in bfloat16, where it is z as IEEE half.  relu's backward
+ *     takes y just as well where there was no residual.
  *   adder_linear_bwd: dz = dy act'(pre); gx = dz w, gw = dz' x, gbias = sum over rows of dz; each of the three nullable.  The
  *     residual's gradient is dy.  pre is not read where act is none; x only for gw, w only for gx.  bfloat16: dz is rounded
  *     to bfloat16 for the two products (the matrix cores' operands), and not for gbias.

@@ -295,3 +295,20 @@ def test_autocast_as_torch_linear(gpu):
         assert layer(x).dtype == torch.float16
     with torch.autocast("cuda", dtype=torch.bfloat16):
         assert layer(x).dtype == torch.bfloat16 and linear_act(x.double().detach(), w.double().detach()).dtype == torch.float64
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("rows,k,n", [(3, 24, 10), (200, 64, 136), (256, 128, 128)])
+def test_derivative_far_from_zero(gpu, rows, k, n, act, dtype):
+    """|z| far beyond 65504: the derivative is one or zero, and the gradients are the plain product's for dy in the rows of positive z,
+    by the same launches."""
+    from addernetcuda_amd.linear import linear_act
+    x, w, b, _, dy = make(rows, k, n, dtype)
+    sign = torch.where(torch.arange(rows, device="cuda") % 3 == 0, -1.0, 1.0)[:, None]
+    x, w = (x.float().abs().add(1) * sign * 2.0 ** 20).to(dtype), w.float().abs().add(2.0 ** -4).to(dtype)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    got = torch.autograd.grad(linear_act(*leaves, act=act), leaves, dy)
+    want = torch.autograd.grad(linear_act(*leaves), leaves, torch.where(sign > 0, dy, torch.zeros_like(dy)))
+    for g, h in zip(got, want):
+        assert torch.equal(g, h)
