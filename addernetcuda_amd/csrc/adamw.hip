@@ -8,7 +8,7 @@
 // largest), and they need no table.  Codes go to the nearest; a second moment that is not zero keeps a code that is not zero,
 // since its root divides.  The parameter is updated with the moments before they are rounded.
 // Memory decides: 28 bytes a float parameter with moments of 32 bits, 16 with moments of 8.  67 million float values: 340 us (5.5 TB/s)
-// and 192 us (5.6 TB/s); in bfloat16 264 us (22 bytes, 5.6 TB/s) and 147 us (10 bytes, 4.6 TB/s: the roots and roundings of the codes
+// and 205 us (5.2 TB/s); in bfloat16 264 us (22 bytes, 5.6 TB/s) and 147 us (10 bytes, 4.6 TB/s: the roots and roundings of the codes
 // begin to count).  65 small tensors, 272 000 values: 4.9 us.  The table of tensors travels by value in the kernel arguments, as
 // that of the SGD step does.
 #include "layers.hpp"
@@ -49,12 +49,16 @@ __device__ __forceinline__ int tensor_of(const B &b, int count) {
     return lo;
 }
 
-// The root and the reciprocal are the plain instructions (one unit in the last place of the update each).  The root's takes moments below
-// the smallest normal float for zero; beside an eps of less than a root of those it is the exact one.
+// The moments are rounded product by product, as the formulas are in float32.  The update's root and reciprocal are the plain instructions
+// (one unit in its last place each).  The root's takes moments below the smallest normal float for zero; beside an eps of less than a
+// root of those it is the exact one.
 __device__ __forceinline__ float adamw_value(float p, float g, float &m, float &v, const AdamWArgs &a, const Corrections &c,
                                              float rate, float decay) {
-    m = fmaf(a.b1, m, a.one_b1 * g);
-    v = fmaf(a.b2, v, a.one_b2 * g * g);
+    {
+#pragma clang fp contract(off)
+        m = a.b1 * m + a.one_b1 * g;
+        v = a.b2 * v + a.one_b2 * g * g;
+    }
     const float root = a.eps < 1e-12f ? sqrtf(v) : __builtin_amdgcn_sqrtf(v);
     return fmaf(-rate * c.c1, m * __builtin_amdgcn_rcpf(fmaf(root, c.c2, a.eps)), p * decay);
 }
@@ -143,12 +147,26 @@ __device__ __forceinline__ float lanes_scale(float t) {
 __device__ __forceinline__ float inverse(float scale) { return scale >= 0x1p-126f ? 1.f / scale : 0.f; }
 
 __device__ __forceinline__ float first_moment(int q, float s) {
-    const float r = (float)q;
-    return r * fabsf(r) * (1.f / (127.f * 127.f)) * s;   // (the square is exact)
+    const float d = (float)q * (1.f / 127.f);
+    return s * (d * fabsf(d));
 }
 __device__ __forceinline__ float second_moment(unsigned q, float s) {
-    const float r = (float)q, r2 = r * r;
+    const float r = (float)q, r2 = r * r;   // (exact)
     return r2 * r2 * (1.f / (255.f * 255.f * 255.f * 255.f)) * s;
+}
+// On the way to a code: a / s for a <= s and y = 1 / s, and a root; correctly rounded where EXACT, else to a unit in the last place.  Exact in
+// float32, so that codes are those of the formulas in float32 arithmetic: else two in a million, next to a tie, go the other way, which the
+// parameters of a step later show (67 million values: 205 us instead of 192).  A bfloat16 parameter does not (147 us).
+template <bool EXACT>
+__device__ __forceinline__ float share(float a, float s, float y) {
+    const float d = a * y;
+    return EXACT ? fmaf(fmaf(-s, d, a), y, d) : d;
+}
+template <bool EXACT>
+__device__ __forceinline__ float root(float x) {
+    if constexpr (!EXACT) return __builtin_amdgcn_sqrtf(x);
+    const float y = __builtin_amdgcn_rsqf(fmaxf(x, 0x1p-120f)), g = x * y;
+    return fmaf(fmaf(-g, g, x), 0.5f * y, g);
 }
 
 // A lane takes a chunk of 16 bytes of the parameter: a wave one block of the state in float32, two in bfloat16 (one: 165 us instead of 147
@@ -158,6 +176,7 @@ static constexpr int kAdamW8Chunk = Chunk<T>::n * kAdamWThreads;
 template <class T>
 __global__ __launch_bounds__(kAdamWThreads) void adamw_8bit_kernel(const AdamW8Batch b, int count, const AdamWArgs a) {
     constexpr int V = Chunk<T>::n, LANES = kStateBlock / V;
+    constexpr bool EXACT = sizeof(T) == 4;
     static_assert(LANES == 64 || LANES == 32, "whole waves or halves");
     const int t = tensor_of(b, count);
     const int i = ((int)blockIdx.x - b.first_block[t]) * kAdamW8Chunk<T> + (int)threadIdx.x * V, left = b.n[t] - i;
@@ -195,9 +214,8 @@ __global__ __launch_bounds__(kAdamWThreads) void adamw_8bit_kernel(const AdamW8B
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float m = mv[4 * h + e], v = vv[4 * h + e];
-            // (the plain root instruction, one unit in the last place: of a number from 0 to 1, towards a code)
-            const float rm = copysignf(rintf(127.f * __builtin_amdgcn_sqrtf(fabsf(m) * im)), m);
-            const float rv = rintf(255.f * __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(v * iv)));
+            const float rm = copysignf(rintf(127.f * root<EXACT>(share<EXACT>(fabsf(m), ns, im))), m);
+            const float rv = rintf(255.f * root<EXACT>(root<EXACT>(share<EXACT>(v, ws, iv))));
             mq[h] = __builtin_amdgcn_cvt_pk_u8_f32(rm < 0.f ? rm + 256.f : rm, e, mq[h]);   // (two's complement)
             vq[h] = __builtin_amdgcn_cvt_pk_u8_f32(fmaxf(rv, v > 0.f ? 1.f : 0.f), e, vq[h]);
         }
