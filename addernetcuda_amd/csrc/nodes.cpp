@@ -71,7 +71,7 @@ struct Rows { Tensor t; long stride, rows; };
 Rows as_rows(const Tensor &t, int64_t width) {
     const int64_t rows = t.numel() / width;
     if (t.is_contiguous()) return {t, (long)width, (long)rows};
-    Tensor v = t.dim() == 2 ? t : t.reshape({rows, width});
+    Tensor v = t.dim() == 2 && t.size(1) == width ? t : t.reshape({rows, width});   // (two dimensions may also be one row: all of them normalised)
     if ((width > 1 && v.stride(1) != 1) || (rows > 1 && v.stride(0) < width && v.stride(0) != 0)) v = v.contiguous();
     return {v, rows > 1 ? (long)v.stride(0) : (long)width, (long)rows};
 }

@@ -191,3 +191,33 @@ def test_refusals(gpu):
         layer_norm(x, w, b, -1e-5)
     with pytest.raises(RuntimeError, match="the last dimension"):
         LayerNorm(20, elementwise_affine=False).cuda()(x)
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=IDS)
+@pytest.mark.parametrize("a,d", [(3, 40), (7, 65), (5, 4000)])
+def test_all_dimensions_normalised_of_matrices_with_gaps(a, d, kind, gpu):
+    """A matrix that is one row as a whole, where its lines do not follow each other: with gaps of NaN, with columns side by side, one line
+    expanded; as input and as gradient."""
+    from addernetcuda_amd.layer_norm import layer_norm, LayerNorm
+    x, w, b, dy = make(1, a * d, kind)
+    want = B.layer_norm(x, w, b, dy, EPS)
+    w, b = w.view(a, d), b.view(a, d)
+
+    def gap(t):
+        big = torch.full((a, d + 3), float("nan"), dtype=t.dtype, device="cuda")
+        big[:, :d] = t
+        return big[:, :d]
+
+    for lay in (gap, lambda t: t.t().contiguous().t()):
+        leaves = [lay(x.view(a, d)).detach().requires_grad_(True), w.detach().requires_grad_(True), b.detach().requires_grad_(True)]
+        y = layer_norm(*leaves, EPS)
+        B.within(y.reshape(1, -1), want["y"], "y")
+        for name, t in zip(("gx", "gw", "gb"), torch.autograd.grad(y, leaves, lay(dy.view(a, d)))):
+            B.within(t.reshape(want[name][0].shape), want[name], name)
+    line = x[:, :d].expand(a, d)
+    assert torch.equal(layer_norm(line, w, b, EPS), layer_norm(line.contiguous(), w, b, EPS))
+    leaf = x.view(a, d).clone().requires_grad_(True)   # a gradient that is one number expanded
+    gx, = torch.autograd.grad(layer_norm(leaf, w, b, EPS).sum(), leaf)
+    B.within(gx.view(1, -1), B.layer_norm(x, w.flatten(), b.flatten(), torch.ones_like(dy), EPS)["gx"], "gx of a sum")
+    plain = LayerNorm((a, d), elementwise_affine=False)
+    assert torch.equal(plain(gap(x.view(a, d))), plain(x.view(a, d)))
