@@ -15,11 +15,13 @@ namespace adder {
 // stores, which two workgroups a compute unit overlap in part; to start them apart from each other changed nothing.
 //
 // A load instruction of a wave fills 1024 consecutive bytes of LDS, 16 a lane: the lanes fetch the chunks in the order in which the
-// tile keeps them.  Loads past a tensor's end return nothing: the buffer descriptor ends with the tensor.  What lies past a row's
-// end (k beyond K in the last tile) is masked in registers, results of rows past M or N are not stored.
+// tile keeps them.  Loads past a tensor's end return nothing: the buffer descriptor ends with the tensor, or with the word that its last value
+// shares (a word that reaches beyond the end is not loaded at all; what lies beside the value in it belongs to a column that is not stored).
+// What lies past a row's end (k beyond K in the last tile) is masked in registers, results of rows past M or N are not stored.
 struct Descriptor { uint64_t base; uint32_t bytes, flags; };
 __device__ __forceinline__ i32x4 descriptor(const char *p, long left) {
-    const Descriptor d{reinterpret_cast<uint64_t>(p), left <= 0 ? 0u : left < 0xffffffffL ? (uint32_t)left : 0xffffffffu, 0x00027000u};
+    const long words = (left + 3) & ~3L;
+    const Descriptor d{reinterpret_cast<uint64_t>(p), left <= 0 ? 0u : words < 0xffffffffL ? (uint32_t)words : 0xffffffffu, 0x00027000u};
     return __builtin_bit_cast(i32x4, d);
 }
 // 16 bytes a lane from base + offset to the 1024 bytes of LDS at `to` (a wave's); no register is written

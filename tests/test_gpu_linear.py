@@ -312,3 +312,29 @@ def test_derivative_far_from_zero(gpu, rows, k, n, act, dtype):
     want = torch.autograd.grad(linear_act(*leaves), leaves, torch.where(sign > 0, dy, torch.zeros_like(dy)))
     for g, h in zip(got, want):
         assert torch.equal(g, h)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows,k,n,more", [(300, 515, 264, 5), (1000, 1027, 130, 5), (2050, 71, 72, 1), (201, 72, 136, 8), (130, 264, 257, 8)])
+def test_aligned_rows_with_gaps_and_expanded_rows(rows, k, n, more, dtype, gpu):
+    """Views whose rows begin at multiples of 16 bytes, of odd and even widths, with NaN between them (the last value of an odd width shares its
+    word with nothing that exists); x, the gradient and the residual as one row expanded."""
+    from addernetcuda_amd.linear import linear_act
+    x, w, b, r, dy = make(rows, k, n, dtype)
+
+    def gap(t):
+        wide = -(-(t.shape[1] + more) // 8) * 8
+        big = torch.full((t.shape[0], wide), float("nan"), dtype=dtype, device="cuda")
+        big[:, :t.shape[1]] = t
+        return big[:, :t.shape[1]]
+
+    row = lambda t: t[:1].expand(t.shape[0], t.shape[1])
+    for lay_x, lay_r, lay_dy in [(gap, gap, gap), (row, row, gap), (gap, gap, row), (row, gap, row)]:
+        for act in ("none", "gelu"):
+            xs, rs, ds = lay_x(x), lay_r(r), lay_dy(dy)
+            want = B.linear(xs, w, b, rs, ds, act)
+            leaves = [xs.detach().requires_grad_(True), w.detach().requires_grad_(True), b.detach().requires_grad_(True)]
+            y = linear_act(leaves[0], leaves[1], leaves[2], rs, act)
+            B.within(y, want["y"], "y")
+            for name, t in zip(("gx", "gw", "gb"), torch.autograd.grad(y, leaves, ds)):
+                B.within(t, want[name], name)
