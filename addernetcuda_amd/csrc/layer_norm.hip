@@ -31,6 +31,16 @@ __device__ __forceinline__ float row_sum(float v, float *lds) {
     return v;
 }
 
+// 1 / sqrt(var + eps) of a row from the sum of the squares of its values' differences from the (rounded) mean and the mean of those differences: `rest`
+// is the mean's rounding, without which a row whose values are large beside their spread loses its digits.  Where the squares leave the range of a
+// float the variance is infinite and the row becomes its bias, as the formula in float32 has it; where they are not numbers, nor is the row.
+__device__ __forceinline__ float norm_rstd(float squares, float inv, float &rest, float eps) {
+    const float mean = squares * inv, off = rest * rest;
+    const bool holds = mean < __builtin_inff() && off < __builtin_inff();
+    rest = holds ? rest : 0.f;
+    return 1.f / sqrtf((holds ? fmaxf(fmaf(squares, inv, -off), 0.f) : mean < __builtin_inff() ? off : mean) + eps);
+}
+
 template <class T, class W, int G>
 __global__ __launch_bounds__(G > kNormFwdThreads ? G : kNormFwdThreads) void layer_norm_fwd_kernel(
     const T *__restrict__ x, long x_stride, const W *__restrict__ w, const W *__restrict__ b, T *__restrict__ y,
@@ -70,9 +80,8 @@ __global__ __launch_bounds__(G > kNormFwdThreads ? G : kNormFwdThreads) void lay
                 r += d;
                 q = fmaf(d, d, q);
             }
-        // what is left of the differences' mean, mu's rounding: a row whose values are large beside their spread keeps its digits
         r = row_sum<G>(r, lds) * inv;
-        const float rs = 1.f / sqrtf(fmaxf(fmaf(row_sum<G>(q, lds), inv, -r * r), 0.f) + eps);
+        const float rs = norm_rstd(row_sum<G>(q, lds), inv, r, eps);
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             float o[V];
@@ -204,7 +213,7 @@ __global__ __launch_bounds__(kNormWide) void layer_norm_wide_fwd_kernel(const T 
             q = fmaf(d, d, q);
         }
         r = row_sum<kNormWide>(r, lds) * inv;
-        const float rs = 1.f / sqrtf(fmaxf(fmaf(row_sum<kNormWide>(q, lds), inv, -r * r), 0.f) + eps);
+        const float rs = norm_rstd(row_sum<kNormWide>(q, lds), inv, r, eps);
         for (int i = threadIdx.x; i < D; i += kNormWide)
             put(y + row * D + i, fmaf((ldf(px + i) - mu - r) * rs, w ? ldf(w + i) : 1.f, b ? ldf(b + i) : 0.f));
         if (mean && threadIdx.x == 0) {

@@ -221,3 +221,28 @@ def test_all_dimensions_normalised_of_matrices_with_gaps(a, d, kind, gpu):
     B.within(gx.view(1, -1), B.layer_norm(x, w.flatten(), b.flatten(), torch.ones_like(dy), EPS)["gx"], "gx of a sum")
     plain = LayerNorm((a, d), elementwise_affine=False)
     assert torch.equal(plain(gap(x.view(a, d))), plain(x.view(a, d)))
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=IDS)
+@pytest.mark.parametrize("d", [8, 264, 1032, 4100, 17000])
+def test_over_the_whole_range(d, kind, gpu):
+    """Where the squares of the differences leave a float's range the variance is infinite: the row is its bias, its gradient zero (and what the
+    others' are without it).  Below that, and where the differences' squares vanish beside eps, as the formula has it.  One value that is not
+    finite makes a row not a number, at any size."""
+    from addernetcuda_amd.layer_norm import layer_norm
+    x, w, b, dy = make(16, d, kind)
+    far = torch.tensor([3e20, 1e24, 1e28, 1e29, 1e30, 1e32, 1e33, 2e33], device="cuda")[:, None]
+    x[:8] = ((x[:8].float() + 3) * far).to(x.dtype)
+    x[8:10] = (x[8:10].float() * 2.0 ** 48).to(x.dtype)   # squares of 2^96 and their sums
+    x[10:12] = (x[10:12].float() * 2.0 ** -80).to(x.dtype)
+    x[12], x[13] = 1e33, -3e28   # constant
+    x[14], x[14, 1], x[15], x[15, d - 1] = 1e30, float("inf"), -1e33, float("nan")
+    leaf = x.detach().requires_grad_(True)
+    y = layer_norm(leaf, w, b, EPS)
+    gx, = torch.autograd.grad(y, leaf, dy)
+    assert torch.equal(y[:8], b.to(y.dtype).expand(8, d)) and not gx[:8].any()
+    assert torch.equal(y[12:14], b.to(y.dtype).expand(2, d))
+    assert torch.isnan(y[14:]).all()
+    want = B.layer_norm(x[8:12], w, b, dy[8:12], EPS)
+    B.within(y[8:12], want["y"], "y")
+    B.within(gx[8:12], want["gx"], "gx")
