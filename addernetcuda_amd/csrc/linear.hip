@@ -172,7 +172,8 @@ __global__ __launch_bounds__(256) void act_bwd_kernel(const T *__restrict__ dy, 
             if constexpr (keeps_half(sizeof(T), ACT)) unpack_half(u, w);
             else unpack(u, w);
 #pragma unroll
-            for (int e = 0; e < V; ++e) d[e] *= slope<kExactAct<T>>(w[e], ACT);
+            for (int e = 0; e < V; ++e)   // (a ReLU selects: where it is off, an infinite dy or one that is no number goes no further)
+                d[e] = ACT != Act::relu ? d[e] * slope<kExactAct<T>>(w[e], ACT) : w[e] <= 0.f ? 0.f : d[e];
             if (dz) store_part(dz + m * N + n, left, d);
         }
 #pragma unroll

@@ -43,10 +43,10 @@ __device__ __forceinline__ float activate(float z, Act act) {
         default: return z;
     }
 }
+// the derivative of a GELU or SiLU
 template <bool EXACT>
 __device__ __forceinline__ float slope(float z, Act act) {
     switch (act) {
-        case Act::relu: return z <= 0.f ? 0.f : 1.f;
         case Act::gelu: {
             float bell;
             const float p = normal_cdf<EXACT>(z, bell);

@@ -338,3 +338,20 @@ def test_aligned_rows_with_gaps_and_expanded_rows(rows, k, n, more, dtype, gpu):
             B.within(y, want["y"], "y")
             for name, t in zip(("gx", "gw", "gb"), torch.autograd.grad(y, leaves, ds)):
                 B.within(t, want[name], name)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("rows,k,n", [(1, 24, 17), (40, 24, 16), (300, 72, 130)])
+def test_relu_lets_nothing_through_where_it_is_off(rows, k, n, residual, dtype, gpu):
+    """Infinite gradients, and ones that are no numbers, at zeros of the result: as if they were zero there."""
+    from addernetcuda_amd.linear import linear_act
+    x, w, b, r, dy = make(rows, k, n, dtype)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    y = linear_act(*leaves, r if residual else None, "relu")
+    off = linear_act(x, w, b, None, "relu").detach() == 0
+    assert off.any()
+    kinds = torch.tensor([float("inf"), float("-inf"), float("nan"), 3.0], device="cuda").to(dtype)
+    broken = torch.where(off, kinds[torch.arange(rows * n, device="cuda").view(rows, n) % 4], dy)
+    for g, h in zip(torch.autograd.grad(y, leaves, broken, retain_graph=True), torch.autograd.grad(y, leaves, torch.where(off, torch.zeros_like(dy), dy))):
+        assert torch.isfinite(g).all() and torch.equal(g, h)
