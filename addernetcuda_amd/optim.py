@@ -140,6 +140,9 @@ class AdamW(torch.optim.AdamW):
                          foreach=False, fused=False, capturable=capturable)
         self.state_bits, self.min_8bit_size = state_bits, min_8bit_size
 
+    def __getstate__(self):   # (copies and pickles: the framework's optimizer keeps its own three parts and nothing else)
+        return {**super().__getstate__(), "state_bits": self.state_bits, "min_8bit_size": self.min_8bit_size}
+
     @staticmethod
     def _kernel_takes(group, params):
         if group["amsgrad"] or group["maximize"]:

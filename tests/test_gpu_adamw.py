@@ -309,3 +309,29 @@ def test_refusals(gpu):
         optim.state_values(torch.zeros(300, dtype=torch.int8, device="cuda"), torch.zeros(1, device="cuda"))
     with pytest.raises(RuntimeError, match="CUDA tensors"):
         optim.state_values(torch.zeros(3, dtype=torch.int8), torch.zeros(1))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("capturable", [False, True])
+@pytest.mark.parametrize("begun", [False, True])
+def test_copies_and_pickles_step_as_the_original(begun, capturable, bits, gpu):
+    import pickle
+    from addernetcuda_amd.optim import AdamW
+    ps = params(torch.float32, 4)
+    opt = AdamW(ps, lr=1e-2, state_bits=bits, min_8bit_size=300, capturable=capturable)
+    if begun:
+        set_grads(ps, 1)
+        opt.step()
+    others = [copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))]
+    for o in [opt] + others:
+        assert (o.state_bits, o.min_8bit_size) == (bits, 300)
+        set_grads(o.param_groups[0]["params"], 2)
+        o.step()
+    for o in others:
+        for p, q in zip(ps, o.param_groups[0]["params"]):
+            assert p is not q and torch.equal(p, q)
+            for name, value in opt.state[p].items():
+                other = o.state[q][name]
+                assert value == other if not isinstance(value, torch.Tensor) else torch.equal(value, other) and value.dtype == other.dtype
+        if capturable:
+            assert len({id(s["step"]) for s in o.state.values()}) == 1

@@ -152,3 +152,23 @@ def test_wrapped_and_transformed_calls_take_torchs_operators():
     _, tangent = torch.func.jvp(f, (x,), (torch.ones_like(x),))
     assert tangent.shape == (4, 3, 5)
     assert torch.autograd.gradgradcheck(lambda t: layer_norm(t, torch.ones(8, dtype=torch.float64)), (x[0].requires_grad_(True),))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_survives_copy_and_pickle(bits):
+    import copy
+    import pickle
+    from addernetcuda_amd.optim import AdamW
+    opt = AdamW([torch.nn.Parameter(torch.ones(5, 4))], lr=0.1, state_bits=bits, min_8bit_size=77)
+    for o in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        assert (o.state_bits, o.min_8bit_size) == (bits, 77)
+        p = o.param_groups[0]["params"][0]
+        p.grad = torch.ones_like(p)
+        if bits == 32:
+            o.step()
+            assert torch.allclose(p, torch.full_like(p, 0.899))
+        else:
+            with pytest.raises(RuntimeError, match="state_bits=8 needs"):
+                o.step()
+        o.load_state_dict(o.state_dict())
+        assert o.state_bits == bits
