@@ -89,6 +89,7 @@ class SGD(torch.optim.SGD):
 STATE_BLOCK = 256   # ADDER_STATE_BLOCK
 _PIECE = 1 << 30    # values of one entry of the kernel's table; longer tensors take several
 _CODES = {"exp_avg": torch.int8, "exp_avg_sq": torch.uint8}
+_MOMENTS = ("exp_avg", "exp_avg_sq", "max_exp_avg_sq")   # that the framework's step holds in the parameter's type
 
 
 def state_values(codes, scales, dtype=torch.float32):
@@ -174,15 +175,19 @@ class AdamW(torch.optim.AdamW):
         return state
 
     def load_state_dict(self, state_dict):
-        """As ``torch.optim.Optimizer.load_state_dict``, but 8-bit moments stay codes, and the others become float32."""
+        """As ``torch.optim.Optimizer.load_state_dict``, but 8-bit moments stay codes, and those of parameters that the kernel takes are
+        float32."""
         super().load_state_dict(state_dict)
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         own = [p for g in self.param_groups for p in g["params"]]
         for i, p in zip(saved, own):
             for name, value in state_dict["state"].get(i, {}).items():
-                if isinstance(value, torch.Tensor) and name != "step":
-                    coded = value.dtype in (torch.int8, torch.uint8)
-                    self.state[p][name] = value.to(device=p.device, dtype=value.dtype if coded else torch.float32, copy=True)
+                if not isinstance(value, torch.Tensor) or name == "step":
+                    continue
+                if value.dtype in (torch.int8, torch.uint8):
+                    self.state[p][name] = value.to(device=p.device, copy=True)
+                elif (p.is_cuda and p.dtype in _ADAMW_TYPES) or name.endswith("_scale"):   # (the others have their parameter's type by now)
+                    self.state[p][name] = value.to(device=p.device, dtype=torch.float32, copy=True)
         for group in self.param_groups:   # parameters of one count share its tensor again (see _kernel_step)
             if group["capturable"]:
                 shared = {}
@@ -210,7 +215,7 @@ class AdamW(torch.optim.AdamW):
                 self._make_states(group, params)
                 if not self._kernel_step(group, params):
                     raise RuntimeError("AdamW: the state does not fit its parameters")
-            elif self.state_bits == 8:
+            elif self.state_bits == 8 or any(self.state[p]["exp_avg"].dtype == torch.int8 for p in params if self.state.get(p)):
                 raise RuntimeError("state_bits=8 needs contiguous float32 or bfloat16 GPU parameters with gradients of their type, on one device")
             else:
                 rest.append(group)
@@ -218,10 +223,14 @@ class AdamW(torch.optim.AdamW):
             for group in rest:
                 for p in group["params"]:
                     state = self.state.get(p)
-                    if state:   # (a tensor of its own for each: the framework counts them one by one)
-                        step = state["step"]
-                        state["step"] = (step.clone() if isinstance(step, torch.Tensor) else
-                                         torch.tensor(float(step), device=p.device if group["capturable"] else "cpu"))
+                    if not state or p.grad is None:
+                        continue
+                    for name in _MOMENTS:
+                        if name in state and state[name].dtype != p.dtype:
+                            state[name] = state[name].to(p.dtype)
+                    step = state["step"]   # (a tensor of its own for each: the framework counts them one by one)
+                    state["step"] = (step.clone() if isinstance(step, torch.Tensor) else
+                                     torch.tensor(float(step), device=p.device if group["capturable"] else "cpu"))
             kept = self.param_groups
             try:
                 self.param_groups = rest

@@ -335,3 +335,32 @@ def test_copies_and_pickles_step_as_the_original(begun, capturable, bits, gpu):
                 assert value == other if not isinstance(value, torch.Tensor) else torch.equal(value, other) and value.dtype == other.dtype
         if capturable:
             assert len({id(s["step"]) for s in o.state.values()}) == 1
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("capturable", [False, True])
+def test_gradients_that_the_kernel_leaves_in_either_type(capturable, dtype, gpu):
+    """One gradient that is not contiguous sends its group to torch for that step, where moments have the parameter's type; before and behind it
+    the kernel's are float32.  What torch does with the same state is what comes out."""
+    from addernetcuda_amd.optim import AdamW
+    a = params(dtype, 3, [(40, 50), (30, 20), (700,)])
+    o = AdamW(a, lr=1e-2, weight_decay=0.1, capturable=capturable)
+    for t in range(6):
+        set_grads(a, t)
+        if t in (2, 3):
+            b = [torch.nn.Parameter(p.detach().clone()) for p in a]
+            r = torch.optim.AdamW(b, lr=1e-2, weight_decay=0.1, foreach=False, capturable=capturable)
+            for p, q in zip(a, b):
+                q.grad = p.grad.clone()
+                r.state[q] = {name: value.detach().clone().to(dtype) for name, value in o.state[p].items() if name != "step"}
+                r.state[q]["step"] = torch.tensor(float(t), device="cuda" if capturable else "cpu")
+            a[1].grad = a[1].grad.t().contiguous().t()
+        o.step()
+        assert all(float(o.state[p]["step"]) == t + 1 for p in a)
+        if t in (2, 3):
+            r.step()
+            for p, q in zip(a, b):
+                assert o.state[p]["exp_avg"].dtype == dtype and torch.equal(o.state[p]["exp_avg"], r.state[q]["exp_avg"])
+                assert torch.equal(o.state[p]["exp_avg_sq"], r.state[q]["exp_avg_sq"]) and torch.equal(p, q)
+        else:
+            assert all(o.state[p]["exp_avg"].dtype == torch.float32 for p in a)

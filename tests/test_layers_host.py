@@ -172,3 +172,41 @@ def test_adamw_survives_copy_and_pickle(bits):
                 o.step()
         o.load_state_dict(o.state_dict())
         assert o.state_bits == bits
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16, torch.float64])
+@pytest.mark.parametrize("amsgrad", [False, True])
+def test_adamw_on_the_cpu_resumes_as_torchs(amsgrad, dtype):
+    """Step, save, load, step: the same numbers and the same types of state as torch.optim.AdamW, whose moments have the parameter's type."""
+    from addernetcuda_amd.optim import AdamW
+    results = []
+    for kind in (AdamW, torch.optim.AdamW):
+        p = torch.nn.Parameter(torch.linspace(-1, 1, 30).to(dtype).view(5, 6))
+        opt = kind([p], lr=0.03, amsgrad=amsgrad)
+        for t in range(4):
+            p.grad = (torch.linspace(1, 2, 30).view(5, 6) / (t + 1)).sin().to(dtype)
+            opt.step()
+            if t == 1:
+                saved = opt.state_dict()
+                opt = kind([p], lr=0.03, amsgrad=amsgrad)
+                opt.load_state_dict(saved)
+        results.append((p, opt.state[p]))
+    (p, mine), (q, theirs) = results
+    assert torch.equal(p, q) and mine.keys() == theirs.keys()
+    for name, value in theirs.items():
+        assert mine[name].dtype == value.dtype and torch.equal(mine[name], value), name
+
+
+def test_adamw_refuses_codes_of_parameters_that_the_kernel_does_not_take():
+    from addernetcuda_amd.optim import AdamW
+    p = torch.nn.Parameter(torch.ones(300))
+    opt = AdamW([p])
+    opt.load_state_dict({"state": {0: {"step": 3, "exp_avg": torch.ones(300, dtype=torch.int8), "exp_avg_scale": torch.ones(2),
+                                       "exp_avg_sq": torch.ones(300, dtype=torch.uint8), "exp_avg_sq_scale": torch.ones(2)}},
+                         "param_groups": opt.state_dict()["param_groups"]})
+    p.grad = torch.ones_like(p)
+    with pytest.raises(RuntimeError, match="state_bits=8 needs"):
+        opt.step()
+    state = opt.state[p]
+    assert torch.equal(p, torch.ones(300)) and state["exp_avg"].dtype == torch.int8 and state["exp_avg_sq"].dtype == torch.uint8
+    assert state["exp_avg_scale"].dtype == torch.float32
