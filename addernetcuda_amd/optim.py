@@ -19,6 +19,20 @@ from ._lib import lib, check, nodes, stream_ptr, on_device
 _MAX = 96   # ADDER_SGD_BATCH_MAX
 
 
+def _torch_step(kind, optimizer, groups):
+    """``kind.step`` for these groups alone.  Hooks belong to the step that this one is part of: the framework wraps a class's ``step`` once one of its
+    own has been made, and would run them again."""
+    step = kind.step
+    if getattr(step, "hooked", False):
+        step = step.__wrapped__
+    kept = optimizer.param_groups
+    try:
+        optimizer.param_groups = groups
+        step(optimizer)
+    finally:
+        optimizer.param_groups = kept
+
+
 class SGD(torch.optim.SGD):
     def __init__(self, params, lr=1e-3, momentum=0.0, dampening=0.0, weight_decay=0.0, nesterov=False, *,
                  maximize=False):
@@ -77,12 +91,7 @@ class SGD(torch.optim.SGD):
                                                           float(group["weight_decay"]), stream_ptr(dev)),
                           "adder_sgd_momentum_step_f32")
         if rest:   # the groups the kernel does not take: the framework's own update, group by group
-            kept = self.param_groups
-            try:
-                self.param_groups = rest
-                super().step()
-            finally:
-                self.param_groups = kept
+            _torch_step(torch.optim.SGD, self, rest)
         return loss
 
 
@@ -231,12 +240,7 @@ class AdamW(torch.optim.AdamW):
                     step = state["step"]   # (a tensor of its own for each: the framework counts them one by one)
                     state["step"] = (step.clone() if isinstance(step, torch.Tensor) else
                                      torch.tensor(float(step), device=p.device if group["capturable"] else "cpu"))
-            kept = self.param_groups
-            try:
-                self.param_groups = rest
-                super().step()
-            finally:
-                self.param_groups = kept
+            _torch_step(torch.optim.AdamW, self, rest)
         return loss
 
     def _make_states(self, group, params):

@@ -210,3 +210,24 @@ def test_adamw_refuses_codes_of_parameters_that_the_kernel_does_not_take():
     state = opt.state[p]
     assert torch.equal(p, torch.ones(300)) and state["exp_avg"].dtype == torch.int8 and state["exp_avg_sq"].dtype == torch.uint8
     assert state["exp_avg_scale"].dtype == torch.float32
+
+
+@pytest.mark.parametrize("name,kw", [("AdamW", {}), ("SGD", {"momentum": 0.9})])
+@pytest.mark.parametrize("made", [False, True])
+def test_hooks_run_once_a_step(made, name, kw):
+    """Also where the whole step is torch's, and an optimizer of torch's own class has been made in the process."""
+    from addernetcuda_amd import optim
+    if made:
+        getattr(torch.optim, name)([torch.nn.Parameter(torch.ones(3))], lr=0.1)
+    p = torch.nn.Parameter(torch.ones(3))
+    opt = getattr(optim, name)([p], lr=0.1, **kw)
+    calls = []
+    opt.register_step_pre_hook(lambda *a: calls.append("pre"))
+    opt.register_step_post_hook(lambda *a: calls.append("post"))
+    for t in range(2):
+        p.grad = torch.ones(3)
+        opt.step()
+    assert calls == ["pre", "post"] * 2 and len(opt.param_groups) == 1 and (p < 0.95).all()
+    with torch.no_grad():
+        before = p.clone()
+    assert opt.step(lambda: torch.tensor(5.0)) == 5.0 and not torch.equal(p, before)   # (still without gradients in the update)
