@@ -187,6 +187,8 @@ class AdamW(torch.optim.AdamW):
         """As ``torch.optim.Optimizer.load_state_dict``, but 8-bit moments stay codes, and those of parameters that the kernel takes are
         float32."""
         super().load_state_dict(state_dict)
+        for group in self.param_groups:   # (the framework's fused step wants counts on the device, which the kernel's numbers are not)
+            group["fused"] = group["fused"] and False
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         own = [p for g in self.param_groups for p in g["params"]]
         for i, p in zip(saved, own):

@@ -364,3 +364,28 @@ def test_gradients_that_the_kernel_leaves_in_either_type(capturable, dtype, gpu)
                 assert torch.equal(o.state[p]["exp_avg_sq"], r.state[q]["exp_avg_sq"]) and torch.equal(p, q)
         else:
             assert all(o.state[p]["exp_avg"].dtype == torch.float32 for p in a)
+
+
+@pytest.mark.parametrize("kind", ["foreach", "fused"])
+def test_a_state_of_torchs_other_steps_goes_both_ways(kind, gpu):
+    """The state of torch's fused or foreach optimizer is taken on by the kernel, and by torch for a gradient that the kernel leaves."""
+    from addernetcuda_amd.optim import AdamW
+    shapes = [(40, 50), (30, 20)]
+    a, b = params(torch.float32, 3, shapes), params(torch.float32, 3, shapes)
+    r = torch.optim.AdamW(b, lr=1e-2, **{kind: True})
+    for t in range(5):
+        for ps in (a, b):
+            set_grads(ps, t)
+        r.step()
+        if t == 0:
+            o = AdamW(a, lr=1e-2)
+            o.load_state_dict(copy.deepcopy(r.state_dict()))
+            with torch.no_grad():
+                for p, q in zip(a, b):
+                    p.copy_(q)
+            continue
+        if t == 2:
+            a[1].grad = a[1].grad.t().contiguous().t()
+        o.step()
+        for p, q in zip(a, b):
+            assert torch.allclose(p, q, rtol=1e-6, atol=1e-6), t
