@@ -200,7 +200,7 @@ class AdamW(torch.optim.AdamW):
                 elif (p.is_cuda and p.dtype in _ADAMW_TYPES) or name.endswith("_scale"):   # (the others have their parameter's type by now)
                     self.state[p][name] = value.to(device=p.device, dtype=torch.float32, copy=True)
         for group in self.param_groups:   # parameters of one count share its tensor again (see _kernel_step)
-            if group["capturable"]:
+            if group["capturable"] and not (group["amsgrad"] or group["maximize"]):
                 shared = {}
                 for p in group["params"]:
                     if self.state.get(p):
@@ -231,40 +231,70 @@ class AdamW(torch.optim.AdamW):
             else:
                 rest.append(group)
         if rest:   # the groups the kernel does not take: the framework's own update, group by group
-            for group in rest:
-                for p in group["params"]:
-                    state = self.state.get(p)
-                    if not state or p.grad is None:
-                        continue
-                    for name in _MOMENTS:
-                        if name in state and state[name].dtype != p.dtype:
-                            state[name] = state[name].to(p.dtype)
-                    step = state["step"]   # (a tensor of its own for each: the framework counts them one by one)
-                    state["step"] = (step.clone() if isinstance(step, torch.Tensor) else
-                                     torch.tensor(float(step), device=p.device if group["capturable"] else "cpu"))
+            shared = [pair for group in rest for pair in self._as_torchs(group)]
             _torch_step(torch.optim.AdamW, self, rest)
+            for count, states in shared:
+                count.add_(1)
+                for state in states:
+                    state["step"] = count
         return loss
+
+    def _as_torchs(self, group):
+        """Prepares the states of a group for the framework's step: moments in the parameter's type, and a count of its own for each parameter, which
+        the framework raises one by one.  Returns the counts on the device that were shared, with the states that go back to them."""
+        self._part_counts(group)
+        users = {}
+        for p in group["params"]:
+            state = self.state.get(p)
+            if not state or p.grad is None:
+                continue
+            for name in _MOMENTS:
+                if name in state and state[name].dtype != p.dtype:
+                    state[name] = state[name].to(p.dtype)
+            step = state["step"]
+            if not isinstance(step, torch.Tensor):
+                state["step"] = torch.tensor(float(step), device=p.device if group["capturable"] else "cpu")
+            else:
+                users.setdefault(id(step), (step, []))[1].append(state)
+        shared = [(step, states) for step, states in users.values() if len(states) > 1]
+        for step, states in shared:
+            for state in states:
+                state["step"] = step.clone()
+        return shared if group["capturable"] else []
+
+    def _part_counts(self, group):
+        """Parameters without a gradient now do not count on with the others: those of one count have a copy of it together from here on."""
+        of = self.state
+        used = {id(of[p]["step"]) for p in group["params"] if p.grad is not None and of.get(p)}
+        left = {}
+        for p in group["params"]:
+            if p.grad is None and of.get(p) and id(of[p]["step"]) in used and isinstance(of[p]["step"], torch.Tensor):
+                step = of[p]["step"]
+                if id(step) not in left:
+                    left[id(step)] = step.clone()
+                of[p]["step"] = left[id(step)]
 
     def _make_states(self, group, params):
         """The states of ``params`` as the kernel wants them: moments as float32 or codes, and the step count as an int or, with
         ``capturable``, as a tensor on the device that the parameters of one count share (one tiny launch counts them all)."""
         of, capturable, dev = self.state, group["capturable"], params[0].device
         fresh = torch.zeros((), dtype=torch.float32, device=dev) if capturable else 0
+        counts = {}   # made here, by their value
         for p in params:
             state = of[p] or self._new_state(p, fresh)
             step = state["step"]
             if not capturable:
                 state["step"] = int(step)
             elif not (isinstance(step, torch.Tensor) and step.is_cuda and step.dtype == torch.float32):
-                state["step"] = torch.tensor(float(step), dtype=torch.float32, device=dev)
+                step = float(step)
+                if step not in counts:
+                    counts[step] = torch.tensor(step, dtype=torch.float32, device=dev)
+                state["step"] = counts[step]
             for name in _CODES:   # (what torch.optim.AdamW made for a group that it had to take before)
                 if state[name].dtype not in (torch.float32, _CODES[name]):
                     state[name] = state[name].float()
-        if capturable:   # parameters without a gradient now do not count on with the others
-            used = {id(of[p]["step"]) for p in params}
-            for p in group["params"]:
-                if p.grad is None and of.get(p) and id(of[p]["step"]) in used:
-                    of[p]["step"] = of[p]["step"].clone()
+        if capturable:
+            self._part_counts(group)
 
     def _kernel_step(self, group, params):
         """The launches of one step, by csrc/nodes.cpp: False, and nothing done, where something is not as the kernels want it."""

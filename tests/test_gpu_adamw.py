@@ -389,3 +389,53 @@ def test_a_state_of_torchs_other_steps_goes_both_ways(kind, gpu):
         o.step()
         for p, q in zip(a, b):
             assert torch.allclose(p, q, rtol=1e-6, atol=1e-6), t
+
+
+def test_counts_that_part_are_as_few_as_they_differ(gpu):
+    """Parameters that stay behind together share one count; a step that torch takes leaves the counts shared; all of them are right, also in a
+    captured step that torch takes."""
+    from addernetcuda_amd.optim import AdamW
+    ps = params(torch.float32, 3, [(40, 50)] * 6)
+    opt = AdamW(ps, lr=1e-3, capturable=True)
+    count = lambda: (len({id(opt.state[p]["step"]) for p in ps}), [int(opt.state[p]["step"]) for p in ps])
+
+    def step(which, across=False, keep=False):
+        if not keep:
+            set_grads(ps, 1)
+            for i, p in enumerate(ps):
+                p.grad = None if i not in which else p.grad.t().contiguous().t() if across else p.grad
+        opt.step()
+
+    step(range(6))
+    assert count() == (1, [1] * 6)
+    step(range(3))
+    assert count() == (2, [2, 2, 2, 1, 1, 1])
+    step(range(3, 6))
+    assert count() == (2, [2] * 6)
+    step(range(6), across=True)
+    assert count() == (2, [3] * 6)
+    step(range(6))
+    assert count() == (2, [4] * 6)
+    step((0, 1, 3), across=True)
+    assert count() == (4, [5, 5, 4, 5, 4, 4])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(range(6), across=True)
+        assert count() == (4, [6, 6, 5, 6, 5, 5])
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            step(range(6), keep=True)
+    torch.cuda.current_stream().wait_stream(side)
+    for t in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert count() == (4, [7 + t, 7 + t, 6 + t, 7 + t, 6 + t, 6 + t])
+    step(range(6))
+    assert count() == (4, [10, 10, 9, 10, 9, 9])
+    plain = AdamW(ps, lr=1e-3)   # a state that counted on the host, and from now on on the device
+    set_grads(ps, 5)
+    plain.step()
+    plain.param_groups[0]["capturable"] = True
+    plain.step()
+    assert len({id(plain.state[p]["step"]) for p in ps}) == 1 and int(plain.state[ps[0]]["step"]) == 2
