@@ -220,6 +220,8 @@ class AdamW(torch.optim.AdamW):
             params = [p for p in group["params"] if p.grad is not None]
             if not params:
                 continue
+            if not group["capturable"] and params[0].is_cuda and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("AdamW: a captured step counts on only where capturable=True keeps its count on the device")
             if self._kernel_step(group, params):
                 continue
             if self._kernel_takes(group, params):

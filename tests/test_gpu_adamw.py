@@ -439,3 +439,23 @@ def test_counts_that_part_are_as_few_as_they_differ(gpu):
     plain.param_groups[0]["capturable"] = True
     plain.step()
     assert len({id(plain.state[p]["step"]) for p in ps}) == 1 and int(plain.state[ps[0]]["step"]) == 2
+
+
+@pytest.mark.parametrize("begun", [False, True])
+def test_a_captured_step_needs_its_count_on_the_device(begun, gpu):
+    """As torch's own optimizer: a count on the host would be frozen into the graph."""
+    from addernetcuda_amd.optim import AdamW
+    ps = params(torch.float32, 3, [(40, 50), (7,)])
+    opt = AdamW(ps, lr=1e-3)
+    set_grads(ps, 1)
+    if begun:
+        opt.step()
+    before = [p.detach().clone() for p in ps]
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="capturable=True"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(ps, before)) and len(opt.state) == (len(ps) if begun else 0)
+    opt.step()
+    assert all(opt.state[p]["step"] == 1 + begun for p in ps)
