@@ -314,12 +314,12 @@ struct Batch {   // what one step count, storage type of the parameter and of it
 
 PyObject *key(const char *name) { return PyUnicode_InternFromString(name); }
 
-// adamw_step(params, states, capturable, lr, lr_device, beta1, beta2, eps, weight_decay, piece): one step of parameters with gradients, with their
+// adamw_step(params, states, capturable, lr, lr_device, beta1, beta2, eps, weight_decay, piece, groups): one step of parameters with gradients, with their
 // states (dicts).  False, and nothing done, where a parameter, a gradient or a state is not what the kernels take; an error where a state does not
 // fit its parameter.
 PyObject *py_adamw_step(PyObject *, PyObject *const *args, Py_ssize_t count) {
     HANDLE_TH_ERRORS
-    TORCH_CHECK(count == 10, "adamw_step: ten arguments");
+    TORCH_CHECK(count == 11, "adamw_step: eleven arguments");
     static PyObject *const names[] = {key("step"), key("exp_avg"), key("exp_avg_sq"), key("exp_avg_scale"), key("exp_avg_sq_scale")};
     PyObject *params = args[0], *states = args[1];
     TORCH_CHECK(PyList_Check(params) && PyList_Check(states) && PyList_GET_SIZE(params) == PyList_GET_SIZE(states), "adamw_step: two lists");
@@ -327,7 +327,7 @@ PyObject *py_adamw_step(PyObject *, PyObject *const *args, Py_ssize_t count) {
     const double lr = PyFloat_AsDouble(args[3]);
     const float *lr_device = reinterpret_cast<const float *>(PyLong_AsSize_t(args[4]));
     const double b1 = PyFloat_AsDouble(args[5]), b2 = PyFloat_AsDouble(args[6]), eps = PyFloat_AsDouble(args[7]), decay = PyFloat_AsDouble(args[8]);
-    const int64_t piece = PyLong_AsLongLong(args[9]);
+    const int64_t piece = PyLong_AsLongLong(args[9]), groups = PyLong_AsLongLong(args[10]);
     if (PyErr_Occurred()) return nullptr;
     TORCH_CHECK(piece > 0 && piece <= kPieceMost && piece % ADDER_STATE_BLOCK == 0, "adamw_step: pieces of whole blocks");
     const Py_ssize_t all = PyList_GET_SIZE(params);
@@ -415,8 +415,13 @@ PyObject *py_adamw_step(PyObject *, PyObject *const *args, Py_ssize_t count) {
         }
         const int type = b.type == at::kFloat ? ADDER_TYPE_F32 : ADDER_TYPE_BF16;
         const size_t most = b.coded ? ADDER_ADAMW_8BIT_BATCH_MAX : ADDER_ADAMW_BATCH_MAX;
-        for (size_t i = 0; i < b.n.size(); i += most) {
-            const int k = (int)(b.n.size() - i < most ? b.n.size() - i : most);
+        for (size_t i = 0, next; i < b.n.size(); i = next) {   // as many as a table holds and a launch has workgroups for
+            int64_t used = 0;
+            for (next = i; next < b.n.size() && next - i < most; ++next) {
+                used += (b.n[next] + 1023) / 1024;
+                if (next > i && used > groups) break;
+            }
+            const int k = (int)(next - i);
             const void *const *g = const_cast<const void *const *>(b.g.data() + i);
             if (b.coded)
                 check(lib.adamw8(k, b.p.data() + i, g, reinterpret_cast<signed char *const *>(b.m.data() + i),

@@ -97,6 +97,7 @@ class SGD(torch.optim.SGD):
 
 STATE_BLOCK = 256   # ADDER_STATE_BLOCK
 _PIECE = 1 << 30    # values of one entry of the kernel's table; longer tensors take several
+_GROUPS = (1 << 24) - 1   # workgroups, of 1024 values at least, that the entry points take in one launch
 _CODES = {"exp_avg": torch.int8, "exp_avg_sq": torch.uint8}
 _MOMENTS = ("exp_avg", "exp_avg_sq", "max_exp_avg_sq")   # that the framework's step holds in the parameter's type
 
@@ -318,4 +319,4 @@ class AdamW(torch.optim.AdamW):
         b1, b2 = group["betas"]
         if isinstance(b1, torch.Tensor) or isinstance(b2, torch.Tensor):
             return False
-        return nodes.adamw_step(params, states, capturable, rate, rate_at, b1, b2, group["eps"], group["weight_decay"], _PIECE)
+        return nodes.adamw_step(params, states, capturable, rate, rate_at, b1, b2, group["eps"], group["weight_decay"], _PIECE, _GROUPS)

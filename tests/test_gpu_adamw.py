@@ -459,3 +459,21 @@ def test_a_captured_step_needs_its_count_on_the_device(begun, gpu):
     assert all(torch.equal(p, q) for p, q in zip(ps, before)) and len(opt.state) == (len(ps) if begun else 0)
     opt.step()
     assert all(opt.state[p]["step"] == 1 + begun for p in ps)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_more_workgroups_than_one_launch_takes(bits, gpu, monkeypatch):
+    """Tensors that are too many values for one launch together go into several: the same bits as in one."""
+    from addernetcuda_amd import optim
+    outs = []
+    for groups in (optim._GROUPS, 3, 1):
+        monkeypatch.setattr(optim, "_GROUPS", groups)
+        ps = params(torch.float32, 5, [(5000,), (7,), (1024, 2), (1024,), (3,), (2000,), (9, 9)])
+        opt = optim.AdamW(ps, lr=1e-2, state_bits=bits, min_8bit_size=600)
+        for t in range(2):
+            set_grads(ps, t)
+            opt.step()
+        outs.append([p.detach().clone() for p in ps] + [opt.state[p]["exp_avg"] for p in ps])
+    for other in outs[1:]:
+        for a, b in zip(outs[0], other):
+            assert torch.equal(a, b)

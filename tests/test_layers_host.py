@@ -231,3 +231,18 @@ def test_hooks_run_once_a_step(made, name, kw):
     with torch.no_grad():
         before = p.clone()
     assert opt.step(lambda: torch.tensor(5.0)) == 5.0 and not torch.equal(p, before)   # (still without gradients in the update)
+
+
+def test_adamw_hands_no_launch_more_than_it_takes():
+    """The limit that the optimizer cuts its launches at is the entry points' own: one value more is refused (before the pointers are looked at)."""
+    from addernetcuda_amd import optim
+    from addernetcuda_amd._lib import lib
+    piece = optim._PIECE
+    most = optim._GROUPS * 1024
+    sizes = [piece] * (most // piece) + [most % piece + 1]
+    ps = (P * len(sizes))()
+    n = (ctypes.c_long * len(sizes))(*sizes)
+    call = lambda k: lib.adder_adamw_step(k, ps, ps, ps, ps, n, None, 0.1, 0.9, 0.99, 1e-8, 0.0, 1, None, 0, None)
+    assert call(len(sizes)) == -3
+    n[len(sizes) - 1] -= 1
+    assert call(len(sizes)) == -1
