@@ -246,3 +246,33 @@ def test_over_the_whole_range(d, kind, gpu):
     want = B.layer_norm(x[8:12], w, b, dy[8:12], EPS)
     B.within(y[8:12], want["y"], "y")
     B.within(gx[8:12], want["gx"], "gx")
+
+
+@pytest.mark.parametrize("affine", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("within_type", [torch.bfloat16, torch.float16])
+def test_autocast_as_torchs(within_type, dtype, affine, gpu):
+    """In place of nn.LayerNorm: float32 out of whatever goes in, gradients of the inputs' own types."""
+    from addernetcuda_amd.layer_norm import LayerNorm
+    x, w, b, dy = make(33, 264, KINDS[0])
+    x = x.to(dtype)
+    mine, theirs = (kind(264, elementwise_affine=affine).cuda() for kind in (LayerNorm, torch.nn.LayerNorm))
+    if affine:
+        for m in (mine, theirs):
+            m.weight.data.copy_(w)
+            m.bias.data.copy_(b)
+    outs = []
+    for m in (mine, theirs):
+        leaf = x.clone().requires_grad_(True)
+        with torch.autocast("cuda", dtype=within_type):
+            y = m(leaf)
+        outs.append([y, *torch.autograd.grad(y, [leaf, *m.parameters()], dy)])
+    for p, q in zip(*outs):
+        assert p.dtype == q.dtype
+    want = B.layer_norm(x.float(), w if affine else None, b if affine else None, dy, EPS)
+    assert outs[0][0].dtype == torch.float32
+    B.within(outs[0][0], want["y"], "y")
+    value, off = want["gx"]
+    B.within(outs[0][1], (value, off + (value.abs() * B.V + 2.0 ** -25 if dtype != torch.float32 else 0)), "gx")
+    for name, t in zip(("gw", "gb"), outs[0][2:]):
+        B.within(t, want[name], name)
