@@ -66,7 +66,8 @@ def linear_act(x, weight, bias=None, residual=None, act="none"):
 
 class LinearAct(nn.Linear):
     """``nn.Linear`` (same parameters and state_dict keys) with the activation behind it and, in the call, a shortcut that is added to
-    the result: ``layer(x, residual=shortcut)``.  float32 parameters are rounded to bfloat16 for a bfloat16 input."""
+    the result: ``layer(x, residual=shortcut)``.  float32 parameters are rounded to bfloat16 for a bfloat16 input (inside ``torch.autocast`` to
+    its type, as by ``nn.Linear``)."""
 
     def __init__(self, in_features, out_features, bias=True, act="none", device=None, dtype=None):
         if act not in ACTS:
@@ -76,7 +77,8 @@ class LinearAct(nn.Linear):
 
     def forward(self, x, residual=None):
         w, b = self.weight, self.bias
-        if x.dtype == torch.bfloat16 and w.dtype == torch.float32:
+        kind = x.device.type
+        if x.dtype == torch.bfloat16 and w.dtype == torch.float32 and not (kind in ("cuda", "cpu") and torch.is_autocast_enabled(kind)):
             w, b = w.to(x.dtype), None if b is None else b.to(x.dtype)
         return linear_act(x, w, b, residual=residual, act=self.act)
 

@@ -246,3 +246,17 @@ def test_adamw_hands_no_launch_more_than_it_takes():
     assert call(len(sizes)) == -3
     n[len(sizes) - 1] -= 1
     assert call(len(sizes)) == -1
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("within", [torch.float16, torch.bfloat16])
+def test_linear_act_inside_autocast_rounds_its_weights_once(within, dtype):
+    """To autocast's type, as nn.Linear: not through bfloat16 on the way to float16."""
+    from addernetcuda_amd.linear import LinearAct
+    mine, theirs = LinearAct(64, 48), torch.nn.Linear(64, 48)
+    theirs.load_state_dict(mine.state_dict())
+    x = torch.randn(5, 64).to(dtype)
+    with torch.autocast("cpu", dtype=within):
+        a, b = mine(x), theirs(x)
+    assert a.dtype == b.dtype and torch.equal(a, b)
+    assert LinearAct(4, 3, device="meta")(torch.empty(2, 4, dtype=torch.bfloat16, device="meta")).shape == (2, 3)
