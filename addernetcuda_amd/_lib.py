@@ -114,11 +114,17 @@ class BnLinks(ctypes.Structure):
                 ("out_dbeta", ctypes.c_void_p)]
 
 
-if not os.path.exists(os.path.join(_HERE, "_nodes.so")):
-    raise ImportError(f"{os.path.join(_HERE, '_nodes.so')} is missing: build it with `python addernetcuda_amd/build.py`.")
-from . import _nodes as nodes   # noqa: E402  (csrc/nodes.cpp: runs on the library that is loaded here)
-
-nodes.bind({_name: ctypes.cast(getattr(lib, _name), ctypes.c_void_p).value for _name in _SIGNATURES})
+@functools.lru_cache(maxsize=None)
+def nodes():
+    """The host module of the layers beside the adder layers (csrc/nodes.cpp), on the library that is loaded here.  Loaded where the first of them
+    runs: it is compiled against torch's C++ interface, which nothing else here needs."""
+    try:
+        from . import _nodes
+    except ImportError as e:
+        raise ImportError(f"{os.path.join(_HERE, '_nodes.so')} is missing or does not fit this torch: build it with "
+                          "`python addernetcuda_amd/build.py`.") from e
+    _nodes.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _SIGNATURES})
+    return _nodes
 
 
 def check(status, what):

@@ -23,7 +23,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
         x, weight, bias = (t.float() if t is not None and t.dtype in _BELOW_F32 else t for t in (x, weight, bias))
     of = weight if weight is not None else bias
     if plain_tensors(x, weight, bias) and x.is_cuda and x.dtype in TYPES and (of is None or of.numel()) and x.shape[-1:] != (0,):
-        return nodes.layer_norm(x, weight, bias, eps)
+        return nodes().layer_norm(x, weight, bias, eps)
     if not eps >= 0:
         raise RuntimeError(f"eps must not be negative, got {eps}")
     shape = tuple(of.shape) if of is not None else tuple(x.shape[-1:])

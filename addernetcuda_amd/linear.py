@@ -60,7 +60,7 @@ def linear_act(x, weight, bias=None, residual=None, act="none"):
         if torch.is_autocast_enabled("cuda"):
             return _autocast_linear_act(x, weight, bias, residual, act)
         if x.dtype in TYPES and weight.numel():
-            return nodes.linear_act(x, weight, bias, residual, code)
+            return nodes().linear_act(x, weight, bias, residual, code)
     return _torch_linear_act(x, weight, bias, residual, act)
 
 

@@ -302,7 +302,7 @@ class AdamW(torch.optim.AdamW):
     def _kernel_step(self, group, params):
         """The launches of one step, by csrc/nodes.cpp: False, and nothing done, where something is not as the kernels want it."""
         lr, capturable, of = group["lr"], group["capturable"], self.state
-        if group["amsgrad"] or group["maximize"]:
+        if group["amsgrad"] or group["maximize"] or not params[0].is_cuda:
             return False
         states = [of[p] for p in params]
         if not all(states):
@@ -319,4 +319,4 @@ class AdamW(torch.optim.AdamW):
         b1, b2 = group["betas"]
         if isinstance(b1, torch.Tensor) or isinstance(b2, torch.Tensor):
             return False
-        return nodes.adamw_step(params, states, capturable, rate, rate_at, b1, b2, group["eps"], group["weight_decay"], _PIECE, _GROUPS)
+        return nodes().adamw_step(params, states, capturable, rate, rate_at, b1, b2, group["eps"], group["weight_decay"], _PIECE, _GROUPS)

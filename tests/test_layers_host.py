@@ -260,3 +260,51 @@ def test_linear_act_inside_autocast_rounds_its_weights_once(within, dtype):
         a, b = mine(x), theirs(x)
     assert a.dtype == b.dtype and torch.equal(a, b)
     assert LinearAct(4, 3, device="meta")(torch.empty(2, 4, dtype=torch.bfloat16, device="meta")).shape == (2, 3)
+
+
+def test_the_adder_layers_do_without_the_host_module():
+    """Where csrc/nodes.cpp is not built, or for another torch, everything but the layers that run on it imports and works."""
+    import subprocess
+    import sys
+    from tests.conftest import ROOT
+    code = """
+import sys
+sys.modules["addernetcuda_amd._nodes"] = None   # what an import of it then finds is an ImportError
+import torch
+from addernetcuda_amd import adder, models, optim, resnet20, train, _lib
+from addernetcuda_amd.linear import LinearAct
+models.token_mlp(width=16, layers=1)
+LinearAct(4, 3)(torch.ones(2, 4))
+p = torch.nn.Parameter(torch.ones(3))
+for opt in (optim.SGD([p], lr=0.1, momentum=0.9), optim.AdamW([p])):
+    for _ in range(2):
+        p.grad = torch.ones(3)
+        opt.step()
+try:
+    _lib.nodes()
+except ImportError as e:
+    assert "build.py" in str(e)
+    print("as it should be")
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True)
+    assert r.returncode == 0 and "as it should be" in r.stdout, r.stderr
+
+
+def test_the_library_is_linked_before_the_host_module_can_fail(monkeypatch):
+    import importlib.util
+    import os
+    from tests.conftest import ROOT
+    spec = importlib.util.spec_from_file_location("a_build", os.path.join(ROOT, "addernetcuda_amd", "build.py"))
+    build = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(build)
+    linked = []
+
+    def no_headers(verbose):
+        raise RuntimeError("g++ failed on nodes.cpp")
+
+    monkeypatch.setattr(build, "_compile", lambda src, verbose: src)
+    monkeypatch.setattr(build, "_build_nodes", no_headers)
+    monkeypatch.setattr(build.subprocess, "check_call", linked.append)
+    with pytest.raises(RuntimeError, match="nodes.cpp"):
+        build.build()
+    assert len(linked) == 1 and build.LIB in linked[0]
