@@ -50,6 +50,14 @@ void check(int status, const char *what) {
     TORCH_CHECK(false, what, ": ", text);
 }
 
+// The interpreter is free for other threads while this lives: a launch waits where the queue is full
+struct Released {
+    PyThreadState *const state = PyEval_SaveThread();
+    Released() = default;
+    Released(const Released &) = delete;
+    ~Released() { PyEval_RestoreThread(state); }
+};
+
 int type_of(const Tensor &t) { return t.scalar_type() == at::kBFloat16 ? ADDER_TYPE_BF16 : ADDER_TYPE_F32; }
 void *stream_of(const Tensor &t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 void *ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
@@ -200,11 +208,16 @@ PyObject *py_linear_act(PyObject *, PyObject *const *args, Py_ssize_t count) {
             residual = residual.expand(shape);
         }
     }
-    w = w.contiguous();
-    if (bias.defined()) bias = bias.contiguous();
-    const bool grad = at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad() || (bias.defined() && bias.requires_grad()) ||
-                                                     (residual.defined() && residual.requires_grad()));
-    return THPVariable_Wrap(grad ? LinearAct::apply(x, w, maybe(bias), maybe(residual), act) : linear_forward(x, w, bias, residual, act, nullptr));
+    Tensor y;
+    {
+        const Released released;
+        w = w.contiguous();
+        if (bias.defined()) bias = bias.contiguous();
+        const bool grad = at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad() || (bias.defined() && bias.requires_grad()) ||
+                                                         (residual.defined() && residual.requires_grad()));
+        y = grad ? LinearAct::apply(x, w, maybe(bias), maybe(residual), act) : linear_forward(x, w, bias, residual, act, nullptr);
+    }
+    return THPVariable_Wrap(std::move(y));
     END_HANDLE_TH_ERRORS
 }
 
@@ -293,10 +306,15 @@ PyObject *py_layer_norm(PyObject *, PyObject *const *args, Py_ssize_t count) {
     }
     int64_t width = 1;
     for (const int64_t d : shape) width *= d;
-    if (weight.defined()) weight = weight.contiguous();
-    if (bias.defined()) bias = bias.contiguous();
-    const bool grad = at::GradMode::is_enabled() && (x.requires_grad() || (weight.defined() && weight.requires_grad()) || (bias.defined() && bias.requires_grad()));
-    return THPVariable_Wrap(grad ? LayerNorm::apply(x, maybe(weight), maybe(bias), width, eps) : norm_forward(x, weight, bias, width, eps, nullptr, nullptr));
+    Tensor y;
+    {
+        const Released released;
+        if (weight.defined()) weight = weight.contiguous();
+        if (bias.defined()) bias = bias.contiguous();
+        const bool grad = at::GradMode::is_enabled() && (x.requires_grad() || (weight.defined() && weight.requires_grad()) || (bias.defined() && bias.requires_grad()));
+        y = grad ? LayerNorm::apply(x, maybe(weight), maybe(bias), width, eps) : norm_forward(x, weight, bias, width, eps, nullptr, nullptr);
+    }
+    return THPVariable_Wrap(std::move(y));
     END_HANDLE_TH_ERRORS
 }
 
@@ -310,6 +328,19 @@ struct Batch {   // what one step count, storage type of the parameter and of it
     bool coded;
     std::vector<void *> p, g, m, v, ms, vs;
     std::vector<long> n;
+};
+
+struct Held {   // references to objects, while this lives
+    std::vector<PyObject *> objects;
+    Held() = default;
+    Held(const Held &) = delete;
+    void add(PyObject *o) {
+        objects.push_back(o);
+        Py_INCREF(o);
+    }
+    ~Held() {
+        for (PyObject *o : objects) Py_DECREF(o);
+    }
 };
 
 PyObject *key(const char *name) { return PyUnicode_InternFromString(name); }
@@ -332,6 +363,12 @@ PyObject *py_adamw_step(PyObject *, PyObject *const *args, Py_ssize_t count) {
     TORCH_CHECK(piece > 0 && piece <= kPieceMost && piece % ADDER_STATE_BLOCK == 0, "adamw_step: pieces of whole blocks");
     const Py_ssize_t all = PyList_GET_SIZE(params);
     std::vector<Batch> batches;
+    Held held;   // what another thread could replace before it is launched: the states' tensors and the gradients
+    std::vector<Tensor> gradients;
+    held.objects.reserve(5 * all);
+    std::vector<long> counts;   // of this step
+    gradients.reserve(all);
+    counts.reserve(all);
     c10::Device device(c10::DeviceType::CPU);
     for (Py_ssize_t i = 0; i < all; ++i) {
         PyObject *po = PyList_GET_ITEM(params, i), *so = PyList_GET_ITEM(states, i);
@@ -345,7 +382,7 @@ PyObject *py_adamw_step(PyObject *, PyObject *const *args, Py_ssize_t count) {
             g.numel() != p.numel())
             Py_RETURN_FALSE;
         PyObject *items[5];
-        for (int k = 0; k < 5; ++k) items[k] = PyDict_GetItem(so, names[k]);
+        for (int k = 0; k < 3; ++k) items[k] = PyDict_GetItem(so, names[k]);
         if (!items[0] || !items[1] || !items[2] || !THPVariable_Check(items[1]) || !THPVariable_Check(items[2])) Py_RETURN_FALSE;
         const Tensor &m = THPVariable_Unpack(items[1]), &v = THPVariable_Unpack(items[2]);
         const bool coded = m.scalar_type() == at::kChar;
@@ -368,13 +405,18 @@ PyObject *py_adamw_step(PyObject *, PyObject *const *args, Py_ssize_t count) {
         };
         fits(m, coded ? at::kChar : at::kFloat, n);
         fits(v, coded ? at::kByte : at::kFloat, n);
+        gradients.push_back(g);
+        counts.push_back(step_count);
+        for (int k = 0; k < 3; ++k) held.add(items[k]);
         Tensor ms, vs;
         if (coded) {
+            for (int k = 3; k < 5; ++k) items[k] = PyDict_GetItem(so, names[k]);
             TORCH_CHECK(items[3] && items[4] && THPVariable_Check(items[3]) && THPVariable_Check(items[4]), "adamw_step: the state does not fit its parameter");
             ms = THPVariable_Unpack(items[3]);
             vs = THPVariable_Unpack(items[4]);
             fits(ms, at::kFloat, (n + ADDER_STATE_BLOCK - 1) / ADDER_STATE_BLOCK);
             fits(vs, at::kFloat, (n + ADDER_STATE_BLOCK - 1) / ADDER_STATE_BLOCK);
+            for (int k = 3; k < 5; ++k) held.add(items[k]);
         }
         Batch *batch = nullptr;
         for (Batch &b : batches)
@@ -382,6 +424,8 @@ PyObject *py_adamw_step(PyObject *, PyObject *const *args, Py_ssize_t count) {
         if (!batch) {
             batches.push_back(Batch{step_count, step, type, coded, {}, {}, {}, {}, {}, {}, {}});
             batch = &batches.back();
+            for (auto *to : {&batch->p, &batch->g, &batch->m, &batch->v}) to->reserve(all - i);
+            batch->n.reserve(all - i);
         }
         const int64_t size = type == at::kFloat ? 4 : 2, state = coded ? 1 : 4;
         for (int64_t at = 0; at < n; at += piece) {   // (empty tensors have no entry)
@@ -398,41 +442,44 @@ PyObject *py_adamw_step(PyObject *, PyObject *const *args, Py_ssize_t count) {
         }
     }
     if (all == 0) Py_RETURN_TRUE;
-    const c10::DeviceGuard guard(device);
-    void *stream = c10::hip::getCurrentHIPStream(device.index()).stream();
-    std::vector<std::pair<float *, Tensor>> advanced;
-    for (const Batch &b : batches) {
-        const float *corr = nullptr;
-        if (capturable) {
-            for (const auto &a : advanced)
-                if (a.first == b.step) corr = a.second.data_ptr<float>();
-            if (!corr) {
-                advanced.emplace_back(b.step, at::empty({2}, at::TensorOptions().dtype(at::kFloat).device(device)));
-                float *to = advanced.back().second.data_ptr<float>();
-                check(lib.advance(b.step, b1, b2, to, stream), "adder_adamw_advance");
-                corr = to;
+    {
+        const Released released;
+        const c10::DeviceGuard guard(device);
+        void *stream = c10::hip::getCurrentHIPStream(device.index()).stream();
+        std::vector<std::pair<float *, Tensor>> advanced;
+        for (const Batch &b : batches) {
+            const float *corr = nullptr;
+            if (capturable) {
+                for (const auto &a : advanced)
+                    if (a.first == b.step) corr = a.second.data_ptr<float>();
+                if (!corr) {
+                    advanced.emplace_back(b.step, at::empty({2}, at::TensorOptions().dtype(at::kFloat).device(device)));
+                    float *to = advanced.back().second.data_ptr<float>();
+                    check(lib.advance(b.step, b1, b2, to, stream), "adder_adamw_advance");
+                    corr = to;
+                }
             }
-        }
-        const int type = b.type == at::kFloat ? ADDER_TYPE_F32 : ADDER_TYPE_BF16;
-        const size_t most = b.coded ? ADDER_ADAMW_8BIT_BATCH_MAX : ADDER_ADAMW_BATCH_MAX;
-        for (size_t i = 0, next; i < b.n.size(); i = next) {   // as many as a table holds and a launch has workgroups for
-            int64_t used = 0;
-            for (next = i; next < b.n.size() && next - i < most; ++next) {
-                used += (b.n[next] + 1023) / 1024;
-                if (next > i && used > groups) break;
+            const int type = b.type == at::kFloat ? ADDER_TYPE_F32 : ADDER_TYPE_BF16;
+            const size_t most = b.coded ? ADDER_ADAMW_8BIT_BATCH_MAX : ADDER_ADAMW_BATCH_MAX;
+            for (size_t i = 0, next; i < b.n.size(); i = next) {   // as many as a table holds and a launch has workgroups for
+                int64_t used = 0;
+                for (next = i; next < b.n.size() && next - i < most; ++next) {
+                    used += (b.n[next] + 1023) / 1024;
+                    if (next > i && used > groups) break;
+                }
+                const int k = (int)(next - i);
+                const void *const *g = const_cast<const void *const *>(b.g.data() + i);
+                if (b.coded)
+                    check(lib.adamw8(k, b.p.data() + i, g, reinterpret_cast<signed char *const *>(b.m.data() + i),
+                                     reinterpret_cast<unsigned char *const *>(b.v.data() + i), reinterpret_cast<float *const *>(b.ms.data() + i),
+                                     reinterpret_cast<float *const *>(b.vs.data() + i), b.n.data() + i, lr_device, lr, b1, b2, eps, decay, b.count, corr, type,
+                                     stream),
+                          "adder_adamw_step_8bit");
+                else
+                    check(lib.adamw(k, b.p.data() + i, g, reinterpret_cast<float *const *>(b.m.data() + i), reinterpret_cast<float *const *>(b.v.data() + i),
+                                    b.n.data() + i, lr_device, lr, b1, b2, eps, decay, b.count, corr, type, stream),
+                          "adder_adamw_step");
             }
-            const int k = (int)(next - i);
-            const void *const *g = const_cast<const void *const *>(b.g.data() + i);
-            if (b.coded)
-                check(lib.adamw8(k, b.p.data() + i, g, reinterpret_cast<signed char *const *>(b.m.data() + i),
-                                 reinterpret_cast<unsigned char *const *>(b.v.data() + i), reinterpret_cast<float *const *>(b.ms.data() + i),
-                                 reinterpret_cast<float *const *>(b.vs.data() + i), b.n.data() + i, lr_device, lr, b1, b2, eps, decay, b.count, corr, type,
-                                 stream),
-                      "adder_adamw_step_8bit");
-            else
-                check(lib.adamw(k, b.p.data() + i, g, reinterpret_cast<float *const *>(b.m.data() + i), reinterpret_cast<float *const *>(b.v.data() + i),
-                                b.n.data() + i, lr_device, lr, b1, b2, eps, decay, b.count, corr, type, stream),
-                      "adder_adamw_step");
         }
     }
     PyObject *next = nullptr;
@@ -441,7 +488,7 @@ PyObject *py_adamw_step(PyObject *, PyObject *const *args, Py_ssize_t count) {
         THPVariable_Unpack(PyList_GET_ITEM(params, i)).unsafeGetTensorImpl()->bump_version();   // (changed in place)
         if (capturable) continue;
         PyObject *so = PyList_GET_ITEM(states, i);
-        const long now = PyLong_AsLong(PyDict_GetItem(so, names[0])) + 1;
+        const long now = counts[i];
         if (now != of) {
             Py_XDECREF(next);
             next = PyLong_FromLong(of = now);
