@@ -80,6 +80,7 @@ _SIGNATURES = {
     "adder_linear_fwd": (_i, [_p, _l, _p, _p, _p, _l, _p, _p, _i, _l, _i, _i, _i, _p, _sz, _p]),
     "adder_linear_bwd_workspace_bytes": (_i, [_l, _i, _i, _i, _i, _szp]),
     "adder_linear_bwd": (_i, [_p, _l, _p, _p, _l, _p, _p, _p, _p, _i, _l, _i, _i, _i, _p, _sz, _p]),
+    "adder_linear_kernel": (_i, [_l] + [_i] * 6 + [ctypes.POINTER(ctypes.c_int)]),
     "adder_layer_norm_fwd": (_i, [_p, _l, _p, _p, _p, _p, _p, _f, _l, _i, _i, _i, _p]),
     "adder_layer_norm_bwd_workspace_bytes": (_i, [_l, _i, _i, _szp]),
     "adder_layer_norm_bwd": (_i, [_p, _l, _p, _l, _p, _p, _p, _p, _p, _p, _l, _i, _i, _i, _p, _sz, _p]),

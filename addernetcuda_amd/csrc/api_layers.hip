@@ -163,6 +163,16 @@ int adder_linear_bwd(const void *dy, long dy_row_stride, const void *pre, const 
     return ADDER_OK;
 }
 
+int adder_linear_kernel(long rows, int in_features, int out_features, int product, int type, int aligned, int outputs, int *kernel) {
+    if (!kernel) return ADDER_ERR_NULL_POINTER;
+    if (int rc = check_linear(rows, in_features, out_features, type)) return rc;
+    if (product < 0 || product > 2 || outputs < 1 || outputs > (product ? 1 : 2)) return ADDER_ERR_BAD_SHAPE;
+    const long M = product == 2 ? out_features : rows, N = product ? in_features : out_features, K = product == 0 ? in_features : product == 1 ? out_features : rows;
+    const auto of = type == ADDER_TYPE_BF16 ? product_kernel<bf16_t> : product_kernel<float>;
+    *kernel = of(M, N, K, product == 2, product != 0, aligned != 0, outputs);
+    return ADDER_OK;
+}
+
 int adder_layer_norm_fwd(const void *x, long x_row_stride, const void *weight, const void *bias, void *y, float *save_mean, float *save_rstd,
                          float eps, long rows, int width, int type, int weight_type, void *stream) {
     if (!x || !y || (save_mean == nullptr) != (save_rstd == nullptr)) return ADDER_ERR_NULL_POINTER;

@@ -179,6 +179,8 @@ template <class T>
 size_t product_workspace_bytes(long M, long N, long K);
 template <class T>
 int launch_product(const Product &p, void *ws, hipStream_t s);
+template <class T>
+int product_kernel(long M, long N, long K, bool a_across, bool b_across, bool aligned, int outputs);   // as adder_linear_kernel numbers them
 // dz = dy * act'(z) (dense; not written where act is none) and part[i, n]: shares of its column sums (nullable)
 template <class T>
 int launch_act_bwd(const T *dy, long dy_stride, const T *z, T *dz, float *part, Act act, long rows, long N, hipStream_t s);

@@ -112,9 +112,8 @@ static ProductPlan plan_stream(long M, long N, long K, int outputs) { return pla
 // Loads of 16 aligned bytes fit a bfloat16 operand: base and rows begin at multiples of them, and what a tile's last load brings
 // beside the operand it can be told from by k alone (k along: rows of whole loads) or is never stored (k across).  A tile's rows
 // lie within 2^32 bytes of each other.
-static bool fits_stream(const void *p, long ld, bool across, long K) {
-    return !(reinterpret_cast<uintptr_t>(p) & 15) && !(ld & 7) && (across || !(K & 7)) && ld < (1L << 22);
-}
+static bool aligned16(const void *p, long ld) { return !(reinterpret_cast<uintptr_t>(p) & 15) && !(ld & 7) && ld < (1L << 22); }
+static bool fits_stream(bool across, long K) { return across || !(K & 7); }
 
 static size_t split_bytes(const ProductPlan &p, long M, long N) { return p.splits > 1 ? sizeof(float) * (size_t)p.splits * M * N : 0; }
 
@@ -129,17 +128,31 @@ size_t product_workspace_bytes(long M, long N, long K) {
     return most;
 }
 
+// The one choice that a launch and adder_linear_kernel make
+enum class Family { rows = 1, stream, staged };
+struct Choice { Family family; ProductPlan plan; };
+template <class T>
+static Choice choose_product(long M, long N, long K, bool a_across, bool b_across, bool aligned, int outputs) {
+    const bool stream = sizeof(T) == 2 && aligned && fits_stream(a_across, K) && fits_stream(b_across, K);
+    const ProductPlan plan = stream ? plan_stream(M, N, K, outputs) : plan_staged<T>(M, N, K, outputs);
+    if (!a_across && !b_across && M <= kRowsMost && N <= kRowsColumns && rows_us<T>(M, N, K) < plan.us) return {Family::rows, ProductPlan{0, 1, K, 0.f}};
+    return {stream ? Family::stream : Family::staged, plan};
+}
+template <class T>
+int product_kernel(long M, long N, long K, bool a_across, bool b_across, bool aligned, int outputs) {
+    const Choice c = choose_product<T>(M, N, K, a_across, b_across, aligned, outputs);
+    return static_cast<int>(c.family) * 10000 + (c.family == Family::rows ? product_rows_tiles(M) : c.plan.shape) * 100 + c.plan.splits;
+}
+
 template <class T>
 int launch_product(const Product &q, void *ws, hipStream_t s) {
-    const bool stream = sizeof(T) == 2 && fits_stream(q.a, q.lda, q.a_across, q.K) && fits_stream(q.b, q.ldb, q.b_across, q.K);
-    const int outputs = q.pre ? 2 : 1;
-    ProductPlan plan = stream ? plan_stream(q.M, q.N, q.K, outputs) : plan_staged<T>(q.M, q.N, q.K, outputs);
-    const bool rows = !q.a_across && !q.b_across && q.M <= kRowsMost && q.N <= kRowsColumns && rows_us<T>(q.M, q.N, q.K) < plan.us;
-    if (rows) plan = ProductPlan{0, 1, q.K, 0.f};
+    const bool aligned = aligned16(q.a, q.lda) && aligned16(q.b, q.ldb);
+    const Choice c = choose_product<T>(q.M, q.N, q.K, q.a_across, q.b_across, aligned, q.pre ? 2 : 1);
+    const ProductPlan &plan = c.plan;
     const ProductArgs p{q.a, q.b, q.bias, q.res, q.out, q.pre, static_cast<float *>(ws), q.lda, q.ldb, q.ldr, q.M, q.N, q.K, plan.k_share, 0, 0,
                         plan.splits, q.act};
-    const int rc = rows ? launch_product_rows<T>(p, s)
-                 : stream ? launch_product_stream(p, q.a_across, q.b_across, static_cast<StreamShape>(plan.shape), s)
+    const int rc = c.family == Family::rows ? launch_product_rows<T>(p, s)
+                 : c.family == Family::stream ? launch_product_stream(p, q.a_across, q.b_across, static_cast<StreamShape>(plan.shape), s)
                  : launch_product_staged<T>(p, q.a_across, q.b_across, static_cast<StagedShape>(plan.shape), s);
     if (rc || plan.splits == 1) return rc;
     hipLaunchKernelGGL(product_join_kernel<T>, dim3((unsigned)ceil_div_l(q.M * ((q.N + 3) / 4), 256)), dim3(256), 0, s, p);
@@ -214,6 +227,7 @@ int launch_act_bwd(const T *dy, long dy_stride, const T *z, T *dz, float *part, 
 #define ADDER_LINEAR_INSTANCE(T)                                                                                      \
     template size_t product_workspace_bytes<T>(long, long, long);                                                     \
     template int launch_product<T>(const Product &, void *, hipStream_t);                                            \
+    template int product_kernel<T>(long, long, long, bool, bool, bool, int);                                          \
     template int launch_act_bwd<T>(const T *, long, const T *, T *, float *, Act, long, long, hipStream_t);
 ADDER_LINEAR_INSTANCE(float)
 ADDER_LINEAR_INSTANCE(bf16_t)

@@ -113,8 +113,11 @@ static int launch_rows(const ProductArgs &p, hipStream_t s) {
 }
 template <class T>
 int launch_product_rows(const ProductArgs &p, hipStream_t s) {
-    if (p.M <= 16) return launch_rows<T, 1>(p, s);
-    return p.M <= 32 ? launch_rows<T, 2>(p, s) : launch_rows<T, 4>(p, s);
+    switch (product_rows_tiles(p.M)) {
+        case 1: return launch_rows<T, 1>(p, s);
+        case 2: return launch_rows<T, 2>(p, s);
+        default: return launch_rows<T, 4>(p, s);
+    }
 }
 template int launch_product_rows<float>(const ProductArgs &, hipStream_t);
 template int launch_product_rows<bf16_t>(const ProductArgs &, hipStream_t);

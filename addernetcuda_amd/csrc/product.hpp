@@ -304,5 +304,6 @@ template <class T>
 int launch_product_staged(const ProductArgs &p, bool a_across, bool b_across, StagedShape shape, hipStream_t s);
 template <class T>
 int launch_product_rows(const ProductArgs &p, hipStream_t s);   // both along; few rows
+inline int product_rows_tiles(long M) { return M <= 16 ? 1 : M <= 32 ? 2 : 4; }   // of sixteen rows that a workgroup takes
 
 }  // namespace adder

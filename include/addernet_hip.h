@@ -514,6 +514,12 @@ ADDER_API int adder_linear_bwd(const void *dy, long dy_row_stride, const void *p
                                const void *w, void *gx, void *gw, void *gbias, int act, long rows, int in_features,
                                int out_features, int type, void *ws, size_t ws_bytes, void *stream);
 
+/* Which kernel a product of the entry points above takes: product 0 the forward's, 1 the input gradient's, 2 the weight gradient's.  10000 x (1 for few rows,
+ * 2 streamed, 3 staged) + 100 x its shape (few rows: tiles of sixteen rows; else the number in the plan's table) + the shares of k.  aligned: bases and
+ * row strides of both operands are multiples of 16 bytes; outputs: 2 where the forward writes pre as well, else 1.  Host code only, for tests that have to
+ * reach a certain kernel, and no promise that the numbers stay. */
+ADDER_API int adder_linear_kernel(long rows, int in_features, int out_features, int product, int type, int aligned, int outputs, int *kernel);
+
 /* Layer normalisation of rows of `width` values: y = (x - mean) rstd weight + bias, rstd = 1 / sqrt(variance + eps) with the
  * biased variance; weight and bias (width) nullable and stored as weight_type says (type, or float32 beside bfloat16 rows).
  *   adder_layer_norm_fwd: save_mean, save_rstd (rows): both or neither; the backward needs them.
