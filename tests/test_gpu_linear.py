@@ -355,3 +355,36 @@ def test_relu_lets_nothing_through_where_it_is_off(rows, k, n, residual, dtype, 
     broken = torch.where(off, kinds[torch.arange(rows * n, device="cuda").view(rows, n) % 4], dy)
     for g, h in zip(torch.autograd.grad(y, leaves, broken, retain_graph=True), torch.autograd.grad(y, leaves, torch.where(off, torch.zeros_like(dy), dy))):
         assert torch.isfinite(g).all() and torch.equal(g, h)
+
+
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("n", [512, 515])
+def test_values_before_the_activation_keep_eleven_bits(act, n, gpu):
+    """bfloat16: the bias's gradient of two rows with opposite gradients and nearly the same z is a difference that rounding to its type hardly
+    touches.  z as a half, rounded toward zero, is 2^-10 |z| + 2^-24 off, which moves the derivative by its own derivative times that (a
+    tenth more for the next term); z as a bfloat16 would not stay within that.  And what the forward hands on is that half."""
+    from addernetcuda_amd._lib import lib, check, ptr, stream_ptr
+    from addernetcuda_amd.linear import ACTS, linear_act
+    g = torch.Generator().manual_seed(n)
+    x = torch.randn(1, 64, generator=g).bfloat16().repeat(2, 1)
+    x[1, :4] += 0.03
+    w, b = (torch.randn(n, 64, generator=g) / 16).bfloat16(), (torch.randn(n, generator=g)).bfloat16()
+    dy = torch.tensor([[1.0], [-1.0]]).expand(2, n).bfloat16()
+    z = (x.double() @ w.double().t() + b.double()).requires_grad_(True)
+    _, slope = B.activation(z, act)
+    bend, = torch.autograd.grad(slope.sum(), z)
+    z, slope = z.detach(), slope.detach()
+    off_z = B.terms(64) * (x.double().abs() @ w.double().abs().t() + b.double().abs())
+    moved = 1.1 * bend.abs() * (2.0 ** -10 * z.abs() + 2.0 ** -24 + off_z) + 24 * B.U * (1 + z.abs())
+    value = slope[0] - slope[1]
+    expected = value, moved.sum(0) + 4 * B.U + B.V * value.abs()
+    leaf = b.cuda().requires_grad_(True)
+    gb, = torch.autograd.grad(linear_act(x.cuda(), w.cuda(), leaf, act=act), leaf, dy.cuda())
+    B.within(gb, expected, "gb")
+    short = B.activation(z.bfloat16().double(), act)[1]
+    with pytest.raises(AssertionError, match="further off"):
+        B.within((short[0] - short[1]).float(), expected, "gb from z in bfloat16")
+    xs, ws, bs = x.cuda(), w.cuda(), b.cuda()
+    y, pre = torch.empty(2, n, dtype=torch.bfloat16, device="cuda"), torch.empty(2, n, dtype=torch.float16, device="cuda")
+    check(lib.adder_linear_fwd(ptr(xs), 64, ptr(ws), ptr(bs), None, 0, ptr(y), ptr(pre), ACTS[act], 2, 64, n, 1, None, 0, stream_ptr(xs.device)), "adder_linear_fwd")
+    assert ((pre.double().cpu() - z).abs() <= 2.0 ** -10 * z.abs() + 2.0 ** -24 + off_z).all()
