@@ -59,3 +59,28 @@ def test_adamw_step(slow_library):
     slow_library("adder_adamw_step")   # (96 entries, 96 microseconds)
     done, ran = others_run_during(lambda: _lib.nodes().adamw_step([p], [state], False, 0.1, 0, 0.9, 0.99, 1e-8, 0.0, 256, 1 << 20))
     assert done and ran and state["step"] == 1 and p.detach().eq(1).all()
+
+
+@pytest.mark.parametrize("layer", ["linear", "norm"])
+def test_python_hooks_run_inside_the_nodes(layer, gpu):
+    """Hooks on what is saved for the backward are Python, called from inside the module; so is what anomaly mode records."""
+    from addernetcuda_amd.layer_norm import layer_norm
+    from addernetcuda_amd.linear import linear_act
+    x, w, b = torch.randn(40, 24, device="cuda"), torch.randn(24, 24, device="cuda"), torch.randn(24, device="cuda")
+    leaves = [t.requires_grad_(True) for t in (x, w if layer == "linear" else b)]
+    run = (lambda: linear_act(x, w, b, act="gelu")) if layer == "linear" else lambda: layer_norm(x, b)
+    want = torch.autograd.grad(run().square().sum(), leaves)
+    packed = []
+
+    def pack(t):
+        packed.append(t.shape)
+        return t.cpu()
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t.cuda()):
+        y = run()
+    assert len(packed) >= 3
+    for g, h in zip(torch.autograd.grad(y.square().sum(), leaves), want):
+        assert torch.equal(g, h)
+    with torch.autograd.detect_anomaly(check_nan=True):
+        with pytest.raises(RuntimeError, match="nan values"):
+            torch.autograd.grad(run(), leaves, torch.full((40, 24), float("nan"), device="cuda"))
