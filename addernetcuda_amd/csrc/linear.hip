@@ -45,22 +45,22 @@ static constexpr int kCUs = 256;
 struct Shape { int bm, bn, per_cu; float step, alone, tile; };
 //                                       8192^3, TFLOP/s
 static constexpr Shape kStreamShapes[] = {
-    {256, 256, 1, 1.55f, 1.55f, 10.f},   // 1320
-    {128, 256, 1, 0.9f, 0.9f, 4.f},      // 1155
-    {128, 128, 2, 0.87f, 0.65f, 3.5f},   // 1155
-    {64, 64, 2, 0.38f, 0.2f, 1.5f},      //  640
+    {256, 256, 1, 1.55f, 1.55f, 10.f},   // 1305
+    {128, 256, 1, 0.9f, 0.9f, 4.f},      // 1146 (taken for shares of long sums: 616 x 28360 -> 16568 in 821 us, 1028 without it)
+    {128, 128, 2, 0.87f, 0.65f, 3.5f},   // 1177
+    {64, 64, 2, 0.38f, 0.2f, 1.5f},      //  719
 };
 template <class T>
 static constexpr Shape kStagedShapes[] = {
-    {128, 128, 2, 1.f, 0.6f, 3.5f},      //  960
-    {64, 64, 4, 0.78f, 0.25f, 1.5f},     //  640
+    {128, 128, 2, 1.f, 0.6f, 3.5f},      // 1033
+    {64, 64, 4, 0.78f, 0.25f, 1.5f},     //  701
 };
 template <>
 constexpr Shape kStagedShapes<float>[] = {
     {128, 128, 2, 2.3f, 1.9f, 3.5f},     //  220
-    {64, 64, 3, 1.25f, 0.65f, 1.5f},     //  155
-    {128, 128, 1, 1.15f, 1.15f, 3.5f},   //  200 (step: that of one or two rounds, 2048^3)
-    {64, 64, 1, 0.53f, 0.53f, 2.5f},     //  145
+    {64, 64, 3, 1.25f, 0.65f, 1.5f},     //  161
+    {128, 128, 1, 1.15f, 1.15f, 3.5f},   //  204 (step: that of one or two rounds, 2048^3)
+    {64, 64, 1, 0.53f, 0.53f, 2.5f},     //  147
 };
 static constexpr int kSplitMax = 16;
 
@@ -162,7 +162,8 @@ int launch_product(const Product &q, void *ws, hipStream_t s) {
 // ---- the activation's derivative and the bias's gradient ---------------------------------------------------------------
 // Memory decides: dy and z are read and dz is written, 41 us for 8192 x 4096 in bfloat16 with a GELU (4.9 TB/s).  A workgroup takes 64 lanes'
 // chunks of columns and a share of the rows; its four waves walk over the rows, and their column sums are added through LDS into
-// one slab a share.  A row at a time and up to four workgroups a compute unit: two or four rows under way in a wave are no faster where there
+// one slab a share.  bfloat16: dz is rounded to the type of the products' operands, and the bias's sums are not; gradients are then 0.0023 from float64
+// where a float32 dz, as two bfloat16 parts, would give 0.0017 for twice the products' work.  A row at a time and up to four workgroups a compute unit: two or four rows under way in a wave are no faster where there
 // are many (53 us with what follows, all three) and leave waves out where there are few (128 x 512: 9.9 and 10.8 us instead of 9.5);
 // 2048 workgroups leave more slabs to fold (16384 x 512: 23.4 us instead of 21.1).
 template <class T, Act ACT>

@@ -14,7 +14,7 @@ namespace adder {
 // product.  An operand that is infinite, not a number, or rounds up to infinity gives a sum that is not finite; a wave that finds some
 // computes those again, in float32.
 //
-// 8192 x 1024 x 4096: 330 us, 208 TFLOP/s (float32 matrix instructions: 155 at their best); 1024^3 18.6 us, 115 TFLOP/s; 1531 x 515 x 1027 21 us.
+// 8192 x 1024 x 4096: 312 us, 220 TFLOP/s (float32 matrix instructions: 155 at their best); 1024^3 20 us, 105 TFLOP/s; 1531 x 515 x 1027 22 us.
 // Where the tiles fill the card, LDS bounds it: 32 values of k of a 64 x 64 tile are 24 KB written and 48 KB read, 576 cycles, beside
 // 384 of the matrix cores and 350 of the splitting; where they do not, each of those waits for the other.
 template <class T>
