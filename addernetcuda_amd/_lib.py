@@ -24,7 +24,7 @@ ADDER_ERR_WORKSPACE, ADDER_ERR_HIP, ADDER_ERR_ALIAS, ADDER_ERR_UNSUPPORTED = -4,
 MAX_ELEMENTS = 0x7fffffff   # of one tensor; entry points answer ADDER_ERR_TOO_LARGE above it
 
 _i, _l, _f, _p, _sz = ctypes.c_int, ctypes.c_long, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t
-_szp, _d = ctypes.POINTER(ctypes.c_size_t), ctypes.c_double
+_szp, _d, _ll = ctypes.POINTER(ctypes.c_size_t), ctypes.c_double, ctypes.c_longlong
 
 _SIGNATURES = {
     "adder_strerror": (ctypes.c_char_p, [_i]),
@@ -87,6 +87,24 @@ _SIGNATURES = {
     "adder_adamw_step": (_i, [_i] + [_p] * 6 + [_d] * 5 + [_l, _p, _i, _p]),
     "adder_adamw_step_8bit": (_i, [_i] + [_p] * 8 + [_d] * 5 + [_l, _p, _i, _p]),
     "adder_adamw_advance": (_i, [_p, _d, _d, _p, _p]),
+    "adder_rms_norm_fwd": (_i, [_p, _l, _p, _l, _p, _p, _p, _p, _f, _l, _i, _i, _i, _p]),
+    "adder_rms_norm_fwd_codes": (_i, [_p, _l, _p, _l, _p, _p, _p, _p, _f, _l, _i, _i, _i, _p]),
+    "adder_rms_norm_bwd_workspace_bytes": (_i, [_l, _i, _i, _szp]),
+    "adder_rms_norm_bwd": (_i, [_p, _l, _p, _l, _p, _l, _p, _p, _p, _p, _l, _i, _i, _i, _p, _sz, _p]),
+    "adder_quantize": (_i, [_p, _l, _i, _p, _p, _l, _i, _i, _p]),
+    "adder_quantize_weight": (_i, [_p, _l, _p, _p, _l, _i, _i, _p]),
+    "adder_linear_codes_workspace_bytes": (_i, [_l, _i, _i, _i, _i, _szp]),
+    "adder_linear_codes": (_i, [_p, _l, _p, _p, _l, _p, _p, _p, _l, _p, _i, _l, _i, _i, _i, _p, _sz, _p]),
+    "adder_linear_codes_kernel": (_i, [_l, _i, _i, ctypes.POINTER(ctypes.c_int)]),
+    "adder_gated_fwd_workspace_bytes": (_i, [_l, _i, _i, _i, _szp]),
+    "adder_gated_fwd": (_i, [_p, _l, _p, _p, _p, _p, _i, _l, _i, _i, _i, _p, _sz, _p]),
+    "adder_gated_bwd_workspace_bytes": (_i, [_l, _i, _i, _i, _szp]),
+    "adder_gated_bwd": (_i, [_p, _l, _p, _p, _l, _p, _p, _p, _p, _i, _l, _i, _i, _i, _p, _sz, _p]),
+    "adder_gated_kernel": (_i, [_l] + [_i] * 5 + [ctypes.POINTER(ctypes.c_int)]),
+    "adder_distill_in_rows": (_i, [_l, _i, _i]),
+    "adder_distill_workspace_bytes": (_i, [_l, _i, _i, _szp]),
+    "adder_distill_fwd": (_i, [_p, _l, _p, _p, _p, _p, _p, _p, _f, _f, _ll, _l, _i, _i, _i, _i, _p, _sz, _p]),
+    "adder_distill_bwd": (_i, [_p, _l, _p, _p, _p, _p, _p, _i, _p, _f, _f, _ll, _l, _i, _i, _i, _i, _p]),
     "adder_state_values": (_i, [_p, _i, _p, _p, _l, _i, _p]),
 }
 for _name, (_res, _args) in _SIGNATURES.items():

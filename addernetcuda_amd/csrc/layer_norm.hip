@@ -10,26 +10,9 @@
 
 namespace adder {
 
-static constexpr int kNormValues = 16;    // per lane
 template <class T>
 static constexpr int kNormChunks = kNormValues / Chunk<T>::n;
 static constexpr int kNormFwdThreads = 256, kNormBwdThreads = 512;
-
-// Sum over the G lanes that share a row, in every one of them.  G > 64: through LDS, and every wave of the workgroup has to come.
-template <int G>
-__device__ __forceinline__ float row_sum(float v, float *lds) {
-    v = lanes_sum<(G < 64 ? G : 64)>(v);
-    if constexpr (G > 64) {
-        const int wave = threadIdx.x >> 6, first = wave / (G / 64) * (G / 64);
-        __syncthreads();   // (the last sum has been read)
-        if ((threadIdx.x & 63) == 0) lds[wave] = v;
-        __syncthreads();
-        v = lds[first];
-#pragma unroll
-        for (int i = 1; i < G / 64; ++i) v += lds[first + i];
-    }
-    return v;
-}
 
 // 1 / sqrt(var + eps) of a row from the sum of the squares of its values' differences from the (rounded) mean and the mean of those differences: `rest`
 // is the mean's rounding, without which a row whose values are large beside their spread loses its digits.  Where the squares leave the range of a
@@ -299,13 +282,6 @@ int launch_fold_columns(const float *part, int parts, int K, long cols, const Fo
 template int launch_fold_columns<float>(const float *, int, int, long, const FoldOut &, hipStream_t);
 template int launch_fold_columns<bf16_t>(const float *, int, int, long, const FoldOut &, hipStream_t);
 
-// Lanes per row: as few as hold it with 16 values each, so that the lanes are full and few steps join them
-static int norm_lanes(int D) {
-    int g = 8;
-    while (g * kNormValues < D) g *= 2;
-    return g;
-}
-
 // At most three workgroups a compute unit, which walk over the rows with the weight in registers: 512 workgroups take 15.5 us for 16384 x 1024 in
 // bfloat16 instead of 13.6, 2048 take 17.9 us for 2048 x 8192 instead of 15.6 and 8.0 for 32768 x 256 instead of 6.9
 static int norm_fwd_blocks(long rows, int G) {
@@ -321,18 +297,6 @@ int layer_norm_bwd_parts(long rows, int D) {
     const long per = G > kNormBwdThreads ? 1 : kNormBwdThreads / G, need = ceil_div_l(rows, per), most = 256;
     return (int)(need < most ? need : most);
 }
-
-#define ADDER_NORM_LANES(G, CALL)            \
-    switch (G) {                             \
-        case 8: CALL(8); break;              \
-        case 16: CALL(16); break;            \
-        case 32: CALL(32); break;            \
-        case 64: CALL(64); break;            \
-        case 128: CALL(128); break;          \
-        case 256: CALL(256); break;          \
-        case 512: CALL(512); break;          \
-        default: CALL(1024); break;          \
-    }
 
 template <class T, class W>
 int launch_layer_norm_fwd(const T *x, long x_stride, const W *w, const W *b, T *y, float *mean, float *rstd, float eps, long rows,

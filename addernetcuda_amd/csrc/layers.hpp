@@ -126,6 +126,42 @@ __device__ __forceinline__ float lanes_sum(float v) {
     return v;
 }
 
+// Sum over the G lanes that share a row, in every one of them.  G > 64: through LDS, and every wave of the workgroup has to come.
+template <int G>
+__device__ __forceinline__ float row_sum(float v, float *lds) {
+    v = lanes_sum<(G < 64 ? G : 64)>(v);
+    if constexpr (G > 64) {
+        const int wave = threadIdx.x >> 6, first = wave / (G / 64) * (G / 64);
+        __syncthreads();   // (the last sum has been read)
+        if ((threadIdx.x & 63) == 0) lds[wave] = v;
+        __syncthreads();
+        v = lds[first];
+#pragma unroll
+        for (int i = 1; i < G / 64; ++i) v += lds[first + i];
+    }
+    return v;
+}
+
+// Rows that stay in registers: lanes a row, as few as hold it with 16 values each, so that the lanes are full and few steps join them
+static constexpr int kNormValues = 16;
+inline int norm_lanes(int D) {
+    int g = 8;
+    while (g * kNormValues < D) g *= 2;
+    return g;
+}
+
+#define ADDER_NORM_LANES(G, CALL)            \
+    switch (G) {                             \
+        case 8: CALL(8); break;              \
+        case 16: CALL(16); break;            \
+        case 32: CALL(32); break;            \
+        case 64: CALL(64); break;            \
+        case 128: CALL(128); break;          \
+        case 256: CALL(256); break;          \
+        case 512: CALL(512); break;          \
+        default: CALL(1024); break;          \
+    }
+
 // out_k[c] = sum over i of part[(i * K + k) * cols + c] for k < K: column sums that workgroups left in `parts` slabs, in a
 // fixed order.  out[k] may be null.
 static constexpr int kFoldMax = 2;
@@ -174,7 +210,10 @@ struct Product {
     long ldr;
     void *out, *pre;
     Act act;
+    long half = 0;   // gated (out[m, n] = act(g) u, both with their bias): the columns of out, H; b has 2 H rows, N = gated_columns(H)
 };
+// Columns of a gated layer's product: both halves, in whole groups of sixteen
+inline long gated_columns(long H) { return (H + 15) / 16 * 32; }
 template <class T>
 size_t product_workspace_bytes(long M, long N, long K);
 template <class T>

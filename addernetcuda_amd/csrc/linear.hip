@@ -8,41 +8,57 @@ namespace adder {
 
 // The shares of the sums added up in their order, and the epilogue: four results a thread.  Memory decides, or the launch: two shares of
 // 4096 x 1024 12 us (42 MB), four of 128 x 512 3 us.
-template <class T>
+template <class T, bool GATED>
 __global__ __launch_bounds__(256) void product_join_kernel(const ProductArgs p) {
-    const long groups = (p.N + 3) / 4, i = (long)blockIdx.x * 256 + threadIdx.x;
+    const long columns = GATED ? p.half : p.N, groups = (columns + 3) / 4, i = (long)blockIdx.x * 256 + threadIdx.x;
     if (i >= p.M * groups) return;
     const long m = i / groups, n = i % groups * 4;
-    const int cnt = p.N - n < 4 ? (int)(p.N - n) : 4;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    const float *q = p.part + m * p.N + n;
+    const int cnt = columns - n < 4 ? (int)(columns - n) : 4;
     const long share = p.M * p.N;
-    int s = 0;
-    if (cnt == 4) {
-        for (; s + 4 <= p.splits; s += 4) {   // (four loads under way)
-            float t[4][4];
+    const auto sum = [&](long column, float (&v)[4]) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u) ld_strip<4>(q + (s + u) * share, t[u]);
+        for (int e = 0; e < 4; ++e) v[e] = 0.f;
+        const float *q = p.part + m * p.N + column;
+        int s = 0;
+        if (GATED || cnt == 4) {   // (gated: whole groups of sixteen)
+            for (; s + 4 <= p.splits; s += 4) {   // (four loads under way)
+                float t[4][4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
+                for (int u = 0; u < 4; ++u) ld_strip<4>(q + (s + u) * share, t[u]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] += t[u][e];
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] += t[u][e];
+            }
         }
-    }
-    for (; s < p.splits; ++s) {
+        for (; s < p.splits; ++s) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] += e < cnt ? q[s * share + e] : 0.f;
+            for (int e = 0; e < 4; ++e) v[e] += e < cnt ? q[s * share + e] : 0.f;
+        }
+    };
+    float v[4];
+    if constexpr (GATED) {
+        float u[4];
+        const long column = (n >> 4) * 32 + (n & 15);
+        sum(column, v);
+        sum(column + 16, u);
+        finish_gated<T>(p, m, n, cnt, v, u);
+    } else {
+        sum(n, v);
+        finish<T>(p, m, n, cnt, v);
     }
-    finish<T>(p, m, n, cnt, v);
+}
+
+template <class T>
+int launch_product_join(const ProductArgs &p, hipStream_t s) {
+    const dim3 grid((unsigned)ceil_div_l(p.M * (((p.half ? p.half : p.N) + 3) / 4), 256));
+    if (p.half) hipLaunchKernelGGL((product_join_kernel<T, true>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((product_join_kernel<T, false>), grid, dim3(256), 0, s, p);
+    return check_launch();
 }
 
 // ---- which kernel ---------------------------------------------------------------------------------------------------
-// A launch's time is estimated for every shape of tile and number of shares of k, and the least is taken.  The workgroups run in rounds
-// of as many as the card holds, each steps * step + tile us: steps of 64 (float32: 32) values of k; `step` measured with every compute
-// unit full (8192 x 8192 x 1024 and 8192^3), less in proportion where fewer workgroups share one, but at least `alone` (1024^3); `tile` the first
-// loads, the epilogue and the start, once more where a second output is written.  Shares of k pay for their sums' way through memory (5 TB/s both ways) and the join's launch.
-static constexpr int kCUs = 256;
-struct Shape { int bm, bn, per_cu; float step, alone, tile; };
+// (the estimate: product.hpp)
 //                                       8192^3, TFLOP/s
 static constexpr Shape kStreamShapes[] = {
     {256, 256, 1, 1.55f, 1.55f, 10.f},   // 1305
@@ -62,10 +78,6 @@ constexpr Shape kStagedShapes<float>[] = {
     {128, 128, 1, 1.15f, 1.15f, 3.5f},   //  204 (step: that of one or two rounds, 2048^3)
     {64, 64, 1, 0.53f, 0.53f, 2.5f},     //  147
 };
-static constexpr int kSplitMax = 16;
-
-struct ProductPlan { int shape, splits; long k_share; float us; };
-
 // The kernel for few rows likewise: workgroups of 16 columns and 16, 32 or 64 rows, whose waves take turns along k, 128 bytes of every
 // row at a time (us each, with the rows' share of the second-level caches: 4096 x 4096, full workgroups)
 static constexpr long kRowsMost = 1024, kRowsColumns = 1L << 25;   // within which the estimate finds it the fastest, and its launch has few enough threads
@@ -78,33 +90,6 @@ static float rows_us(long M, long N, long K) {
     return 3.f + ceilf(groups / kCUs) * (1.3f + turns * kTurn[sizeof(T) == 4][mt]);
 }
 
-template <int N>
-static ProductPlan plan_product(const Shape (&shapes)[N], int bk, long M, long N_, long K, int outputs) {
-    static constexpr int kSplits[] = {1, 2, 3, 4, 6, 8, 12, kSplitMax};
-    ProductPlan best{0, 1, K, 0.f};
-    const long steps = ceil_div_l(K, bk);
-    for (int i = 0; i < N; ++i) {
-        const Shape &h = shapes[i];
-        const float tiles = (float)ceil_div_l(M, h.bm) * (float)ceil_div_l(N_, h.bn);
-        for (int splits : kSplits) {
-            if (splits > steps || (splits > 1 && tiles * splits > 4.f * kCUs)) break;
-            const long share = ceil_div_l(steps, splits);
-            const float groups = tiles * splits;
-            const float slots = (float)(kCUs * h.per_cu), whole = floorf(groups / slots), rest = groups - whole * slots;
-            float us = 3.f + whole * (share * h.step + h.tile * outputs);
-            if (rest > 0.f) {
-                const float shared = h.step * ceilf(rest / kCUs) / h.per_cu;
-                us += share * (shared > h.alone ? shared : h.alone) + h.tile * outputs;
-            }
-            if (splits > 1) us += 3.f + (float)M * (float)N_ * splits * 8.f / 5e6f;
-            if (best.us == 0.f || us < best.us) {
-                const int used = (int)ceil_div_l(steps, share);
-                best = ProductPlan{i, used, used > 1 ? share * bk : K, us};
-            }
-        }
-    }
-    return best;
-}
 template <class T>
 static ProductPlan plan_staged(long M, long N, long K, int outputs) { return plan_product(kStagedShapes<T>, sizeof(T) == 4 ? 32 : 64, M, N, K, outputs); }
 static ProductPlan plan_stream(long M, long N, long K, int outputs) { return plan_product(kStreamShapes, 64, M, N, K, outputs); }
@@ -146,17 +131,16 @@ int product_kernel(long M, long N, long K, bool a_across, bool b_across, bool al
 
 template <class T>
 int launch_product(const Product &q, void *ws, hipStream_t s) {
-    const bool aligned = aligned16(q.a, q.lda) && aligned16(q.b, q.ldb);
+    const bool aligned = aligned16(q.a, q.lda) && aligned16(q.b, q.ldb) && (!q.half || (q.half + 256) * q.ldb < (1L << 31));   // (gated: a tile's rows are half the weight apart)
     const Choice c = choose_product<T>(q.M, q.N, q.K, q.a_across, q.b_across, aligned, q.pre ? 2 : 1);
     const ProductPlan &plan = c.plan;
     const ProductArgs p{q.a, q.b, q.bias, q.res, q.out, q.pre, static_cast<float *>(ws), q.lda, q.ldb, q.ldr, q.M, q.N, q.K, plan.k_share, 0, 0,
-                        plan.splits, q.act};
+                        plan.splits, q.act, q.half};
     const int rc = c.family == Family::rows ? launch_product_rows<T>(p, s)
                  : c.family == Family::stream ? launch_product_stream(p, q.a_across, q.b_across, static_cast<StreamShape>(plan.shape), s)
                  : launch_product_staged<T>(p, q.a_across, q.b_across, static_cast<StagedShape>(plan.shape), s);
     if (rc || plan.splits == 1) return rc;
-    hipLaunchKernelGGL(product_join_kernel<T>, dim3((unsigned)ceil_div_l(q.M * ((q.N + 3) / 4), 256)), dim3(256), 0, s, p);
-    return check_launch();
+    return launch_product_join<T>(p, s);
 }
 
 // ---- the activation's derivative and the bias's gradient ---------------------------------------------------------------
@@ -228,6 +212,7 @@ int launch_act_bwd(const T *dy, long dy_stride, const T *z, T *dz, float *part, 
 #define ADDER_LINEAR_INSTANCE(T)                                                                                      \
     template size_t product_workspace_bytes<T>(long, long, long);                                                     \
     template int launch_product<T>(const Product &, void *, hipStream_t);                                            \
+    template int launch_product_join<T>(const ProductArgs &, hipStream_t);                                            \
     template int product_kernel<T>(long, long, long, bool, bool, bool, int);                                          \
     template int launch_act_bwd<T>(const T *, long, const T *, T *, float *, Act, long, long, hipStream_t);
 ADDER_LINEAR_INSTANCE(float)

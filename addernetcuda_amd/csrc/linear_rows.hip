@@ -23,33 +23,39 @@ __device__ __forceinline__ void multiply(f32x4 &acc, const uint4 &b, const uint4
     acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b), __builtin_bit_cast(bf16x8, a), acc, 0, 0, 0);
 }
 
-template <class T, int MT>
+template <class T, int MT, bool GATED>
 __global__ __launch_bounds__(kRowsWaves<MT> * 64) void product_rows_kernel(const ProductArgs p) {
-    constexpr int E = Chunk<T>::n, BK = 8 * E, U = MT == 1 ? 2 : 1;   // blocks that a wave multiplies while as many arrive
+    constexpr int E = Chunk<T>::n, BK = 8 * E, U = MT == 1 && !GATED ? 2 : 1;   // blocks that a wave multiplies while as many arrive
+    constexpr int NB = GATED ? 2 : 1;   // gated: sixteen rows of either half of w
     extern __shared__ __align__(16) char lds[];
     f32x4 *sums = reinterpret_cast<f32x4 *>(lds);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, l16 = lane & 15;
-    const long n0 = (long)blockIdx.x * 16, m0 = (long)blockIdx.y * (16 * MT);
+    const long n0 = (long)blockIdx.x * 16, columns = GATED ? p.half : p.N, m0 = (long)blockIdx.y * (16 * MT);
     const T *a = static_cast<const T *>(p.a), *b = static_cast<const T *>(p.b);
     const int mine = (lane >> 4) * E;   // of half a block's values of k
     // (rows past the last: that one again; their results are not stored)
-    const T *pb = b + (n0 + l16 < p.N ? n0 + l16 : p.N - 1) * p.ldb + mine, *pa[MT];
+    const T *pb[NB], *pa[MT];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) pb[j] = b + ((n0 + l16 < columns ? n0 + l16 : columns - 1) + j * columns) * p.ldb + mine;
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
         const long m = m0 + i * 16 + l16;
         pa[i] = a + (m < p.M ? m : p.M - 1) * p.lda + mine;
     }
-    f32x4 acc[MT];
+    f32x4 acc[NB][MT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    struct Blocks { uint4 b[U][2], a[U][MT][2]; };
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    struct Blocks { uint4 b[U][NB][2], a[U][MT][2]; };
     auto load = [&](Blocks &t, long kb) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const long k = (kb + u * waves) * BK + h * (4 * E);
-                t.b[u][h] = load_raw(pb + k);
+#pragma unroll
+                for (int j = 0; j < NB; ++j) t.b[u][j][h] = load_raw(pb[j] + k);
 #pragma unroll
                 for (int i = 0; i < MT; ++i) t.a[u][i][h] = load_raw(pa[i] + k);
             }
@@ -60,7 +66,9 @@ __global__ __launch_bounds__(kRowsWaves<MT> * 64) void product_rows_kernel(const
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int i = 0; i < MT; ++i) multiply(acc[i], t.b[u][h], t.a[u][i][h], T{});
+                for (int j = 0; j < NB; ++j)
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) multiply(acc[j][i], t.b[u][j][h], t.a[u][i][h], T{});
     };
     const long whole = p.K / BK, turn = U * waves, last = whole - (U - 1) * waves;   // (a turn begins below `last`)
     long kb = wave;
@@ -84,32 +92,52 @@ __global__ __launch_bounds__(kRowsWaves<MT> * 64) void product_rows_kernel(const
         for (int h = 0; h < 2; ++h) {
             const long rest = left - h * (4 * E);
             const int valid = rest < 0 ? 0 : rest < E ? (int)rest : E;
-            const uint4 fb = load_raw_part(pb + k + h * (4 * E), valid);
+            uint4 fb[NB];
 #pragma unroll
-            for (int i = 0; i < MT; ++i) multiply(acc[i], fb, load_raw_part(pa[i] + k + h * (4 * E), valid), T{});
+            for (int j = 0; j < NB; ++j) fb[j] = load_raw_part(pb[j] + k + h * (4 * E), valid);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const uint4 fa = load_raw_part(pa[i] + k + h * (4 * E), valid);
+#pragma unroll
+                for (int j = 0; j < NB; ++j) multiply(acc[j][i], fb[j], fa, T{});
+            }
         }
     }
 #pragma unroll
-    for (int i = 0; i < MT; ++i) sums[(wave * MT + i) * 64 + lane] = acc[i];
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) sums[((wave * NB + j) * MT + i) * 64 + lane] = acc[j][i];
     __syncthreads();
     for (int t = threadIdx.x; t < MT * 64; t += blockDim.x) {
-        f32x4 s = sums[t];
-        for (int w = 1; w < waves; ++w) s += sums[w * MT * 64 + t];
+        float v[NB][4];
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            f32x4 s = sums[j * MT * 64 + t];
+            for (int w = 1; w < waves; ++w) s += sums[(w * NB + j) * MT * 64 + t];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[j][e] = s[e];
+        }
         const long m = m0 + t / 64 * 16 + (t & 15), n = n0 + (t >> 4 & 3) * 4;
-        if (m < p.M && n < p.N) {
-            const float v[4] = {s[0], s[1], s[2], s[3]};
-            finish<T>(p, m, n, p.N - n < 4 ? (int)(p.N - n) : 4, v);
+        if (m < p.M && n < columns) {
+            const int cnt = columns - n < 4 ? (int)(columns - n) : 4;
+            if constexpr (GATED) finish_gated<T>(p, m, n, cnt, v[0], v[1]);
+            else finish<T>(p, m, n, cnt, v[0]);
         }
     }
 }
 
+template <class T, int MT, bool GATED>
+static int launch_rows_of(const ProductArgs &p, hipStream_t s) {
+    const long blocks = ceil_div_l(p.K, 8 * Chunk<T>::n);
+    const int waves = (int)(blocks < kRowsWaves<MT> ? blocks : kRowsWaves<MT>), bytes = waves * MT * (GATED ? 2048 : 1024);
+    if (int rc = allow_dynamic_lds<&product_rows_kernel<T, MT, GATED>>(bytes)) return rc;
+    hipLaunchKernelGGL((product_rows_kernel<T, MT, GATED>), dim3((unsigned)ceil_div_l(GATED ? p.half : p.N, 16), (unsigned)ceil_div_l(p.M, 16 * MT)),
+                       dim3(waves * 64), bytes, s, p);
+    return check_launch();
+}
 template <class T, int MT>
 static int launch_rows(const ProductArgs &p, hipStream_t s) {
-    const long blocks = ceil_div_l(p.K, 8 * Chunk<T>::n);
-    const int waves = (int)(blocks < kRowsWaves<MT> ? blocks : kRowsWaves<MT>);
-    hipLaunchKernelGGL((product_rows_kernel<T, MT>), dim3((unsigned)ceil_div_l(p.N, 16), (unsigned)ceil_div_l(p.M, 16 * MT)), dim3(waves * 64),
-                       waves * MT * 1024, s, p);
-    return check_launch();
+    return p.half ? launch_rows_of<T, MT, true>(p, s) : launch_rows_of<T, MT, false>(p, s);
 }
 template <class T>
 int launch_product_rows(const ProductArgs &p, hipStream_t s) {

@@ -38,7 +38,7 @@ __device__ __forceinline__ void split(float x, float y, uint32_t (&o)[3]) {
 // again, whose results are not stored; with k across the rows, the chunk that ends beyond the last column is read as the last whole
 // chunk and shifted on its way to LDS (EDGE; below a chunk's columns: NARROW, no main loop).  Only the last tile of a k that is no whole
 // number of tiles holds zeros, and is read on its own.
-template <class T, int R, bool ACROSS, int THREADS>
+template <class T, int R, bool ACROSS, int THREADS, bool GATED = false>
 struct Staged {
     static constexpr int E = Chunk<T>::n, BK = kStagedK<T>, P = kStagedPlanes<T>;
     typedef LdsTile<R, BK, ACROSS> Tile;
@@ -54,7 +54,7 @@ struct Staged {
     static __device__ __forceinline__ bool edge(long all, long row0) { return ACROSS && row0 + R > all; }
     static __device__ __forceinline__ bool narrow(long all) { return ACROSS && all < E; }
 
-    __device__ __forceinline__ void setup(const T *p, long ld, long all, long row0, long k_begin) {
+    __device__ __forceinline__ void setup(const T *p, long ld, long all, long row0, long k_begin, long half = 0) {
         step = ACROSS ? BK * ld : BK;
 #pragma unroll
         for (int i = 0; i < per; ++i) {
@@ -64,7 +64,7 @@ struct Staged {
                 at[i] = p + (k_begin + r) * ld + col;
                 shift[i] = row0 + c < all ? (int)(row0 + c - col) : 0;
             } else {
-                at[i] = p + (row0 + r < all ? row0 + r : all - 1) * ld + k_begin + c;
+                at[i] = p + (GATED ? gated_row(row0 + r, half) : row0 + r < all ? row0 + r : all - 1) * ld + k_begin + c;
             }
         }
     }
@@ -76,12 +76,13 @@ struct Staged {
         for (int i = 0; i < per; ++i) at[i] += go;
     }
     // the tile from k on, of which `left` values of k exist
-    static __device__ __forceinline__ void load_last(Values &t, const T *p, long ld, long all, long row0, long k, int left) {
+    static __device__ __forceinline__ void load_last(Values &t, const T *p, long ld, long all, long row0, long k, int left, long half = 0) {
 #pragma unroll
         for (int i = 0; i < per; ++i) {
             const int r = row_of(i), c = column_of(i);
             const long rows = all - row0 - (ACROSS ? c : r);
             if constexpr (ACROSS) t.v[i] = load_raw_part(p + (k + r) * ld + row0 + c, r >= left || rows <= 0 ? 0 : rows < E ? (int)rows : E);
+            else if constexpr (GATED) t.v[i] = load_raw_part(p + gated_row(row0 + r, half) * ld + k + c, gated_exists(row0 + r, half) ? left - c : 0);
             else t.v[i] = load_raw_part(p + (row0 + r) * ld + k + c, rows <= 0 ? 0 : left - c);
         }
     }
@@ -127,7 +128,7 @@ __device__ __forceinline__ f32x4 mfma(const bf16x8 &b, const bf16x8 &a, const f3
 }
 
 // A wave's sums over its share of k that are not finite, with the float32 matrix instructions straight from memory
-template <int TM, int TN, bool AA, bool BA>
+template <int TM, int TN, bool AA, bool BA, bool GATED>
 __device__ __forceinline__ void sum_again(const ProductArgs &p, f32x4 (&acc)[TM][TN], long m0, long n0, long k_begin, long k_end, int lane) {
     const float *a = static_cast<const float *>(p.a), *b = static_cast<const float *>(p.b);
     f32x4 again[TM][TN];
@@ -146,7 +147,8 @@ __device__ __forceinline__ void sum_again(const ProductArgs &p, f32x4 (&acc)[TM]
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
             const long n = n0 + j * 16 + (lane & 15);
-            fb[j] = k < k_end && n < p.N ? b[BA ? k * p.ldb + n : n * p.ldb + k] : 0.f;
+            if constexpr (GATED) fb[j] = k < k_end && gated_exists(n, p.half) ? b[gated_row(n, p.half) * p.ldb + k] : 0.f;
+            else fb[j] = k < k_end && n < p.N ? b[BA ? k * p.ldb + n : n * p.ldb + k] : 0.f;
         }
 #pragma unroll
         for (int i = 0; i < TM; ++i)
@@ -164,11 +166,12 @@ __device__ __forceinline__ void sum_again(const ProductArgs &p, f32x4 (&acc)[TM]
 // WM x WN waves of TM x TN tiles of 16 x 16.  AHEAD: tiles of k in registers or on their way there (small ones are multiplied faster than the
 // next arrives).  BUFFERS = 2: one barrier a tile, and the next is split and stored while this one is multiplied.  KG: groups of so many
 // waves that share the tiles of k, each with buffers of its own; their sums are added through LDS.
-template <class T, int WM, int WN, int TM, int TN, int AHEAD, int BUFFERS, int KG, bool AA, bool BA>
+template <class T, int WM, int WN, int TM, int TN, int AHEAD, int BUFFERS, int KG, bool AA, bool BA, bool GATED>
 __global__ __launch_bounds__(WM *WN * 64 * KG, KG == 1 ? 2 : 1) void product_staged_kernel(const ProductArgs p) {
     constexpr int BM = WM * TM * 16, BN = WN * TN * 16, BK = kStagedK<T>, P = kStagedPlanes<T>, THREADS = WM * WN * 64;
     typedef Staged<T, BM, AA, THREADS> SA;
-    typedef Staged<T, BN, BA, THREADS> SB;
+    typedef Staged<T, BN, BA, THREADS, GATED> SB;
+    static_assert(!GATED || (!AA && !BA), "gated: a forward's product");
     constexpr int BYTES = P * (SA::Tile::bytes + SB::Tile::bytes);
     extern __shared__ __align__(16) char all_lds[];
     const int lane = threadIdx.x & 63, wave = (threadIdx.x % THREADS) >> 6, group = __builtin_amdgcn_readfirstlane(threadIdx.x / THREADS);
@@ -222,7 +225,7 @@ __global__ __launch_bounds__(WM *WN * 64 * KG, KG == 1 ? 2 : 1) void product_sta
         SA sa;
         SB sb;
         sa.setup(a, p.lda, p.M, m0, k_begin + (long)first * BK);
-        sb.setup(b, p.ldb, p.N, n0, k_begin + (long)first * BK);
+        sb.setup(b, p.ldb, p.N, n0, k_begin + (long)first * BK, p.half);
         typename SA::Values va[AHEAD];
         typename SB::Values vb[AHEAD];
         int next = 0;
@@ -272,7 +275,7 @@ __global__ __launch_bounds__(WM *WN * 64 * KG, KG == 1 ? 2 : 1) void product_sta
         typename SB::Values vb;
         if (group == KG - 1) {
             SA::load_last(va, a, p.lda, p.M, m0, k, left);
-            SB::load_last(vb, b, p.ldb, p.N, n0, k, left);
+            SB::load_last(vb, b, p.ldb, p.N, n0, k, left, p.half);
         }
         __syncthreads();
         if (group == KG - 1) {
@@ -316,26 +319,27 @@ __global__ __launch_bounds__(WM *WN * 64 * KG, KG == 1 ? 2 : 1) void product_sta
             for (int j = 0; j < TN; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) finite = finite && fabsf(acc[i][j][e]) < __builtin_inff();
-        if (!__all(finite)) sum_again<TM, TN, AA, BA>(p, acc, m0 + wm, n0 + wn, k_begin, k_end, lane);
+        if (!__all(finite)) sum_again<TM, TN, AA, BA, GATED>(p, acc, m0 + wm, n0 + wn, k_begin, k_end, lane);
     }
-    finish_wave<T, TM, TN>(p, acc, m0 + wm, n0 + wn, lane);
+    finish_wave<T, GATED, TM, TN>(p, acc, m0 + wm, n0 + wn, lane);
 }
 
-template <class T, int WM, int WN, int TM, int TN, int AHEAD, int BUFFERS, int KG, bool AA, bool BA>
+template <class T, int WM, int WN, int TM, int TN, int AHEAD, int BUFFERS, int KG, bool AA, bool BA, bool GATED>
 static int launch_staged_layout(ProductArgs p, hipStream_t s) {
     constexpr int BM = WM * TM * 16, BN = WN * TN * 16, bytes = KG * BUFFERS * kStagedPlanes<T> * (BM + BN) * kStagedK<T> * 2;
     p.tiles_m = (int)ceil_div_l(p.M, BM);
     p.tiles_n = (int)ceil_div_l(p.N, BN);
-    if (int rc = allow_dynamic_lds<&product_staged_kernel<T, WM, WN, TM, TN, AHEAD, BUFFERS, KG, AA, BA>>(bytes)) return rc;
-    hipLaunchKernelGGL((product_staged_kernel<T, WM, WN, TM, TN, AHEAD, BUFFERS, KG, AA, BA>), dim3((unsigned)p.tiles_m * p.tiles_n, p.splits),
+    if (int rc = allow_dynamic_lds<&product_staged_kernel<T, WM, WN, TM, TN, AHEAD, BUFFERS, KG, AA, BA, GATED>>(bytes)) return rc;
+    hipLaunchKernelGGL((product_staged_kernel<T, WM, WN, TM, TN, AHEAD, BUFFERS, KG, AA, BA, GATED>), dim3((unsigned)p.tiles_m * p.tiles_n, p.splits),
                        dim3(WM * WN * 64 * KG), bytes, s, p);
     return check_launch();
 }
 template <class T, int WM, int WN, int TM, int TN, int AHEAD, int BUFFERS, int KG = 1>
 static int launch_staged(const ProductArgs &p, bool a_across, bool b_across, hipStream_t s) {
-    if (a_across) return launch_staged_layout<T, WM, WN, TM, TN, AHEAD, BUFFERS, KG, true, true>(p, s);
-    return b_across ? launch_staged_layout<T, WM, WN, TM, TN, AHEAD, BUFFERS, KG, false, true>(p, s)
-                    : launch_staged_layout<T, WM, WN, TM, TN, AHEAD, BUFFERS, KG, false, false>(p, s);
+    if (p.half) return launch_staged_layout<T, WM, WN, TM, TN, AHEAD, BUFFERS, KG, false, false, true>(p, s);
+    if (a_across) return launch_staged_layout<T, WM, WN, TM, TN, AHEAD, BUFFERS, KG, true, true, false>(p, s);
+    return b_across ? launch_staged_layout<T, WM, WN, TM, TN, AHEAD, BUFFERS, KG, false, true, false>(p, s)
+                    : launch_staged_layout<T, WM, WN, TM, TN, AHEAD, BUFFERS, KG, false, false, false>(p, s);
 }
 template <>
 int launch_product_staged<float>(const ProductArgs &p, bool a_across, bool b_across, StagedShape shape, hipStream_t s) {

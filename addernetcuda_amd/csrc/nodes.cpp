@@ -5,100 +5,13 @@
 // every tensor from Python more than a microsecond a tensor -- as much as or more than these kernels take on all but large tensors.  The module
 // is compiled against torch's C++ interface; the kernels stay behind include/addernet_hip.h, whose entry points it is handed by address (bind), so
 // that it runs on the library that the package has loaded.
-#include <Python.h>
+#include "nodes.hpp"
 
-#include <ATen/ops/empty.h>
-#include <ATen/ops/zeros.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
-#include <torch/csrc/autograd/python_variable.h>
+namespace nodes {
 
-#include <string>
-#include <vector>
-
-#include "../../include/addernet_hip.h"
+Library lib;
 
 namespace {
-
-using at::Tensor;
-using torch::autograd::AutogradContext;
-using torch::autograd::Variable;
-using torch::autograd::variable_list;
-
-struct Library {
-    decltype(&adder_strerror) strerror_;
-    decltype(&adder_last_hip_error) last_hip_error;
-    decltype(&adder_linear_fwd_workspace_bytes) linear_fwd_bytes;
-    decltype(&adder_linear_fwd) linear_fwd;
-    decltype(&adder_linear_bwd_workspace_bytes) linear_bwd_bytes;
-    decltype(&adder_linear_bwd) linear_bwd;
-    decltype(&adder_layer_norm_fwd) norm_fwd;
-    decltype(&adder_layer_norm_bwd_workspace_bytes) norm_bwd_bytes;
-    decltype(&adder_layer_norm_bwd) norm_bwd;
-    decltype(&adder_adamw_step) adamw;
-    decltype(&adder_adamw_step_8bit) adamw8;
-    decltype(&adder_adamw_advance) advance;
-} lib;
-
-void check(int status, const char *what) {
-    if (status == ADDER_OK) return;
-    std::string text = lib.strerror_(status);
-    if (status == ADDER_ERR_HIP) text += std::string(": ") + lib.last_hip_error();
-    TORCH_CHECK(false, what, ": ", text);
-}
-
-// The interpreter is free for other threads while this lives: a launch waits where the queue is full
-struct Released {
-    PyThreadState *const state = PyEval_SaveThread();
-    Released() = default;
-    Released(const Released &) = delete;
-    ~Released() { PyEval_RestoreThread(state); }
-};
-
-int type_of(const Tensor &t) { return t.scalar_type() == at::kBFloat16 ? ADDER_TYPE_BF16 : ADDER_TYPE_F32; }
-void *stream_of(const Tensor &t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
-void *ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
-Tensor bytes_for(size_t n, const Tensor &like) {
-    return n ? at::empty({(int64_t)n}, like.options().dtype(at::kByte)) : Tensor();
-}
-Tensor filled(bool zeros, at::IntArrayRef shape, const at::TensorOptions &options) {
-    return zeros ? at::zeros(shape, options) : at::empty(shape, options);
-}
-std::string shape_text(at::IntArrayRef s) {   // as Python prints it
-    std::string t = "(";
-    for (size_t i = 0; i < s.size(); ++i) t += std::to_string(s[i]) + (i + 1 < s.size() ? ", " : s.size() == 1 ? "," : "");
-    return t + ")";
-}
-
-// t as rows of `width` neighbouring values, and their stride: a view where it is one.  Values of one row lie side by side, and rows that are not all
-// the same one do not overlap.
-struct Rows { Tensor t; long stride, rows; };
-Rows as_rows(const Tensor &t, int64_t width) {
-    const int64_t rows = t.numel() / width;
-    if (t.is_contiguous()) return {t, (long)width, (long)rows};
-    Tensor v = t.dim() == 2 && t.size(1) == width ? t : t.reshape({rows, width});   // (two dimensions may also be one row: all of them normalised)
-    if ((width > 1 && v.stride(1) != 1) || (rows > 1 && v.stride(0) < width && v.stride(0) != 0)) v = v.contiguous();
-    return {v, rows > 1 ? (long)v.stride(0) : (long)width, (long)rows};
-}
-
-// Gradients that these nodes give have no formula to be differentiated again: whoever tries is told so
-variable_list once(variable_list grads, const char *what) {
-    if (!at::GradMode::is_enabled()) return grads;
-    variable_list some;
-    for (const auto &g : grads)
-        if (g.defined()) some.push_back(g.detach().requires_grad_(true));
-    if (some.empty()) return grads;
-    auto error = std::make_shared<torch::autograd::DelayedError>(std::string("trying to differentiate twice a function that was marked with once_differentiable: ") + what,
-                                                                 (int64_t)some.size());
-    auto wrapped = (*error)(std::move(some));
-    size_t k = 0;
-    for (auto &g : grads)
-        if (g.defined()) g = wrapped[k++];
-    return grads;
-}
 
 // ---- linear layers -----------------------------------------------------------------------------------------------------
 Tensor linear_forward(const Tensor &x, const Tensor &w, const Tensor &bias, const Tensor &residual, int64_t act, Tensor *pre) {
@@ -120,10 +33,6 @@ Tensor linear_forward(const Tensor &x, const Tensor &w, const Tensor &bias, cons
           "adder_linear_fwd");
     return y;
 }
-
-// Arguments that may be absent reach a node as optionals; its edges count those that are there
-typedef std::optional<Variable> Maybe;
-Maybe maybe(const Tensor &t) { return t.defined() ? Maybe(t) : Maybe(); }
 
 struct LinearAct : public torch::autograd::Function<LinearAct> {
     static Variable forward(AutogradContext *ctx, const Variable &x, const Variable &w, const Maybe &has_bias, const Maybe &has_residual, int64_t act) {
@@ -175,12 +84,6 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
         return once(std::move(out), "linear_act");
     }
 };
-
-Tensor optional_tensor(PyObject *o, const char *name) {
-    if (o == Py_None) return Tensor();
-    if (!THPVariable_Check(o)) throw torch::TypeError(std::string(name) + " must be a torch.Tensor");
-    return THPVariable_Unpack(o);
-}
 
 // linear_act(x, weight, bias or None, residual or None, act): all plain GPU tensors, x float32 or bfloat16, no empty weight
 PyObject *py_linear_act(PyObject *, PyObject *const *args, Py_ssize_t count) {
@@ -523,20 +426,46 @@ PyObject *py_bind(PyObject *, PyObject *names) {
     take("adder_adamw_step", lib.adamw);
     take("adder_adamw_step_8bit", lib.adamw8);
     take("adder_adamw_advance", lib.advance);
+    take("adder_rms_norm_fwd", lib.rms_fwd);
+    take("adder_rms_norm_fwd_codes", lib.rms_fwd_codes);
+    take("adder_rms_norm_bwd_workspace_bytes", lib.rms_bwd_bytes);
+    take("adder_rms_norm_bwd", lib.rms_bwd);
+    take("adder_quantize", lib.quantize);
+    take("adder_quantize_weight", lib.quantize_weight);
+    take("adder_linear_codes_workspace_bytes", lib.codes_bytes);
+    take("adder_linear_codes", lib.codes);
+    take("adder_gated_fwd_workspace_bytes", lib.gated_fwd_bytes);
+    take("adder_gated_fwd", lib.gated_fwd);
+    take("adder_gated_bwd_workspace_bytes", lib.gated_bwd_bytes);
+    take("adder_gated_bwd", lib.gated_bwd);
+    take("adder_distill_in_rows", lib.distill_in_rows);
+    take("adder_distill_workspace_bytes", lib.distill_bytes);
+    take("adder_distill_fwd", lib.distill_fwd);
+    take("adder_distill_bwd", lib.distill_bwd);
     if (PyErr_Occurred()) return nullptr;
     Py_RETURN_NONE;
     END_HANDLE_TH_ERRORS
 }
 
-PyMethodDef methods[] = {
+PyMethodDef own_methods[] = {
     {"bind", py_bind, METH_O, nullptr},
     {"linear_act", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(py_linear_act)), METH_FASTCALL, nullptr},
     {"layer_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(py_layer_norm)), METH_FASTCALL, nullptr},
     {"adamw_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(py_adamw_step)), METH_FASTCALL, nullptr},
-    {nullptr, nullptr, 0, nullptr},
 };
-PyModuleDef module = {PyModuleDef_HEAD_INIT, "_nodes", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+PyObject *create() {
+    static std::vector<PyMethodDef> methods;
+    if (methods.empty()) {
+        methods.assign(std::begin(own_methods), std::end(own_methods));
+        methods.insert(methods.end(), block_methods.begin(), block_methods.end());
+        methods.push_back({nullptr, nullptr, 0, nullptr});
+    }
+    static PyModuleDef module = {PyModuleDef_HEAD_INIT, "_nodes", nullptr, -1, methods.data(), nullptr, nullptr, nullptr, nullptr};
+    return PyModule_Create(&module);
+}
 
 }  // namespace
+}  // namespace nodes
 
-PyMODINIT_FUNC PyInit__nodes() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__nodes() { return nodes::create(); }

@@ -76,6 +76,54 @@ __device__ __forceinline__ void unpack_half(const uint4 &u, float (&v)[8]) {
     for (int e = 0; e < 8; ++e) v[e] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[e / 2] >> (16 * (e & 1))));
 }
 
+// The activation and its derivative together
+template <bool EXACT>
+__device__ __forceinline__ void both(float z, Act act, float &value, float &slope_) {
+    switch (act) {
+        case Act::relu:
+            value = relu_keep_nan(z);
+            slope_ = z <= 0.f ? 0.f : 1.f;
+            break;
+        case Act::gelu: {
+            float bell;
+            const float p = normal_cdf<EXACT>(z, bell);
+            value = z * p;
+            slope_ = fmaf(0.39894228f * z, bell, p);
+            break;
+        }
+        case Act::silu: {
+            const float s = sigmoid<EXACT>(z);
+            value = z * s;
+            slope_ = fmaf(value, 1.f - s, s);
+            break;
+        }
+        default:
+            value = z;
+            slope_ = 1.f;
+    }
+}
+
+// What a gated layer's forward keeps of its two sums, g and u.  Unlike the z above they are factors of the gradients, so their range counts as
+// much as their digits.  In bfloat16 four neighbouring columns (from a multiple of four on) are four IEEE halves of 11 bits where the largest
+// magnitude among them is from 2^-12 to 65504 -- what is left out of a smaller one is then at most 2^-13 of the largest -- and else four bfloat16.
+// The lowest bit of the first says which (one: halves): gradients are 0.0024 from float64 with it, 0.0029 from bfloat16 alone.  A ReLU's g is
+// always bfloat16: its derivative hangs on the sign of the smallest numbers.
+__device__ __forceinline__ uint2 keep_group(const float (&z)[4], bool halves = true) {
+    const float top = fmaxf(fmaxf(fabsf(z[0]), fabsf(z[1])), fmaxf(fabsf(z[2]), fabsf(z[3])));
+    const bool half = halves && top >= 0x1p-12f && top <= 65504.f;
+    const uint32_t lo = pack_half(z[0], z[1]) | 1u, hi = pack_half(z[2], z[3]);
+    const uint32_t blo = pack_bf16(z[0], z[1]) & ~1u, bhi = pack_bf16(z[2], z[3]);
+    return make_uint2(half ? lo : blo, half ? hi : bhi);
+}
+__device__ __forceinline__ void unpack_kept(const uint4 &u, float (&v)[4]) { unpack(u, v); }
+__device__ __forceinline__ void unpack_kept(const uint4 &u, float (&v)[8]) {
+    float h[8];
+    unpack_half(u, h);
+    unpack(u, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (e < 4 ? u.x : u.z) & 1u ? h[e] : v[e];
+}
+
 // ---- products ------------------------------------------------------------------------------------------------------
 struct ProductArgs {
     const void *a, *b, *bias, *res;
@@ -84,7 +132,17 @@ struct ProductArgs {
     long lda, ldb, ldr, M, N, K, k_share;
     int tiles_m, tiles_n, splits;
     Act act;
+    long half;            // gated: H, the result's columns; N counts the sums of both halves, in whole groups of sixteen
 };
+
+// Gated layers: the weight's first H rows give g, the others u.  A product's columns are then groups of 32: sixteen of g and the same sixteen of u,
+// so that neighbouring tiles of a wave hold what belongs together.  Column v of the product: its row of the weight (one that exists where
+// column v does not), and whether it exists.
+__device__ __forceinline__ long gated_row(long v, long H) {
+    const long c = (v >> 5) * 16 + (v & 15);
+    return (c < H ? c : H - 1) + (v & 16 ? H : 0);
+}
+__device__ __forceinline__ bool gated_exists(long v, long H) { return (v >> 5) * 16 + (v & 15) < H; }
 
 __device__ __forceinline__ void keep(float *p, float z, Act) { *p = z; }
 __device__ __forceinline__ void keep(bf16_t *p, float z, Act act) { *p = keeps_half(2, act) ? (bf16_t)pack_half(z, 0.f) : round_bf16(z); }
@@ -212,10 +270,155 @@ __device__ __forceinline__ void finish_tile(const ProductArgs &p, const f32x4 (&
     }
 }
 
+// `cnt` <= 4 neighbouring columns of row m from column n (a multiple of four) of a gated layer on: y = act(g + bg) (u + bu), and what is kept
+template <class T>
+__device__ __forceinline__ void finish_gated(const ProductArgs &p, long m, long n, int cnt, const float (&gate)[4], const float (&up)[4]) {
+    const T *bias = static_cast<const T *>(p.bias);
+    T *out = static_cast<T *>(p.out) + m * p.half + n, *pre = static_cast<T *>(p.pre);
+    float g[4], u[4], y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        g[e] = e < cnt ? gate[e] + (bias ? ldf(bias + n + e) : 0.f) : 0.f;
+        u[e] = e < cnt ? up[e] + (bias ? ldf(bias + p.half + n + e) : 0.f) : 0.f;
+    }
+    switch (p.act) {   // (outside the loop: one branch for four values)
+        case Act::relu:
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = activate<kExactAct<T>>(g[e], Act::relu) * u[e];
+            break;
+        case Act::gelu:
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = activate<kExactAct<T>>(g[e], Act::gelu) * u[e];
+            break;
+        case Act::silu:
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = activate<kExactAct<T>>(g[e], Act::silu) * u[e];
+            break;
+        default:
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = g[e] * u[e];
+    }
+    T *kg = pre + m * 2 * p.half + n, *ku = kg + p.half;
+    if (cnt == 4) {
+        put4(out, y);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+            if (e < cnt) put(out + e, y[e]);
+    }
+    if (!pre) return;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (e < cnt) {
+                kg[e] = g[e];
+                ku[e] = u[e];
+            }
+    } else {
+        const uint2 a = keep_group(g, p.act != Act::relu), b = keep_group(u);
+        const uint32_t w[2][2] = {{a.x, a.y}, {b.x, b.y}};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (e < cnt) {
+                kg[e] = (bf16_t)(w[0][e / 2] >> (16 * (e & 1)));
+                ku[e] = (bf16_t)(w[1][e / 2] >> (16 * (e & 1)));
+            }
+    }
+}
+
+// The same for a wave's tile whose columns all exist (in bfloat16 the exchange of finish_tile, for two groups at a time where a wave has them)
+template <class T, int TM, int TN, Act ACT>
+__device__ __forceinline__ void finish_gated_tile(const ProductArgs &p, const f32x4 (&acc)[TM][TN], long m0, long n0, int lane) {
+    constexpr int G = Chunk<T>::n / 4 < TN / 2 ? Chunk<T>::n / 4 : TN / 2;   // groups of sixteen columns that make chunks together
+    const T *bias = static_cast<const T *>(p.bias);
+    T *out = static_cast<T *>(p.out), *pre = static_cast<T *>(p.pre);
+    const int quad = lane >> 4;
+    const long c0 = n0 / 2;
+    float b[TN][4];
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) b[j][e] = 0.f;
+        if (bias) ld_strip<4>(bias + (j & 1 ? p.half : 0) + c0 + (j / 2) * 16 + quad * 4, b[j]);
+    }
+    const long at = c0 + (G == 1 ? quad * 4 : (quad & 1) * 16 + (quad >> 1) * 8);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+        const long m = m0 + i * 16 + (lane & 15);
+#pragma unroll
+        for (int j = 0; j < TN; j += 2 * G) {
+            float g[G][4], u[G][4], y[G][4];
+#pragma unroll
+            for (int h = 0; h < G; ++h)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    g[h][e] = acc[i][j + 2 * h][e] + b[j + 2 * h][e];
+                    u[h][e] = acc[i][j + 2 * h + 1][e] + b[j + 2 * h + 1][e];
+                    y[h][e] = activate<kExactAct<T>>(g[h][e], ACT) * u[h][e];
+                }
+            T *o = out + m * p.half + at + j * 8, *k = pre + m * 2 * p.half + at + j * 8;
+            if constexpr (sizeof(T) == 4) {
+                store_raw(o, pack(y[0]));
+                if (pre) {
+                    store_raw(k, pack(g[0]));
+                    store_raw(k + p.half, pack(u[0]));
+                }
+            } else if constexpr (G == 2) {
+                const auto write = [](T *to, uint2 a, uint2 c) {   // (odd rows of sixteen lanes of the first with the even ones of the second)
+                    swap_rows(a.x, c.x);
+                    swap_rows(a.y, c.y);
+                    store_raw(to, make_uint4(a.x, a.y, c.x, c.y));
+                };
+                write(o, make_uint2(pack_bf16(y[0][0], y[0][1]), pack_bf16(y[0][2], y[0][3])), make_uint2(pack_bf16(y[1][0], y[1][1]), pack_bf16(y[1][2], y[1][3])));
+                if (pre) {
+                    write(k, keep_group(g[0], ACT != Act::relu), keep_group(g[1], ACT != Act::relu));
+                    write(k + p.half, keep_group(u[0]), keep_group(u[1]));
+                }
+            } else {
+                put4(o, y[0]);
+                if (pre) {
+                    const auto write = [](T *to, uint2 a) {
+                        *reinterpret_cast<u16x4_any *>(to) = u16x4_any{(uint16_t)a.x, (uint16_t)(a.x >> 16), (uint16_t)a.y, (uint16_t)(a.y >> 16)};
+                    };
+                    write(k, keep_group(g[0], ACT != Act::relu));
+                    write(k + p.half, keep_group(u[0]));
+                }
+            }
+        }
+    }
+}
+
 // A wave's results: the epilogue, or the sums of a share of k
-template <class T, int TM, int TN>
+template <class T, bool GATED, int TM, int TN>
 __device__ __forceinline__ void finish_wave(const ProductArgs &p, const f32x4 (&acc)[TM][TN], long m0, long n0, int lane) {
-    if (p.splits == 1 && m0 + TM * 16 <= p.M && n0 + TN * 16 <= p.N) {
+    if constexpr (GATED) {
+        static_assert(TN % 2 == 0, "a wave holds both halves of a column");
+        if (p.splits == 1) {
+            if (m0 + TM * 16 <= p.M && n0 / 2 + TN * 8 <= p.half) {
+                switch (p.act) {
+                    case Act::relu: finish_gated_tile<T, TM, TN, Act::relu>(p, acc, m0, n0, lane); break;
+                    case Act::gelu: finish_gated_tile<T, TM, TN, Act::gelu>(p, acc, m0, n0, lane); break;
+                    case Act::silu: finish_gated_tile<T, TM, TN, Act::silu>(p, acc, m0, n0, lane); break;
+                    default: finish_gated_tile<T, TM, TN, Act::none>(p, acc, m0, n0, lane);
+                }
+                return;
+            }
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+                const long m = m0 + i * 16 + (lane & 15);
+                if (m >= p.M) continue;
+#pragma unroll
+                for (int j = 0; j < TN; j += 2) {
+                    const long n = n0 / 2 + j * 8 + (lane >> 4) * 4;
+                    if (n >= p.half) continue;
+                    const float g[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+                    const float u[4] = {acc[i][j + 1][0], acc[i][j + 1][1], acc[i][j + 1][2], acc[i][j + 1][3]};
+                    finish_gated<T>(p, m, n, p.half - n < 4 ? (int)(p.half - n) : 4, g, u);
+                }
+            }
+            return;
+        }
+    } else if (p.splits == 1 && m0 + TM * 16 <= p.M && n0 + TN * 16 <= p.N) {
         switch (p.act) {
             case Act::relu: finish_tile<T, TM, TN, Act::relu>(p, acc, m0, n0, lane); break;
             case Act::gelu: finish_tile<T, TM, TN, Act::gelu>(p, acc, m0, n0, lane); break;
@@ -295,9 +498,50 @@ __device__ __forceinline__ void tile_of(int id, int tiles_m, int tiles_n, int &t
     tn = in / high;
 }
 
+// ---- which shape ----------------------------------------------------------------------------------------------------
+// A launch's time is estimated for every shape of tile and number of shares of k, and the least is taken.  The workgroups run in rounds
+// of as many as the card holds, each steps * step + tile us: steps of 64 (float32: 32) values of k; `step` measured with every compute
+// unit full (8192 x 8192 x 1024 and 8192^3), less in proportion where fewer workgroups share one, but at least `alone` (1024^3); `tile` the first
+// loads, the epilogue and the start, once more where a second output is written.  Shares of k pay for their sums' way through memory (5 TB/s both ways) and the join's launch.
+static constexpr int kCUs = 256;
+struct Shape { int bm, bn, per_cu; float step, alone, tile; };
+static constexpr int kSplitMax = 16;
+
+struct ProductPlan { int shape, splits; long k_share; float us; };
+
+template <int N>
+ProductPlan plan_product(const Shape (&shapes)[N], int bk, long M, long N_, long K, int outputs) {
+    static constexpr int kSplits[] = {1, 2, 3, 4, 6, 8, 12, kSplitMax};
+    ProductPlan best{0, 1, K, 0.f};
+    const long steps = ceil_div_l(K, bk);
+    for (int i = 0; i < N; ++i) {
+        const Shape &h = shapes[i];
+        const float tiles = (float)ceil_div_l(M, h.bm) * (float)ceil_div_l(N_, h.bn);
+        for (int splits : kSplits) {
+            if (splits > steps || (splits > 1 && tiles * splits > 4.f * kCUs)) break;
+            const long share = ceil_div_l(steps, splits);
+            const float groups = tiles * splits;
+            const float slots = (float)(kCUs * h.per_cu), whole = floorf(groups / slots), rest = groups - whole * slots;
+            float us = 3.f + whole * (share * h.step + h.tile * outputs);
+            if (rest > 0.f) {
+                const float shared = h.step * ceilf(rest / kCUs) / h.per_cu;
+                us += share * (shared > h.alone ? shared : h.alone) + h.tile * outputs;
+            }
+            if (splits > 1) us += 3.f + (float)M * (float)N_ * splits * 8.f / 5e6f;
+            if (best.us == 0.f || us < best.us) {
+                const int used = (int)ceil_div_l(steps, share);
+                best = ProductPlan{i, used, used > 1 ? share * bk : K, us};
+            }
+        }
+    }
+    return best;
+}
 // Launches of the tiled kernels; p has everything but its tiles
 enum class StreamShape { big, wide, mid, small };   // 256 x 256, 128 x 256, 128 x 128, 64 x 64 results a workgroup
+// (p.half: a gated layer's, both operands along)
 int launch_product_stream(ProductArgs p, bool a_across, bool b_across, StreamShape shape, hipStream_t s);
+template <class T>
+int launch_product_join(const ProductArgs &p, hipStream_t s);   // the shares' sums, added up
 // 128 x 128, 64 x 64, and (float32) both by twice as many waves, for launches that leave a compute unit one workgroup
 enum class StagedShape { large, small, alone, pair };
 template <class T>

@@ -40,8 +40,10 @@ import torch.nn.functional as F
 
 from . import adder as _adder
 from .bn_act import BatchNormAct2d
+from .gated import GatedLinear
 from .layer_norm import LayerNorm
 from .linear import LinearAct
+from .rms_norm import RMSNorm
 from .unit import adder_bn_act
 from .resnet20 import StemConv2d   # nn.Conv2d with the same parameters; forward and weight gradient through the tiled kernels
 
@@ -413,3 +415,52 @@ class TokenMLP(nn.Module):
 def token_mlp(**kwargs):
     """``TokenMLP`` with its defaults: 128 channels, 64 patches, four pairs of MLPs."""
     return TokenMLP(**kwargs)
+
+
+class GatedMLP(nn.Module):
+    """``s + down(silu(gate(norm(s))) * up(norm(s)))`` over the last dimension, with an RMS norm and ``s`` the input or, where something is ``added`` to it, their
+    sum: three kernels (the sum is the norm's, gate and up are one product, the shortcut rides on the last)."""
+
+    def __init__(self, width, hidden, act="silu", fused=True):
+        super().__init__()
+        self.fused, self.act = fused, act
+        self.norm = RMSNorm(width) if fused else nn.RMSNorm(width, eps=1e-6)
+        self.gated = GatedLinear(width, hidden, act=act) if fused else nn.Linear(width, 2 * hidden, bias=False)
+        self.down = LinearAct(hidden, width, bias=False) if fused else nn.Linear(hidden, width, bias=False)
+
+    def forward(self, x, added=None):
+        if self.fused:
+            y, s = (self.norm(x), x) if added is None else self.norm(added, residual=x)
+            return self.down(self.gated(y), residual=s)
+        s = x if added is None else added + x
+        gate, up = self.gated(self.norm(s)).chunk(2, -1)
+        return s + self.down({"none": lambda t: t, "relu": F.relu, "gelu": F.gelu, "silu": F.silu}[self.act](gate) * up)
+
+
+class GatedTokenMLP(nn.Module):
+    """``TokenMLP`` with gated blocks: an adder layer and BatchNorm, then ``layers`` times a linear layer over the patches, whose result is added, and a gated block
+    over the channels; RMS norm, the patches' mean, a linear classifier.  For 32x32 images."""
+
+    def __init__(self, width=128, layers=4, patch=4, num_classes=10, image=32, adder2d_cls=None, fused=True, **adder_kw):
+        super().__init__()
+        make = adder2d_cls or _adder.adder2d
+        tokens = (image // patch) ** 2
+        self.fused = fused
+        self.stem = make(3, width, kernel_size=patch, stride=patch, padding=0, bias=False, **adder_kw)
+        self.bn = _bn(width, False, fused)
+        self.over_tokens = nn.ModuleList([LinearAct(tokens, tokens, act="gelu") if fused else nn.Linear(tokens, tokens) for _ in range(layers)])
+        self.over_channels = nn.ModuleList([GatedMLP(width, 2 * width, fused=fused) for _ in range(layers)])
+        self.norm = RMSNorm(width) if fused else nn.RMSNorm(width, eps=1e-6)
+        self.classifier = LinearAct(width, num_classes) if fused else nn.Linear(width, num_classes)
+
+    def forward(self, x):
+        x = self.bn(self.stem(x)).flatten(2).transpose(1, 2)   # (images, patches, channels)
+        for tokens, channels in zip(self.over_tokens, self.over_channels):
+            mixed = tokens(x.transpose(1, 2))
+            x = channels(x, added=(mixed if self.fused else F.gelu(mixed)).transpose(1, 2))
+        return self.classifier(self.norm(x).mean(1))
+
+
+def gated_mlp(**kwargs):
+    """``GatedTokenMLP`` with its defaults: 128 channels, 64 patches, four gated blocks."""
+    return GatedTokenMLP(**kwargs)

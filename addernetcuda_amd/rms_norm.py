@@ -1,0 +1,60 @@
+"""Root-mean-square normalisation over the last dimension of a tensor, with the addition of a shortcut in front of it: the sum, its norm and, in
+the backward, the shortcut's own gradient in one pass over the rows each (csrc/rms_norm.hip).  Arguments, outputs and the autograd node are
+csrc/nodes_blocks.cpp; the same norm with a result of 8-bit codes is ``fp8.rms_norm_fp8``.
+
+float32, or bfloat16 with a bfloat16 or float32 weight; sums and statistics are 32 bits.  Inside ``torch.autocast`` the result is float32, as
+torch's own is.  CPU tensors, other types, tensor subclasses and calls that something records, traces or transforms go through torch's own
+operators.
+"""
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+
+from ._lib import nodes, plain_tensors
+from .layer_norm import _BELOW_F32
+from .linear import TYPES, _plus
+
+
+def _check(x, weight, eps):
+    if not eps >= 0:
+        raise RuntimeError(f"eps must not be negative, got {eps}")
+    if x.dim() == 0:
+        raise RuntimeError("x must have a dimension")
+    if weight is not None and tuple(weight.shape) != tuple(x.shape[-1:]):
+        raise RuntimeError(f"weight must have shape ({x.shape[-1]},), got {tuple(weight.shape)}")
+
+
+def _torch_rms_norm(x, weight, eps, residual):
+    _check(x, weight, eps)
+    s = x if residual is None else _plus(x, residual)
+    if weight is not None and weight.dtype != s.dtype:
+        y = F.rms_norm(s.to(weight.dtype), s.shape[-1:], weight, eps).to(s.dtype)
+    else:
+        y = F.rms_norm(s, s.shape[-1:], weight, eps)
+    return y if residual is None else (y, s)
+
+
+def rms_norm(x, weight=None, eps=1e-6, residual=None):
+    """``s / sqrt(mean(s^2) + eps) * weight`` over the last dimension of ``s``, which is ``x`` or, where a ``residual`` is given that broadcasts
+    to its shape, ``x + residual``; then the result is the pair of this and ``s``."""
+    if x.is_cuda and torch.is_autocast_enabled("cuda"):   # (torch casts everything below float32 to it)
+        x, weight, residual = (t.float() if t is not None and t.dtype in _BELOW_F32 else t for t in (x, weight, residual))
+    if plain_tensors(x, weight, residual) and x.is_cuda and x.dtype in TYPES and x.shape[-1:] != (0,):
+        return nodes().rms_norm(x, weight, eps, residual)
+    return _torch_rms_norm(x, weight, eps, residual)
+
+
+class RMSNorm(nn.RMSNorm):
+    """``nn.RMSNorm`` over the last dimension (same arguments, parameters and state_dict keys) through the kernels above; in the call, a
+    shortcut that is added first: ``y, s = norm(x, residual=shortcut)``."""
+
+    def __init__(self, width, eps=1e-6, elementwise_affine=True, device=None, dtype=None):
+        super().__init__(width, eps=eps, elementwise_affine=elementwise_affine, device=device, dtype=dtype)
+        if len(self.normalized_shape) != 1:
+            raise ValueError(f"RMSNorm is over the last dimension, got {tuple(self.normalized_shape)}")
+
+    def forward(self, x, residual=None):
+        if tuple(x.shape[-1:]) != tuple(self.normalized_shape):
+            raise RuntimeError(f"x has shape {tuple(x.shape)} but the last dimension is to be {self.normalized_shape[0]}")
+        eps = self.eps if self.eps is not None else torch.finfo(x.dtype).eps
+        return rms_norm(x, self.weight, eps, residual)

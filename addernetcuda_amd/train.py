@@ -16,6 +16,8 @@ processes are needed.  What it adds: the training step of a full batch runs as o
     python -m addernetcuda_amd.train --data cifar10.npz --epochs 400 --output-dir models/
     python -m addernetcuda_amd.train --data cifar10.npz --resume models/addernet.pt --eval-only
     python -m addernetcuda_amd.train --arch token_mlp --optimizer adamw8bit --lr 0.002 --weight-decay 0.05
+    python -m addernetcuda_amd.train --arch gated_mlp --optimizer adamw --lr 0.002 --teacher models/resnet20.pt --teacher-arch resnet20
+    python -m addernetcuda_amd.train --arch gated_mlp --resume models/addernet.pt --eval-only --fp8
     (npz keys: x_train (N,32,32,3) or (N,3,32,32) uint8, y_train (N,), x_test, y_test)
 """
 import argparse
@@ -109,11 +111,29 @@ def evaluate(net, x_u8, y, batch, bf16=False):
     return loss_sum / n, correct / n
 
 
-def train_step(net, opt, images, labels, bf16=False):
+class Teacher:
+    """A trained network that a student learns from: its ``top`` largest logits for a batch, and how much they count beside the labels."""
+
+    def __init__(self, net, top=5, temperature=4.0, weight=0.5, bf16=False):
+        self.net, self.top, self.temperature, self.weight, self.bf16 = net.eval(), top, temperature, weight, bf16
+
+    def __call__(self, images):
+        with torch.no_grad():
+            logits = forward_pass(self.net, images, self.bf16)
+            return logits.topk(min(self.top, logits.shape[1]), 1)
+
+    def loss(self, logits, labels, top):
+        from addernetcuda_amd.distill import distillation_loss
+        return distillation_loss(logits, *top, labels, temperature=self.temperature, alpha=self.weight)
+
+
+def train_step(net, opt, images, labels, bf16=False, teacher=None, top=None):
+    """``teacher`` and ``top``, its logits for these images: they join the labels in the loss."""
     from addernetcuda_amd.adder import batched_eta_scaling
     from addernetcuda_amd.head import cross_entropy
     opt.zero_grad(set_to_none=True)
-    loss = cross_entropy(forward_pass(net, images, bf16), labels)   # nn.CrossEntropyLoss of main.py:66,90
+    logits = forward_pass(net, images, bf16)
+    loss = cross_entropy(logits, labels) if teacher is None else teacher.loss(logits, labels, top)   # nn.CrossEntropyLoss of main.py:66,90
     with batched_eta_scaling():   # the adaptive scaling of all adder layers in two launches
         loss.backward()
     opt.step()
@@ -128,29 +148,33 @@ class GraphedStep:
     frozen into the graph); BatchNorm's running statistics and the optimizer state are updated by the graph's
     own kernels.  All calls must come from the same (non-default) stream."""
 
-    def __init__(self, net, opt, warmup=3, bf16=False):
-        self.net, self.opt, self.warmup, self.bf16 = net, opt, warmup, bf16
-        self.graph = self.images = self.labels = self.loss = None
+    def __init__(self, net, opt, warmup=3, bf16=False, teacher=None):
+        self.net, self.opt, self.warmup, self.bf16, self.teacher = net, opt, warmup, bf16, teacher
+        self.graph = self.images = self.labels = self.loss = self.top = None
         self.calls = 0
 
     def __call__(self, images, labels):
         self.calls += 1
+        top = None if self.teacher is None else self.teacher(images)   # (outside the capture)
         if self.graph is None and self.calls <= self.warmup:
-            return train_step(self.net, self.opt, images, labels, self.bf16)
+            return train_step(self.net, self.opt, images, labels, self.bf16, self.teacher, top)
         if self.graph is None:
             self.images, self.labels = images.clone(), labels.clone()
+            self.top = None if top is None else tuple(t.clone() for t in top)
             self.opt.zero_grad(set_to_none=True)
             self.graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(self.graph, stream=torch.cuda.current_stream()):
-                self.loss = train_step(self.net, self.opt, self.images, self.labels, self.bf16)
+                self.loss = train_step(self.net, self.opt, self.images, self.labels, self.bf16, self.teacher, self.top)
         else:
             self.images.copy_(images)
             self.labels.copy_(labels)
+            for mine, t in zip(self.top or (), top or ()):
+                mine.copy_(t)
         self.graph.replay()
         return self.loss.clone()
 
 
-def train_one_epoch(net, opt, x_u8, y, batch, generator=None, graphed=None, bf16=False):
+def train_one_epoch(net, opt, x_u8, y, batch, generator=None, graphed=None, bf16=False, teacher=None):
     """``graphed``: a GraphedStep for batches of exactly ``batch`` images (the tail batch runs eagerly)."""
     net.train()
     n = x_u8.shape[0]
@@ -162,17 +186,20 @@ def train_one_epoch(net, opt, x_u8, y, batch, generator=None, graphed=None, bf16
             break
         images = augment(normalise(x_u8[idx]), generator)
         step = graphed if graphed is not None and idx.numel() == batch else None
-        losses.append(step(images, y[idx]) if step else train_step(net, opt, images, y[idx], bf16))
+        if step:
+            losses.append(step(images, y[idx]))
+        else:
+            losses.append(train_step(net, opt, images, y[idx], bf16, teacher, None if teacher is None else teacher(images)))
     return torch.stack(losses).mean().item()
 
 
-ARCHS = ("resnet20", "vgg_small", "densenet_cifar", "resnet50", "token_mlp")
+ARCHS = ("resnet20", "vgg_small", "densenet_cifar", "resnet50", "token_mlp", "gated_mlp")
 OPTIMIZERS = ("sgd", "adamw", "adamw8bit")
 
 
 def build_network(arch, eta, num_classes=10):
     """The reference's networks for 32x32 inputs (main.py:66 builds resnet20; vgg.py, densenet.py and resnet50.py
-    are its other model files), and ``token_mlp``: an adder layer with residual MLPs behind it."""
+    are its other model files), and ``token_mlp`` and ``gated_mlp``: an adder layer with residual MLPs, or gated blocks, behind it."""
     if arch == "resnet20":
         from addernetcuda_amd.resnet20 import resnet20
         return resnet20(eta=eta, num_classes=num_classes)
@@ -206,13 +233,23 @@ def run(args):
     # the learning rate lives on the device so that the captured step sees each epoch's value
     lr_now = torch.tensor(float(args.lr), device=dev)
     opt = build_optimizer(args.optimizer, net.parameters(), lr_now, args.weight_decay)
+    if args.fp8 and not args.eval_only:
+        raise ValueError("--fp8 goes with --eval-only: there are no gradients through codes of 8 bits")
     if args.eval_only:   # the reference's test.py: load a checkpoint, one pass over the test split
+        if args.fp8:
+            from addernetcuda_amd.fp8 import serve_fp8
+            serve_fp8(net)
         test_loss, acc = evaluate(net, *data["test"], args.test_batch_size, args.bf16_activations)
         print(f"test loss {test_loss:.4f}  accuracy {acc:.4f}", flush=True)
         return [{"epoch": 0, "test_loss": test_loss, "accuracy": acc}]
     os.makedirs(args.output_dir, exist_ok=True)
     gen = torch.Generator(device=dev).manual_seed(args.seed)
-    graphed = None if args.no_graph else GraphedStep(net, opt, bf16=args.bf16_activations)
+    teacher = None
+    if args.teacher:
+        taught = build_network(args.teacher_arch, args.eta).to(dev)
+        taught.load_state_dict(torch.load(args.teacher, map_location=dev, weights_only=True))
+        teacher = Teacher(taught, args.teacher_top, args.temperature, args.teacher_weight, args.bf16_activations)
+    graphed = None if args.no_graph else GraphedStep(net, opt, bf16=args.bf16_activations, teacher=teacher)
     stream = torch.cuda.Stream()   # graph capture needs a stream of its own; the eager steps share it
     best, history = 0.0, []
     for epoch in range(1, args.epochs + 1):
@@ -222,7 +259,7 @@ def run(args):
         t0 = time.time()
         stream.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(stream):
-            train_loss = train_one_epoch(net, opt, *data["train"], args.batch_size, gen, graphed, args.bf16_activations)
+            train_loss = train_one_epoch(net, opt, *data["train"], args.batch_size, gen, graphed, args.bf16_activations, teacher)
         torch.cuda.synchronize()
         dt = time.time() - t0
         test_loss, acc = evaluate(net, *data["test"], args.test_batch_size, args.bf16_activations)
@@ -256,6 +293,12 @@ def parse_args(argv=None):
     p.add_argument("--optimizer", choices=OPTIMIZERS, default="sgd", help="sgd as in main.py:67, or AdamW with its state in 32 or 8 bits")
     p.add_argument("--weight-decay", type=float, default=None, help="5e-4 for sgd (main.py:67), 1e-2 for adamw")
     p.add_argument("--arch", choices=ARCHS, default="resnet20", help="network (main.py:66 trains resnet20)")
+    p.add_argument("--fp8", action="store_true", help="with --eval-only: the gated blocks of gated_mlp in 8 bits")
+    p.add_argument("--teacher", type=str, default=None, help="state_dict of a network whose top logits are learned beside the labels")
+    p.add_argument("--teacher-arch", choices=ARCHS, default="resnet20", help="the teacher's network")
+    p.add_argument("--teacher-top", type=int, default=5, help="how many of its logits")
+    p.add_argument("--teacher-weight", type=float, default=0.5, help="how much they count; the labels count the rest")
+    p.add_argument("--temperature", type=float, default=4.0, help="at which student and teacher are compared")
     return p.parse_args(argv)
 
 

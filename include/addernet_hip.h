@@ -31,7 +31,8 @@
  *   [optional]  the cross-entropy loss in one launch each way (adder_cross_entropy_*)
  *   [optional]  the momentum-SGD update of all parameters in one launch (adder_sgd_momentum_step_f32)
  *   [layers]    what networks put beside adder layers, in float32 and bfloat16: linear layers (adder_linear_*), layer
- *               normalisation (adder_layer_norm_*), the AdamW update (adder_adamw_*)
+ *               normalisation (adder_layer_norm_*), the AdamW update (adder_adamw_*), RMS norm (adder_rms_norm_*), gated linear layers
+ *               (adder_gated_*), products of 8-bit codes (adder_quantize*, adder_linear_codes*), the loss against a teacher (adder_distill_*)
  */
 #ifndef ADDERNET_HIP_H
 #define ADDERNET_HIP_H
@@ -564,6 +565,80 @@ ADDER_API int adder_adamw_step_8bit(int count, void *const *params, const void *
 ADDER_API int adder_adamw_advance(float *step_device, double beta1, double beta2, float *corrections, void *stream);
 ADDER_API int adder_state_values(const void *codes, int is_signed, const float *scales, void *values, long n, int type,
                                  void *stream);
+
+/* RMS norm of rows of `width` values with the addition in front of it: s = x + residual (residual nullable), rstd = 1 / sqrt(mean(s^2) + eps),
+ * y = s rstd weight (weight nullable, stored as weight_type says: type, or float32 beside bfloat16 rows).  y is taken from s before that is rounded.
+ *   adder_rms_norm_fwd: sum (nullable): s.  save_rstd (rows, nullable): what the backward needs beside s.
+ *   adder_rms_norm_fwd_codes: y as codes of 8 bits (below) with their scales.
+ *   adder_rms_norm_bwd: x is s (the forward's x where there was no residual); dsum (nullable): the gradient of s beside dy's.
+ *     gx = dsum + rstd (g - h mean(g h)) with g = dy weight and h = s rstd: the gradient of x and of the residual; gweight = sum over
+ *     rows of dy h.  Each nullable; the workspace is needed for gweight. */
+ADDER_API int adder_rms_norm_fwd(const void *x, long x_row_stride, const void *residual, long residual_row_stride, const void *weight, void *sum,
+                                 void *y, float *save_rstd, float eps, long rows, int width, int type, int weight_type, void *stream);
+ADDER_API int adder_rms_norm_fwd_codes(const void *x, long x_row_stride, const void *residual, long residual_row_stride, const void *weight, void *sum,
+                                       unsigned char *codes, float *scales, float eps, long rows, int width, int type, int weight_type, void *stream);
+ADDER_API int adder_rms_norm_bwd_workspace_bytes(long rows, int width, int type, size_t *bytes);
+ADDER_API int adder_rms_norm_bwd(const void *dy, long dy_row_stride, const void *dsum, long dsum_row_stride, const void *x, long x_row_stride,
+                                 const void *weight, const float *save_rstd, void *gx, void *gweight, long rows, int width, int type, int weight_type,
+                                 void *ws, size_t ws_bytes, void *stream);
+
+/* Codes of 8 bits: OCP e4m3 (four bits of exponent, three of mantissa, largest 448, no infinities).  ADDER_CODE_BLOCK neighbouring values of a row share a
+ * scale (a weight's: ADDER_CODE_BLOCK x ADDER_CODE_BLOCK of its values do):
+ *     top = max(largest magnitude among them, 2^-100),   scale = top / 448,   code = e4m3(v 448 / top), to nearest even
+ * and a code stands for code * scale.  A value that is not a number has a code that is none; a block with an infinite one is not a number as a whole.
+ *   adder_quantize: rows of `width` values; codes (rows, width), scales (rows, ceil(width / ADDER_CODE_BLOCK)).  act >= 0 (adder_act): the input has rows
+ *     of 2 width values, and act(first half) * second half is what becomes codes.
+ *   adder_quantize_weight: codes (rows, width), scales (ceil(rows / ADDER_CODE_BLOCK), ceil(width / ADDER_CODE_BLOCK)).
+ *   adder_linear_codes: y = act(x w' + bias) + residual of such codes, x (rows, in_features) with x_scales as adder_quantize gives them, w (out_features,
+ *     in_features) with w_scales as adder_quantize_weight does; bias, residual and y of `type`.  Row strides in codes.  Sums in 32 bits.
+ *     The workspace's size depends on whether bases and row strides of x and w are multiples of 16 (the others are copied into it first).
+ *   adder_linear_codes_kernel: which kernel it takes: 10000 x (1 for few rows, 2 streamed) + 100 x its shape + the shares of k, as
+ *     adder_linear_kernel says. */
+#define ADDER_CODE_BLOCK 128
+ADDER_API int adder_quantize(const void *x, long x_row_stride, int act, unsigned char *codes, float *scales, long rows, int width, int type, void *stream);
+ADDER_API int adder_quantize_weight(const void *w, long w_row_stride, unsigned char *codes, float *scales, long rows, int width, int type, void *stream);
+ADDER_API int adder_linear_codes_workspace_bytes(long rows, int in_features, int out_features, int x_aligned, int w_aligned, size_t *bytes);
+ADDER_API int adder_linear_codes(const unsigned char *x, long x_row_stride, const float *x_scales, const unsigned char *w, long w_row_stride,
+                                 const float *w_scales, const void *bias, const void *residual, long residual_row_stride, void *y, int act, long rows,
+                                 int in_features, int out_features, int type, void *ws, size_t ws_bytes, void *stream);
+ADDER_API int adder_linear_codes_kernel(long rows, int in_features, int out_features, int *kernel);
+
+/* Gated linear layer: g = x wg' + bg, u = x wu' + bu, y = act(g) u; w (2 hidden, in_features) dense: wg, then wu; bias (2 hidden) likewise, nullable;
+ * y (rows, hidden).
+ *   adder_gated_fwd: pre (nullable): receives what the backward needs of g and u, rows x 2 hidden values of the type's size.  In bfloat16 that is
+ *     not g and u themselves but a form of 16 bits of its own with their range and, mostly, three bits more.
+ *   adder_gated_bwd: dg = dy u act'(g), du = dy act(g); gx = [dg du] w, gw = [dg du]' x, gbias the sums of [dg du] over the rows; each nullable.
+ *     x is read only for gw, w only for gx.  bfloat16: dg and du are rounded to bfloat16 for the two products, and not for gbias.
+ *   adder_gated_kernel: as adder_linear_kernel, of the forward's product. */
+ADDER_API int adder_gated_fwd_workspace_bytes(long rows, int in_features, int hidden, int type, size_t *bytes);
+ADDER_API int adder_gated_fwd(const void *x, long x_row_stride, const void *w, const void *bias, void *y, void *pre, int act, long rows, int in_features,
+                              int hidden, int type, void *ws, size_t ws_bytes, void *stream);
+ADDER_API int adder_gated_bwd_workspace_bytes(long rows, int in_features, int hidden, int type, size_t *bytes);
+ADDER_API int adder_gated_bwd(const void *dy, long dy_row_stride, const void *pre, const void *x, long x_row_stride, const void *w, void *gx, void *gw,
+                              void *gbias, int act, long rows, int in_features, int hidden, int type, void *ws, size_t ws_bytes, void *stream);
+ADDER_API int adder_gated_kernel(long rows, int in_features, int hidden, int type, int aligned, int outputs, int *kernel);
+
+/* The loss of logits l (rows, classes) against a teacher's K largest logits t (rows, K; dense, float32 or bfloat16 as top_type says) at the classes i
+ * (rows, K; dense) and the labels y (rows; nullable), and its gradient:
+ *     q = softmax(l / T),  o = softmax(l),  p = softmax(t / T) over the K
+ *     row = a T^2 sum_k p_k (log p_k - log q[i_k]) - (1 - a) log o[y],   loss = sum of the rows that count / their number
+ * Rows with y == ignore do not count; where none does the loss is zero.  Without labels a is 1.  A teacher's logit of -infinity has p = 0 and adds
+ * nothing; where all K are, the row has no teacher's part.  A class may be among the K more than once.  A class that does not exist, or a
+ * teacher's logit that is not a number, makes the row's loss and gradient not a number.  K at most ADDER_DISTILL_TOP_MAX.
+ *   adder_distill_fwd: stats: ADDER_DISTILL_STATS (rows + 1) floats for the backward.  grad (rows, classes; nullable, and null where
+ *     adder_distill_in_rows answers 0): the gradient for a grad_loss of one, written on the way.
+ *   adder_distill_bwd: the gradient for grad_loss[0], one float in device memory.  unit: grad already holds the one for a grad_loss of one, and
+ *     nothing is done where that is what grad_loss is. */
+#define ADDER_DISTILL_TOP_MAX 1024
+#define ADDER_DISTILL_STATS 8
+ADDER_API int adder_distill_in_rows(long rows, int classes, int type);
+ADDER_API int adder_distill_workspace_bytes(long rows, int classes, int type, size_t *bytes);
+ADDER_API int adder_distill_fwd(const void *logits, long logits_row_stride, const void *top, const long long *classes_of_top, const long long *labels,
+                                float *loss, float *stats, void *grad, float temperature, float alpha, long long ignore, long rows, int classes, int K,
+                                int type, int top_type, void *ws, size_t ws_bytes, void *stream);
+ADDER_API int adder_distill_bwd(const void *logits, long logits_row_stride, const void *top, const long long *classes_of_top, const long long *labels,
+                                const float *stats, const float *grad_loss, int unit, void *grad, float temperature, float alpha, long long ignore,
+                                long rows, int classes, int K, int type, int top_type, void *stream);
 
 #ifdef __cplusplus
 }
