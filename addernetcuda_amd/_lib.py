@@ -93,9 +93,9 @@ _SIGNATURES = {
     "adder_rms_norm_bwd": (_i, [_p, _l, _p, _l, _p, _l, _p, _p, _p, _p, _l, _i, _i, _i, _p, _sz, _p]),
     "adder_quantize": (_i, [_p, _l, _i, _p, _p, _l, _i, _i, _p]),
     "adder_quantize_weight": (_i, [_p, _l, _p, _p, _l, _i, _i, _p]),
-    "adder_linear_codes_workspace_bytes": (_i, [_l, _i, _i, _i, _i, _szp]),
+    "adder_linear_codes_workspace_bytes": (_i, [_l, _i, _i, _i, _i, _i, _szp]),
     "adder_linear_codes": (_i, [_p, _l, _p, _p, _l, _p, _p, _p, _l, _p, _i, _l, _i, _i, _i, _p, _sz, _p]),
-    "adder_linear_codes_kernel": (_i, [_l, _i, _i, ctypes.POINTER(ctypes.c_int)]),
+    "adder_linear_codes_kernel": (_i, [_l, _i, _i, _i, ctypes.POINTER(ctypes.c_int)]),
     "adder_gated_fwd_workspace_bytes": (_i, [_l, _i, _i, _i, _szp]),
     "adder_gated_fwd": (_i, [_p, _l, _p, _p, _p, _p, _i, _l, _i, _i, _i, _p, _sz, _p]),
     "adder_gated_bwd_workspace_bytes": (_i, [_l, _i, _i, _i, _szp]),

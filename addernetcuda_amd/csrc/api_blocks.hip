@@ -27,6 +27,11 @@ static int rms_norm(const void *x, long x_row_stride, const void *residual, long
     return weight_type == ADDER_TYPE_F32 ? launch_rms_norm_fwd<bf16_t, float>(p, s) : launch_rms_norm_fwd<bf16_t, bf16_t>(p, s);
 }
 
+static size_t codes_bytes(long rows, int in, int out, int type, bool x_aligned, bool w_aligned) {
+    return type == ADDER_TYPE_BF16 ? codes_product_workspace_bytes<bf16_t>(rows, out, in, x_aligned, w_aligned)
+                                   : codes_product_workspace_bytes<float>(rows, out, in, x_aligned, w_aligned);
+}
+
 static int check_gated(long rows, int in, int hidden, int type) {
     if (rows <= 0 || in <= 0 || hidden <= 0 || !known(type)) return ADDER_ERR_BAD_SHAPE;
     if (hidden > kMaxWidth / 2 - 16) return ADDER_ERR_TOO_LARGE;
@@ -133,10 +138,10 @@ int adder_quantize_weight(const void *w, long w_row_stride, unsigned char *codes
                                    : launch_quantize_weight(static_cast<const float *>(w), w_row_stride, codes, scales, rows, width, s);
 }
 
-int adder_linear_codes_workspace_bytes(long rows, int in_features, int out_features, int x_aligned, int w_aligned, size_t *bytes) {
+int adder_linear_codes_workspace_bytes(long rows, int in_features, int out_features, int type, int x_aligned, int w_aligned, size_t *bytes) {
     if (!bytes) return ADDER_ERR_NULL_POINTER;
-    if (int rc = check_linear(rows, in_features, out_features, ADDER_TYPE_BF16)) return rc;
-    *bytes = whole(codes_product_workspace_bytes(rows, out_features, in_features, x_aligned != 0, w_aligned != 0));
+    if (int rc = check_linear(rows, in_features, out_features, type)) return rc;
+    *bytes = whole(codes_bytes(rows, in_features, out_features, type, x_aligned != 0, w_aligned != 0));
     return ADDER_OK;
 }
 
@@ -153,7 +158,7 @@ int adder_linear_codes(const unsigned char *x, long x_row_stride, const float *x
         in_features >= (1 << 23) || (residual && wide(rows, residual_row_stride)))
         return ADDER_ERR_TOO_LARGE;
     const auto aligned = [](const void *p, long ld) { return !((reinterpret_cast<uintptr_t>(p) | (uintptr_t)ld) & 15); };
-    const size_t need = codes_product_workspace_bytes(rows, out_features, in_features, aligned(x, x_row_stride), aligned(w, w_row_stride));
+    const size_t need = codes_bytes(rows, in_features, out_features, type, aligned(x, x_row_stride), aligned(w, w_row_stride));
     if (int rc = check_workspace(ws, ws_bytes, need)) return rc;
     const size_t blocks = blocks_of(in_features), e = size_of(type);
     const Span outs[] = {{y, e * (size_t)rows * out_features}, {ws, need}};
@@ -167,17 +172,17 @@ int adder_linear_codes(const unsigned char *x, long x_row_stride, const float *x
     return type == ADDER_TYPE_BF16 ? launch_codes_product<bf16_t>(p, ws, s) : launch_codes_product<float>(p, ws, s);
 }
 
-int adder_linear_codes_kernel(long rows, int in_features, int out_features, int *kernel) {
+int adder_linear_codes_kernel(long rows, int in_features, int out_features, int type, int *kernel) {
     if (!kernel) return ADDER_ERR_NULL_POINTER;
-    if (int rc = check_linear(rows, in_features, out_features, ADDER_TYPE_BF16)) return rc;
-    *kernel = codes_product_kernel(rows, out_features, in_features);
+    if (int rc = check_linear(rows, in_features, out_features, type)) return rc;
+    *kernel = type == ADDER_TYPE_BF16 ? codes_product_kernel<bf16_t>(rows, out_features, in_features) : codes_product_kernel<float>(rows, out_features, in_features);
     return ADDER_OK;
 }
 
 int adder_gated_fwd_workspace_bytes(long rows, int in_features, int hidden, int type, size_t *bytes) {
     if (!bytes) return ADDER_ERR_NULL_POINTER;
     if (int rc = check_gated(rows, in_features, hidden, type)) return rc;
-    *bytes = whole(product_bytes(rows, gated_columns(hidden), in_features, type));
+    *bytes = whole(product_bytes(rows, gated_columns(hidden), in_features, type, true));
     return ADDER_OK;
 }
 
@@ -187,7 +192,7 @@ int adder_gated_fwd(const void *x, long x_row_stride, const void *w, const void 
     if (int rc = check_gated(rows, in_features, hidden, type)) return rc;
     if (!known_act(act) || bad_stride(x_row_stride, rows, in_features)) return ADDER_ERR_BAD_SHAPE;
     if (wide(rows, x_row_stride)) return ADDER_ERR_TOO_LARGE;
-    const size_t need = product_bytes(rows, gated_columns(hidden), in_features, type), e = size_of(type), ny = e * (size_t)rows * hidden;
+    const size_t need = product_bytes(rows, gated_columns(hidden), in_features, type, true), e = size_of(type), ny = e * (size_t)rows * hidden;
     if (int rc = check_workspace(ws, ws_bytes, need)) return rc;
     const Span outs[] = {{y, ny}, {pre, 2 * ny}, {ws, need}};
     const Span ins[] = {{x, span(rows, x_row_stride, in_features, type)}, {w, e * 2 * (size_t)hidden * in_features}, {bias, e * 2 * (size_t)hidden}};
@@ -249,7 +254,7 @@ int adder_gated_kernel(long rows, int in_features, int hidden, int type, int ali
     if (int rc = check_gated(rows, in_features, hidden, type)) return rc;
     if (outputs < 1 || outputs > 2) return ADDER_ERR_BAD_SHAPE;
     const auto of = type == ADDER_TYPE_BF16 ? product_kernel<bf16_t> : product_kernel<float>;
-    *kernel = of(rows, gated_columns(hidden), in_features, false, false, aligned != 0, outputs);
+    *kernel = of(rows, gated_columns(hidden), in_features, false, false, aligned != 0, outputs, true);
     return ADDER_OK;
 }
 

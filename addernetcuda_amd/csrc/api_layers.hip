@@ -138,7 +138,7 @@ int adder_linear_kernel(long rows, int in_features, int out_features, int produc
     if (product < 0 || product > 2 || outputs < 1 || outputs > (product ? 1 : 2)) return ADDER_ERR_BAD_SHAPE;
     const long M = product == 2 ? out_features : rows, N = product ? in_features : out_features, K = product == 0 ? in_features : product == 1 ? out_features : rows;
     const auto of = type == ADDER_TYPE_BF16 ? product_kernel<bf16_t> : product_kernel<float>;
-    *kernel = of(M, N, K, product == 2, product != 0, aligned != 0, outputs);
+    *kernel = of(M, N, K, product == 2, product != 0, aligned != 0, outputs, false);
     return ADDER_OK;
 }
 

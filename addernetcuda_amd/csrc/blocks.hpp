@@ -84,7 +84,10 @@ struct CodesProduct {
     void *out;
     Act act;
 };
+// T: type of the result
+template <class T>
 int codes_product_kernel(long M, long N, long K);   // as adder_linear_codes_kernel numbers them
+template <class T>
 size_t codes_product_workspace_bytes(long M, long N, long K, bool x_aligned, bool w_aligned);
 template <class T>
 int launch_codes_product(const CodesProduct &p, void *ws, hipStream_t s);

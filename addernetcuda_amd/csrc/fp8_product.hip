@@ -132,22 +132,31 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void codes_stream_kernel(const Code
             }
             return join(lo, hi);
         };
+        Operand<T> fa[2];
+        f32x4 t[2][TN];
+        const auto add = [&](int i, int j) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(t[i & 1][j][e], s[i], acc[i][j][e]);
+        };
 #pragma unroll
         for (int j = 0; j < TN; ++j) fb[j].set(fragment(tb, wn + j * 16));
+        fa[0].set(fragment(ta, wm));
 #pragma unroll
         for (int i = 0; i < TM; ++i) s[i] = xs[i * 16] * by;
+        // A row of tiles is multiplied while the one before it is scaled and the next one's operand is read, in this order
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
-            Operand<T> fa;
-            fa.set(fragment(ta, wm + i * 16));
-            f32x4 t[TN];
+            if (i + 1 < TM) fa[(i + 1) & 1].set(fragment(ta, wm + (i + 1) * 16));
 #pragma unroll
-            for (int j = 0; j < TN; ++j) t[j] = block_sums(fb[j], fa);
-#pragma unroll
-            for (int j = 0; j < TN; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(t[j][e], s[i], acc[i][j][e]);
+            for (int j = 0; j < TN; ++j) {
+                __builtin_amdgcn_sched_barrier(0);
+                t[i & 1][j] = block_sums(fb[j], fa[i & 1]);
+                if (i > 0) add(i - 1, j);
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
+#pragma unroll
+        for (int j = 0; j < TN; ++j) add(TM - 1, j);
     };
     const int full = (int)((k_end - k_begin) / kCodeBlock);
     for (int s = 0; s < full; ++s) {
@@ -177,8 +186,7 @@ static int launch_stream(CodesArgs p, hipStream_t s) {
 // ---- few rows of x: the time is that of reading w -------------------------------------------------------------------------
 // As the other layers' (linear_rows.hip): sixteen rows of w and up to 16 MT rows of x a workgroup, whose waves take turns along the blocks
 // of k, straight from memory, and add their sums through LDS.  Any strides and alignment.
-template <int MT>
-static constexpr int kCodesWaves = MT == 4 ? 8 : 16;
+static constexpr int kCodesWaves = 8;
 typedef int i32x4_any __attribute__((ext_vector_type(4), aligned(1)));
 __device__ __forceinline__ i32x4 load_codes(const uint8_t *p) { return *reinterpret_cast<const i32x4_any *>(p); }
 __device__ __forceinline__ i32x4 load_codes_part(const uint8_t *p, long valid) {
@@ -191,7 +199,7 @@ __device__ __forceinline__ i32x4 load_codes_part(const uint8_t *p, long valid) {
 }
 
 template <class T, int MT>
-__global__ __launch_bounds__(kCodesWaves<MT> * 64) void codes_rows_kernel(const CodesArgs p) {
+__global__ __launch_bounds__(kCodesWaves * 64) void codes_rows_kernel(const CodesArgs p) {
     constexpr int U = MT == 1 ? 2 : 1;   // blocks that a wave multiplies while as many arrive
     extern __shared__ __align__(16) char lds[];
     f32x4 *sums = reinterpret_cast<f32x4 *>(lds);
@@ -280,44 +288,71 @@ __global__ __launch_bounds__(kCodesWaves<MT> * 64) void codes_rows_kernel(const 
 
 template <class T, int MT>
 static int launch_rows(const CodesArgs &p, hipStream_t s) {
-    const int waves = p.blocks < kCodesWaves<MT> ? p.blocks : kCodesWaves<MT>;
+    const int waves = p.blocks < kCodesWaves ? p.blocks : kCodesWaves;
     hipLaunchKernelGGL((codes_rows_kernel<T, MT>), dim3((unsigned)ceil_div_l(p.N, 16), (unsigned)ceil_div_l(p.M, 16 * MT)), dim3(waves * 64),
                        waves * MT * 1024, s, p);
     return check_launch();
 }
 
-// ---- operands whose rows are not 16 aligned bytes: a copy that is -------------------------------------------------------------
-__global__ __launch_bounds__(256) void align_codes_kernel(const uint8_t *__restrict__ from, long ld, uint4 *__restrict__ to, long rows, int K, int chunks) {
-    const long all = rows * chunks;
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < all; i += (long)gridDim.x * 256) {
-        const long row = i / chunks;
-        const int at = (int)(i - row * chunks) * 16;
-        const i32x4 u = load_codes_part(from + row * ld + at, K - at);
-        to[i] = make_uint4((uint32_t)u[0], (uint32_t)u[1], (uint32_t)u[2], (uint32_t)u[3]);
+// ---- operands whose rows are not 16 aligned bytes: copies that are, one or both in a launch ------------------------------------
+struct AlignArgs {
+    const uint8_t *from[2];
+    uint4 *to[2];
+    long ld[2], chunks_of[2];   // chunks_of: all of an operand's, none where it is aligned
+    int K, chunks;              // chunks: a row's
+};
+__global__ __launch_bounds__(256) void align_codes_kernel(const AlignArgs p) {
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < p.chunks_of[0] + p.chunks_of[1]; i += (long)gridDim.x * 256) {
+        const int o = i >= p.chunks_of[0];
+        const long c = o ? i - p.chunks_of[0] : i, row = c / p.chunks;
+        const int at = (int)(c - row * p.chunks) * 16;
+        const i32x4 u = load_codes_part((o ? p.from[1] : p.from[0]) + row * (o ? p.ld[1] : p.ld[0]) + at, p.K - at);
+        (o ? p.to[1] : p.to[0])[c] = make_uint4((uint32_t)u[0], (uint32_t)u[1], (uint32_t)u[2], (uint32_t)u[3]);
     }
 }
 static long padded(long K) { return (K + 15) & ~15L; }
 static size_t copy_bytes(long rows, long K) { return ((size_t)rows * padded(K) + 255) & ~(size_t)255; }
 
 // ---- which kernel ---------------------------------------------------------------------------------------------------------------
-static constexpr Shape kCodesShapes[] = {
-    {256, 256, 1, 1.55f, 1.55f, 10.f},
-    {128, 128, 2, 0.87f, 0.65f, 3.5f},
-    {64, 64, 2, 0.38f, 0.2f, 1.5f},
+// (the estimate: product.hpp; a step is a block of 128 values of k.  Measured as 8192 x 4096 -> 4096, 8192 x 1024 -> 8192 and, alone, as 64 and 128
+// workgroups.  256 x 256 results of float32 would not fit the registers beside their operands.)
+template <class T>
+static constexpr Shape kCodesShapes[] = {   // 8192 x 4096 -> 4096, TFLOP/s
+    {128, 128, 2, 2.f, 1.1f, 4.f},          //  886
+    {64, 64, 2, 0.755f, 0.5f, 1.9f},        //  653
 };
-// Up to 64 rows take the kernel for few
-static constexpr long kCodesRows = 64;
-static ProductPlan plan_codes(long M, long N, long K) { return plan_product(kCodesShapes, kCodeBlock, M, N, K, 1); }
+template <>
+constexpr Shape kCodesShapes<bf16_t>[] = {
+    {128, 128, 2, 1.3f, 0.655f, 3.25f},     // 1501
+    {64, 64, 2, 0.6f, 0.33f, 1.6f},         //  817
+    {256, 256, 1, 2.07f, 2.07f, 5.9f},      // 1864
+};
+// The kernel for few rows likewise: workgroups of 16 columns whose waves take turns along the blocks of k (us each, measured at 4096 x 4096 and
+// 8192 x 8192).  With 33 to 64 rows it was behind the small tiles (64 x 4096 -> 4096 in 16.5 us instead of 11.4).
+static constexpr long kCodesRowsMost = 32;
+static float codes_rows_us(long M, long N, long K) {
+    const float groups = (float)ceil_div_l(N, 16), turns = (float)ceil_div_l(ceil_div_l(K, kCodeBlock), kCodesWaves);
+    return 3.f + ceilf(groups / kCUs) * (0.4f + turns * (M <= 16 ? 1.1f : 1.75f));
+}
+// The one choice that a launch and the queries make; shape -1: the kernel for few rows
+template <class T>
+static ProductPlan plan_codes(long M, long N, long K) {
+    const ProductPlan plan = plan_product(kCodesShapes<T>, kCodeBlock, M, N, K, 1);
+    return M <= kCodesRowsMost && codes_rows_us(M, N, K) < plan.us ? ProductPlan{-1, 1, K, 0.f} : plan;
+}
 static size_t split_bytes(const ProductPlan &plan, long M, long N) { return plan.splits > 1 ? (sizeof(float) * (size_t)plan.splits * M * N + 255) & ~(size_t)255 : 0; }
 
+template <class T>
 size_t codes_product_workspace_bytes(long M, long N, long K, bool x_aligned, bool w_aligned) {
-    if (M <= kCodesRows) return 0;
-    return split_bytes(plan_codes(M, N, K), M, N) + (x_aligned ? 0 : copy_bytes(M, K)) + (w_aligned ? 0 : copy_bytes(N, K));
+    const ProductPlan plan = plan_codes<T>(M, N, K);
+    if (plan.shape < 0) return 0;
+    return split_bytes(plan, M, N) + (x_aligned ? 0 : copy_bytes(M, K)) + (w_aligned ? 0 : copy_bytes(N, K));
 }
 
+template <class T>
 int codes_product_kernel(long M, long N, long K) {
-    if (M <= kCodesRows) return 10000 + 100 * (M <= 16 ? 1 : M <= 32 ? 2 : 4) + 1;
-    const ProductPlan plan = plan_codes(M, N, K);
+    const ProductPlan plan = plan_codes<T>(M, N, K);
+    if (plan.shape < 0) return 10000 + 100 * (M <= 16 ? 1 : 2) + 1;
     return 20000 + 100 * plan.shape + plan.splits;
 }
 
@@ -331,31 +366,43 @@ int launch_codes_product(const CodesProduct &q, void *ws, hipStream_t s) {
     p.act = q.act;
     p.xs = q.xs; p.ws = q.ws;
     p.blocks = (int)ceil_div_l(q.K, kCodeBlock);
-    if (q.M <= kCodesRows) return q.M <= 16 ? launch_rows<T, 1>(p, s) : q.M <= 32 ? launch_rows<T, 2>(p, s) : launch_rows<T, 4>(p, s);
-    const ProductPlan plan = plan_codes(q.M, q.N, q.K);
+    const ProductPlan plan = plan_codes<T>(q.M, q.N, q.K);
+    if (plan.shape < 0) return q.M <= 16 ? launch_rows<T, 1>(p, s) : launch_rows<T, 2>(p, s);
     char *at = static_cast<char *>(ws);
     p.part = reinterpret_cast<float *>(at);
     at += split_bytes(plan, q.M, q.N);
     p.splits = plan.splits;
     p.k_share = plan.k_share;
-    const auto align = [&](const void *&from, long &ld, long rows) -> int {
-        if (!((reinterpret_cast<uintptr_t>(from) | (uintptr_t)ld) & 15)) return ADDER_OK;
-        const int chunks = (int)(padded(q.K) / 16);
-        const long groups = ceil_div_l(rows * chunks, 256);
-        hipLaunchKernelGGL(align_codes_kernel, dim3((unsigned)(groups < 16384 ? groups : 16384)), dim3(256), 0, s, static_cast<const uint8_t *>(from), ld,
-                           reinterpret_cast<uint4 *>(at), rows, (int)q.K, chunks);
+    AlignArgs g{{}, {}, {}, {}, (int)q.K, (int)(padded(q.K) / 16)};
+    const auto align = [&](int i, const void *&from, long &ld, long rows) {
+        if (!((reinterpret_cast<uintptr_t>(from) | (uintptr_t)ld) & 15)) return;
+        g.from[i] = static_cast<const uint8_t *>(from);
+        g.ld[i] = ld;
+        g.to[i] = reinterpret_cast<uint4 *>(at);
+        g.chunks_of[i] = rows * g.chunks;
         from = at;
         ld = padded(q.K);
         at += copy_bytes(rows, q.K);
-        return check_launch();
     };
-    if (int rc = align(p.a, p.lda, q.M)) return rc;
-    if (int rc = align(p.b, p.ldb, q.N)) return rc;
-    const int rc = plan.shape == 0 ? launch_stream<T, 2, 4, 8, 4, 2>(p, s) : plan.shape == 1 ? launch_stream<T, 2, 2, 4, 4, 2>(p, s) : launch_stream<T, 2, 2, 2, 2, 4>(p, s);
+    align(0, p.a, p.lda, q.M);
+    align(1, p.b, p.ldb, q.N);
+    if (const long all = g.chunks_of[0] + g.chunks_of[1]) {
+        const long groups = ceil_div_l(all, 256);
+        hipLaunchKernelGGL(align_codes_kernel, dim3((unsigned)(groups < 16384 ? groups : 16384)), dim3(256), 0, s, g);
+        if (int rc = check_launch()) return rc;
+    }
+    int rc = ADDER_ERR_UNSUPPORTED;
+    if (plan.shape == 0) rc = launch_stream<T, 2, 2, 4, 4, 2>(p, s);
+    else if (plan.shape == 1) rc = launch_stream<T, 2, 2, 2, 2, 4>(p, s);
+    else if constexpr (sizeof(T) == 2) rc = launch_stream<T, 2, 4, 8, 4, 2>(p, s);
     if (rc || plan.splits == 1) return rc;
     return launch_product_join<T>(p, s);
 }
-template int launch_codes_product<float>(const CodesProduct &, void *, hipStream_t);
-template int launch_codes_product<bf16_t>(const CodesProduct &, void *, hipStream_t);
+#define ADDER_CODES_PRODUCT_INSTANCE(T)                                                     \
+    template size_t codes_product_workspace_bytes<T>(long, long, long, bool, bool);          \
+    template int codes_product_kernel<T>(long, long, long);                                  \
+    template int launch_codes_product<T>(const CodesProduct &, void *, hipStream_t);
+ADDER_CODES_PRODUCT_INSTANCE(float)
+ADDER_CODES_PRODUCT_INSTANCE(bf16_t)
 
 }  // namespace adder

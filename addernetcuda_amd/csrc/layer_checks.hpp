@@ -29,8 +29,8 @@ static int check_linear(long rows, int in, int out, int type) {
 }
 static bool known_act(int act) { return act >= ADDER_ACT_NONE && act <= ADDER_ACT_SILU; }
 
-static size_t product_bytes(long M, long N, long K, int type) {
-    return type == ADDER_TYPE_BF16 ? product_workspace_bytes<bf16_t>(M, N, K) : product_workspace_bytes<float>(M, N, K);
+static size_t product_bytes(long M, long N, long K, int type, bool gated = false) {
+    return type == ADDER_TYPE_BF16 ? product_workspace_bytes<bf16_t>(M, N, K, gated) : product_workspace_bytes<float>(M, N, K, gated);
 }
 static int product(const Product &p, int type, void *ws, hipStream_t s) {
     return type == ADDER_TYPE_BF16 ? launch_product<bf16_t>(p, ws, s) : launch_product<float>(p, ws, s);

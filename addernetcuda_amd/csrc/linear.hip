@@ -66,6 +66,13 @@ static constexpr Shape kStreamShapes[] = {
     {128, 128, 2, 0.87f, 0.65f, 3.5f},   // 1177
     {64, 64, 2, 0.38f, 0.2f, 1.5f},      //  719
 };
+// Gated layers, whose results are half as many columns (8192 x 1024 -> 4096 with what the backward needs: 151, 182, 174, 287 us)
+static constexpr Shape kGatedShapes[] = {
+    {256, 256, 1, 1.55f, 1.55f, 6.1f},
+    {128, 256, 1, 0.9f, 0.9f, 3.f},
+    {128, 128, 2, 0.87f, 0.65f, 3.75f},
+    {64, 64, 2, 0.38f, 0.2f, 1.5f},
+};
 template <class T>
 static constexpr Shape kStagedShapes[] = {
     {128, 128, 2, 1.f, 0.6f, 3.5f},      // 1033
@@ -92,7 +99,7 @@ static float rows_us(long M, long N, long K) {
 
 template <class T>
 static ProductPlan plan_staged(long M, long N, long K, int outputs) { return plan_product(kStagedShapes<T>, sizeof(T) == 4 ? 32 : 64, M, N, K, outputs); }
-static ProductPlan plan_stream(long M, long N, long K, int outputs) { return plan_product(kStreamShapes, 64, M, N, K, outputs); }
+static ProductPlan plan_stream(long M, long N, long K, int outputs, bool gated) { return plan_product(gated ? kGatedShapes : kStreamShapes, 64, M, N, K, outputs); }
 
 // Loads of 16 aligned bytes fit a bfloat16 operand: base and rows begin at multiples of them, and what a tile's last load brings
 // beside the operand it can be told from by k alone (k along: rows of whole loads) or is never stored (k across).  A tile's rows
@@ -103,10 +110,10 @@ static bool fits_stream(bool across, long K) { return across || !(K & 7); }
 static size_t split_bytes(const ProductPlan &p, long M, long N) { return p.splits > 1 ? sizeof(float) * (size_t)p.splits * M * N : 0; }
 
 template <class T>
-size_t product_workspace_bytes(long M, long N, long K) {
+size_t product_workspace_bytes(long M, long N, long K, bool gated) {
     size_t most = 0;   // whichever kernel strides and alignments leave, with and without a second output
     for (int outputs = 1; outputs <= 2; ++outputs) {
-        const size_t staged = split_bytes(plan_staged<T>(M, N, K, outputs), M, N), stream = sizeof(T) == 2 ? split_bytes(plan_stream(M, N, K, outputs), M, N) : 0;
+        const size_t staged = split_bytes(plan_staged<T>(M, N, K, outputs), M, N), stream = sizeof(T) == 2 ? split_bytes(plan_stream(M, N, K, outputs, gated), M, N) : 0;
         if (staged > most) most = staged;
         if (stream > most) most = stream;
     }
@@ -117,22 +124,22 @@ size_t product_workspace_bytes(long M, long N, long K) {
 enum class Family { rows = 1, stream, staged };
 struct Choice { Family family; ProductPlan plan; };
 template <class T>
-static Choice choose_product(long M, long N, long K, bool a_across, bool b_across, bool aligned, int outputs) {
+static Choice choose_product(long M, long N, long K, bool a_across, bool b_across, bool aligned, int outputs, bool gated) {
     const bool stream = sizeof(T) == 2 && aligned && fits_stream(a_across, K) && fits_stream(b_across, K);
-    const ProductPlan plan = stream ? plan_stream(M, N, K, outputs) : plan_staged<T>(M, N, K, outputs);
+    const ProductPlan plan = stream ? plan_stream(M, N, K, outputs, gated) : plan_staged<T>(M, N, K, outputs);
     if (!a_across && !b_across && M <= kRowsMost && N <= kRowsColumns && rows_us<T>(M, N, K) < plan.us) return {Family::rows, ProductPlan{0, 1, K, 0.f}};
     return {stream ? Family::stream : Family::staged, plan};
 }
 template <class T>
-int product_kernel(long M, long N, long K, bool a_across, bool b_across, bool aligned, int outputs) {
-    const Choice c = choose_product<T>(M, N, K, a_across, b_across, aligned, outputs);
+int product_kernel(long M, long N, long K, bool a_across, bool b_across, bool aligned, int outputs, bool gated) {
+    const Choice c = choose_product<T>(M, N, K, a_across, b_across, aligned, outputs, gated);
     return static_cast<int>(c.family) * 10000 + (c.family == Family::rows ? product_rows_tiles(M) : c.plan.shape) * 100 + c.plan.splits;
 }
 
 template <class T>
 int launch_product(const Product &q, void *ws, hipStream_t s) {
     const bool aligned = aligned16(q.a, q.lda) && aligned16(q.b, q.ldb) && (!q.half || (q.half + 256) * q.ldb < (1L << 31));   // (gated: a tile's rows are half the weight apart)
-    const Choice c = choose_product<T>(q.M, q.N, q.K, q.a_across, q.b_across, aligned, q.pre ? 2 : 1);
+    const Choice c = choose_product<T>(q.M, q.N, q.K, q.a_across, q.b_across, aligned, q.pre ? 2 : 1, q.half != 0);
     const ProductPlan &plan = c.plan;
     const ProductArgs p{q.a, q.b, q.bias, q.res, q.out, q.pre, static_cast<float *>(ws), q.lda, q.ldb, q.ldr, q.M, q.N, q.K, plan.k_share, 0, 0,
                         plan.splits, q.act, q.half};
@@ -210,10 +217,10 @@ int launch_act_bwd(const T *dy, long dy_stride, const T *z, T *dz, float *part, 
 }
 
 #define ADDER_LINEAR_INSTANCE(T)                                                                                      \
-    template size_t product_workspace_bytes<T>(long, long, long);                                                     \
+    template size_t product_workspace_bytes<T>(long, long, long, bool);                                                \
     template int launch_product<T>(const Product &, void *, hipStream_t);                                            \
     template int launch_product_join<T>(const ProductArgs &, hipStream_t);                                            \
-    template int product_kernel<T>(long, long, long, bool, bool, bool, int);                                          \
+    template int product_kernel<T>(long, long, long, bool, bool, bool, int, bool);                                   \
     template int launch_act_bwd<T>(const T *, long, const T *, T *, float *, Act, long, long, hipStream_t);
 ADDER_LINEAR_INSTANCE(float)
 ADDER_LINEAR_INSTANCE(bf16_t)

@@ -256,7 +256,7 @@ PyObject *py_linear_fp8(PyObject *, PyObject *const *args, Py_ssize_t count) {
             if (bias.defined()) bias = bias.contiguous();
             const auto aligned = [](const Rows &t) { return !((reinterpret_cast<uintptr_t>(t.t.data_ptr()) | (uintptr_t)t.stride) & 15); };
             size_t need = 0;
-            check(lib.codes_bytes(a.rows, (int)k, (int)n, aligned(a), aligned(b), &need), "adder_linear_codes_workspace_bytes");
+            check(lib.codes_bytes(a.rows, (int)k, (int)n, type, aligned(a), aligned(b), &need), "adder_linear_codes_workspace_bytes");
             const Tensor space = bytes_for(need, x);
             check(lib.codes(static_cast<const unsigned char *>(a.t.data_ptr()), a.stride, xs.data_ptr<float>(), static_cast<const unsigned char *>(b.t.data_ptr()),
                             b.stride, ws.data_ptr<float>(), ptr(bias), ptr(r.t), r.stride, y.data_ptr(), act, a.rows, (int)k, (int)n, type, ptr(space), need,

@@ -597,11 +597,12 @@ ADDER_API int adder_rms_norm_bwd(const void *dy, long dy_row_stride, const void 
 #define ADDER_CODE_BLOCK 128
 ADDER_API int adder_quantize(const void *x, long x_row_stride, int act, unsigned char *codes, float *scales, long rows, int width, int type, void *stream);
 ADDER_API int adder_quantize_weight(const void *w, long w_row_stride, unsigned char *codes, float *scales, long rows, int width, int type, void *stream);
-ADDER_API int adder_linear_codes_workspace_bytes(long rows, int in_features, int out_features, int x_aligned, int w_aligned, size_t *bytes);
+ADDER_API int adder_linear_codes_workspace_bytes(long rows, int in_features, int out_features, int type, int x_aligned, int w_aligned,
+                                                 size_t *bytes);
 ADDER_API int adder_linear_codes(const unsigned char *x, long x_row_stride, const float *x_scales, const unsigned char *w, long w_row_stride,
                                  const float *w_scales, const void *bias, const void *residual, long residual_row_stride, void *y, int act, long rows,
                                  int in_features, int out_features, int type, void *ws, size_t ws_bytes, void *stream);
-ADDER_API int adder_linear_codes_kernel(long rows, int in_features, int out_features, int *kernel);
+ADDER_API int adder_linear_codes_kernel(long rows, int in_features, int out_features, int type, int *kernel);
 
 /* Gated linear layer: g = x wg' + bg, u = x wu' + bu, y = act(g) u; w (2 hidden, in_features) dense: wg, then wu; bias (2 hidden) likewise, nullable;
  * y (rows, hidden).

@@ -68,11 +68,11 @@ def test_codes_refuse():
     assert lin(rows=1 << 40) == -3 and lin(ldx=1 << 23) == -3 and lin(ldw=1 << 23) == -3 and lin(k=1 << 23, ldx=1 << 23, ldw=1 << 23) == -3
     for bad in ({"y": A[0]}, {"y": A[1]}, {"y": A[2]}, {"y": A[3]}, {"b": A[4]}, {"r": A[4], "ldr": 32}):
         assert lin(**bad) == -6
-    rc, need = size(lib.adder_linear_codes_workspace_bytes, 200, 100, 70, 0, 0)
-    assert rc == 0 and need >= (200 + 70) * 100 and size(lib.adder_linear_codes_workspace_bytes, 200, 112, 70, 1, 1)[1] < need
+    rc, need = size(lib.adder_linear_codes_workspace_bytes, 200, 100, 70, 0, 0, 0)
+    assert rc == 0 and need >= (200 + 70) * 100 and size(lib.adder_linear_codes_workspace_bytes, 200, 112, 70, 0, 1, 1)[1] < need
     for bad in ({"work": None}, {"nb": need - 300}, {"work": P((7 << 36) + 8)}):
         assert lin(rows=200, k=100, ldx=100, ldw=100, n=70, **bad) == -4
-    assert size(lib.adder_linear_codes_workspace_bytes, 0, 1, 1, 0, 0)[0] == -2 and lib.adder_linear_codes_kernel(1, 1, 1, None) == -1
+    assert size(lib.adder_linear_codes_workspace_bytes, 0, 1, 1, 0, 0, 0)[0] == -2 and lib.adder_linear_codes_kernel(1, 1, 1, 0, None) == -1
 
 
 def test_gated_refuses():

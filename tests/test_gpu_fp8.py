@@ -61,7 +61,7 @@ def test_quantize_of_what_is_no_number(gpu):
 
 
 # few rows, tiles' borders, widths that no block and no load divides, shares of k
-SIZES = [(1, 1, 1), (1, 128, 16), (2, 127, 130), (16, 4096, 100), (17, 1000, 33), (33, 96, 300), (64, 2048, 129), (65, 128, 64), (70, 144, 200), (100, 1000, 257), (128, 4096, 128),
+SIZES = [(1, 1, 1), (1, 128, 16), (2, 127, 130), (16, 4096, 100), (17, 1000, 33), (30, 515, 77), (33, 96, 300), (64, 2048, 129), (20, 8192, 8192),  (65, 128, 64), (70, 144, 200), (100, 1000, 257), (128, 4096, 128),
          (130, 16, 1000), (200, 333, 77), (300, 640, 640), (513, 272, 1030), (1100, 528, 2000), (2048, 1024, 1024), (2300, 512, 4200)]
 
 
@@ -76,27 +76,34 @@ def test_products(rows, k, n, dtype, gpu):
     within(linear_fp8(x, xs, w, ws, b, r, act, dtype), B.linear_codes(x, xs, w, ws, b, r, act, dtype), "with everything")
 
 
+# sizes of the large shapes, whose results are looked at in part
+LARGE = [(4096, 1024, 4096), (8200, 300, 4100)]
+
+
 def test_each_kernel_is_reached():
-    """Sizes above take each shape of the kernels, the streamed ones with and without shares of k."""
+    """The sizes take each shape of the kernels, the streamed ones with and without shares of k."""
     import ctypes
     from addernetcuda_amd._lib import lib
-    got = set()
-    for rows, k, n in SIZES + [(4096, 1024, 4096), (8192, 4096, 4096)]:
-        v = ctypes.c_int()
-        assert lib.adder_linear_codes_kernel(rows, k, n, ctypes.byref(v)) == 0
-        got.add((v.value // 100, v.value % 100 > 1))
-    assert {g[0] for g in got} >= {101, 102, 104, 200, 201, 202}, got
+    for dtype in DTYPES:
+        got = set()
+        for rows, k, n in SIZES + LARGE:
+            v = ctypes.c_int()
+            assert lib.adder_linear_codes_kernel(rows, k, n, int(dtype == torch.bfloat16), ctypes.byref(v)) == 0
+            got.add((v.value // 100, v.value % 100 > 1))
+        want = {101, 102, 200, 201} | ({202} if dtype == torch.bfloat16 else set())
+        assert {g[0] for g in got} == want and {(201, True), (201, False), (200, False)} <= got, got
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 def test_large(dtype, gpu):
     from addernetcuda_amd.fp8 import linear_fp8
-    (x, xs), (w, ws) = codes(4096, 1024), weight(4096, 1024)
-    want = B.linear_codes(x[:512], xs[:512], w, ws, None, None, "none", dtype)
-    within(linear_fp8(x, xs, w, ws, dtype=dtype)[:512], want, "product")
-    (x, xs), (w, ws) = codes(8192, 128), weight(8200, 128)
-    got = linear_fp8(x, xs, w, ws, dtype=dtype)
-    within(got[-300:], B.linear_codes(x[-300:], xs[-300:], w, ws, None, None, "none", dtype), "the last rows")
+    for rows, k, n in LARGE:
+        (x, xs), (w, ws) = codes(rows, k), weight(n, k)
+        r = normal(300, n, seed=3).to(dtype).cuda()
+        r = torch.cat([r, r.new_zeros(rows - 600, n), r])
+        got = linear_fp8(x, xs, w, ws, residual=r, dtype=dtype)
+        for at in (slice(0, 300), slice(rows - 300, rows)):
+            within(got[at], B.linear_codes(x[at], xs[at], w, ws, None, r[at], "none", dtype), f"rows {at}")
 
 
 def test_layouts(gpu):
