@@ -131,6 +131,13 @@ class LinearFp8(nn.Module):
         self.register_buffer("weight_scale", torch.ones(-(-out_features // BLOCK), -(-in_features // BLOCK), device=device))
         self.register_buffer("bias", torch.zeros(out_features, device=device) if bias else None)
 
+    def _apply(self, fn, recurse=True):
+        """``to(...)``, ``half()`` and the like move codes and scales and leave their types: a code of another type would be another number."""
+        def moved(t):
+            r = fn(t)
+            return r if r.dtype == t.dtype else t.to(r.device)
+        return super()._apply(moved, recurse)
+
     @classmethod
     @torch.no_grad()
     def of(cls, layer, gate=None):

@@ -42,12 +42,12 @@ def rms_norm(x, w, r, dy, ds, eps):
 
 
 def _kept(z, halves):
-    """What is kept of z for the backward is off by: halves (an ulp of 2^-10, or of 2^-24) where the largest of four neighbouring columns allows it,
+    """What is kept of z for the backward is off by: halves (half an ulp of 2^-10, or of 2^-24, and the last bit of the first of four) where the largest of four neighbouring columns allows it,
     else bfloat16 whose first of four may lose its last bit."""
     n = z.shape[1]
     top = torch.nn.functional.pad(z.abs(), (0, -n % 4)).unflatten(1, (-1, 4)).amax(2).repeat_interleave(4, 1)[:, :n]
     fits = (top > 2.0 ** -11.9) & (top < 65000) & halves
-    return torch.where(fits, 2.0 ** -10 * z.abs() + 2.0 ** -24, 3 * V * z.abs() + 1e-40)
+    return torch.where(fits, 1.5 * 2.0 ** -10 * z.abs() + 2.0 ** -24, 3 * V * z.abs() + 1e-40)
 
 
 def gated_linear(x, w, b, dy, act):

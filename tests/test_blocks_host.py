@@ -176,3 +176,19 @@ def test_distillation_on_the_cpu():
     assert torch.isnan(loss.detach())
     bad = torch.isnan(torch.autograd.grad(loss, l)[0]).all(1)
     assert bad.nonzero().flatten().tolist() == [5, 6]
+
+
+def test_8_bit_layers_keep_their_types():
+    from addernetcuda_amd.fp8 import CODES, LinearFp8
+    from addernetcuda_amd.linear import LinearAct
+    made = LinearFp8.of(LinearAct(130, 20, act="relu"))
+    x = torch.randn(3, 130)
+    with torch.no_grad():
+        want = made(x)
+    for change in (lambda m: m.bfloat16(), lambda m: m.half(), lambda m: m.double(), lambda m: m.to(torch.bfloat16), lambda m: m.to("cpu"), lambda m: m.float()):
+        change(made)
+        assert made.weight.dtype == CODES and made.weight_scale.dtype == made.bias.dtype == torch.float32
+        with torch.no_grad():
+            assert torch.equal(made(x), want)
+    assert not list(made.parameters()) and set(made.state_dict()) == {"weight", "weight_scale", "bias"}
+    assert LinearFp8(8, 8).to("meta").weight.device.type == "meta"

@@ -168,3 +168,19 @@ def test_refusals(gpu):
         gated_linear(x, w, act="tanh")
     with pytest.raises(ValueError):
         GatedLinear(4, 4, act="tanh")
+
+
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+def test_gradient_against_differences(act, gpu):
+    """The kernels' gradients beside the differences of the formula in 64 bits."""
+    from addernetcuda_amd.gated import gated_linear
+    x, w, b, dy = make(5, 12, 9, torch.float32)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    grads = torch.autograd.grad(gated_linear(*leaves, act), leaves, dy)
+    values = [t.detach().double().cpu() for t in leaves]
+    of = lambda v: float((B.gated_linear(*v, None, act)["y"][0] * dy.double().cpu()).sum())
+    for k, at in ((0, (2, 3)), (1, (4, 5)), (1, (13, 2)), (2, (3,)), (2, (15,))):
+        lo, hi = ([t.clone() for t in values] for _ in range(2))
+        lo[k][at] -= 1e-5
+        hi[k][at] += 1e-5
+        assert abs((of(hi) - of(lo)) / 2e-5 - float(grads[k][at])) < 1e-5 * (1 + abs(float(grads[k][at])))

@@ -162,3 +162,22 @@ def test_refusals(gpu):
         rms_norm_fp8(x.requires_grad_(True))
     with pytest.raises(RuntimeError):
         RMSNorm(25).cuda()(x)
+
+
+def test_gradient_against_differences(gpu):
+    """The kernels' gradients beside the differences of the formula in 64 bits."""
+    from addernetcuda_amd.rms_norm import rms_norm
+    x, w, r, dy, ds = make(4, 30, torch.float32)
+    leaves = [t.requires_grad_(True) for t in (x, w, r)]
+    grads = torch.autograd.grad(rms_norm(*leaves[:2], EPS, residual=r), leaves, (dy, ds))
+    values = [t.detach().double().cpu() for t in leaves]
+
+    def of(v):
+        out = B.rms_norm(*v, None, None, EPS)
+        return float((out["y"][0] * dy.double().cpu()).sum() + (out["sum"][0] * ds.double().cpu()).sum())
+
+    for k, at in ((0, (2, 3)), (0, (0, 29)), (1, (4,)), (2, (3, 7))):
+        lo, hi = ([t.clone() for t in values] for _ in range(2))
+        lo[k][at] -= 1e-5
+        hi[k][at] += 1e-5
+        assert abs((of(hi) - of(lo)) / 2e-5 - float(grads[k][at])) < 1e-5 * (1 + abs(float(grads[k][at])))
