@@ -192,3 +192,18 @@ def test_8_bit_layers_keep_their_types():
             assert torch.equal(made(x), want)
     assert not list(made.parameters()) and set(made.state_dict()) == {"weight", "weight_scale", "bias"}
     assert LinearFp8(8, 8).to("meta").weight.device.type == "meta"
+
+
+def test_gated_sizes_take_their_kernels_and_no_size_another():
+    import random
+    from tests.test_gpu_gated import BF16, F32, KERNELS, gated_kernel
+    for (dtype, *kernel), (rows, k, h) in KERNELS.items():
+        assert gated_kernel(rows, k, h, dtype, kernel[0] == 2) == tuple(kernel), (dtype, kernel)
+    r = random.Random(7)
+    for _ in range(10000):
+        rows, k, h = (int(2 ** r.uniform(0, 15)) for _ in range(3))
+        for dtype in (F32, BF16):
+            for aligned in (False, True):
+                for outputs in (1, 2):
+                    got = gated_kernel(rows, k, h, dtype, aligned, outputs)
+                    assert any(key[:3] == (dtype, *got[:2]) for key in KERNELS), (rows, k, h, got)

@@ -63,19 +63,29 @@ def test_values_outside_a_halfs_range(scale, gpu):
         check(70, 64, 72, torch.bfloat16, act, scale=scale)
 
 
-# (bfloat16, aligned): a size for each shape of the streamed tiles, with one share of k and with more; then the others
-KERNELS = {(torch.bfloat16, 2, 0): (8192, 512, 2048), (torch.bfloat16, 2, 2): (1024, 512, 1024), (torch.bfloat16, 2, 3): (256, 256, 512),
-           (torch.bfloat16, 3, 0): (2001, 255, 1001), (torch.bfloat16, 3, 1): (300, 255, 301), (torch.float32, 3, 0): (2048, 256, 2048), (torch.float32, 3, 1): (700, 256, 700)}
+# Each kernel that the forward's product can take -- type, family (1 for few rows, 2 streamed, 3 staged), shape, with shares of k or without, as
+# adder_gated_kernel numbers them for a call that keeps what the backward needs -- and a size that takes it
+F32, BF16 = DTYPES
+KERNELS = {(F32, 1, 1, False): (7, 130, 70), (F32, 1, 2, False): (19, 133, 40), (F32, 1, 4, False): (40, 40, 70), (F32, 3, 0, False): (194, 16, 12304),
+           (F32, 3, 0, True): (69, 850, 8194), (F32, 3, 1, False): (17, 16, 14), (F32, 3, 1, True): (33, 544, 16), (F32, 3, 2, False): (67, 33, 13218),
+           (F32, 3, 2, True): (68, 715, 4227), (F32, 3, 3, False): (18, 544, 6160), (F32, 3, 3, True): (7, 6681, 516), (BF16, 1, 1, False): (2, 270, 13),
+           (BF16, 1, 2, False): (19, 65, 10), (BF16, 1, 4, False): (33, 65, 9), (BF16, 2, 0, False): (265, 16, 13232), (BF16, 2, 0, True): (17309, 5888, 124),
+           (BF16, 2, 1, False): (132, 16, 11648), (BF16, 2, 1, True): (65, 3320, 4421), (BF16, 2, 2, False): (17384, 16, 132), (BF16, 2, 2, True): (8936, 4600, 38),
+           (BF16, 2, 3, False): (20, 16, 8), (BF16, 2, 3, True): (33, 1104, 9), (BF16, 3, 0, False): (196, 73, 14883), (BF16, 3, 0, True): (65, 4485, 4169),
+           (BF16, 3, 1, False): (20, 14, 17), (BF16, 3, 1, True): (33, 1027, 14)}
+
+
+def gated_kernel(rows, k, h, dtype, aligned, outputs=2):
+    import ctypes
+    from addernetcuda_amd._lib import lib
+    got = ctypes.c_int()
+    assert lib.adder_gated_kernel(rows, k, h, int(dtype == BF16), int(aligned), outputs, ctypes.byref(got)) == 0
+    return got.value // 10000, got.value // 100 % 100, got.value % 100 > 1
 
 
 @pytest.mark.parametrize("key", KERNELS, ids=str)
 def test_kernels(key, gpu):
-    import ctypes
-    from addernetcuda_amd._lib import lib
-    rows, k, h = KERNELS[key]
-    got = ctypes.c_int()
-    assert lib.adder_gated_kernel(rows, k, h, int(key[0] == torch.bfloat16), int(k % 8 == 0), 2, ctypes.byref(got)) == 0
-    check(rows, k, h, key[0], "silu")
+    check(*KERNELS[key], key[0], "silu")
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
