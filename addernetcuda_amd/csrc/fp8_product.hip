@@ -331,12 +331,13 @@ constexpr Shape kCodesShapes<bf16_t>[] = {
     {64, 64, 2, 0.6f, 0.33f, 1.6f},         //  817
     {256, 256, 1, 2.07f, 2.07f, 5.9f},      // 1864
 };
-// The kernel for few rows likewise: workgroups of 16 columns whose waves take turns along the blocks of k (us each, measured at 4096 x 4096 and
-// 8192 x 8192).  With 33 to 64 rows it was behind the small tiles (64 x 4096 -> 4096 in 16.5 us instead of 11.4).
+// The kernel for few rows likewise: workgroups of 16 columns whose waves take turns along the blocks of k, us each; more rows of x are more to read
+// from the second-level caches (one row, 4096 to 4096, 8192 to 8192 and 8192 to 1024: 6.6, 16.6, 7.9 us, the small tiles 9.9, 18.7, 8.7; sixteen
+// rows 8.3, 25, 12.4 and 10.3, 19.9, 9.2).  With 33 to 64 rows it was behind them (64 x 4096 -> 4096 in 16.5 us instead of 11.4).
 static constexpr long kCodesRowsMost = 32;
 static float codes_rows_us(long M, long N, long K) {
     const float groups = (float)ceil_div_l(N, 16), turns = (float)ceil_div_l(ceil_div_l(K, kCodeBlock), kCodesWaves);
-    return 3.f + ceilf(groups / kCUs) * (0.4f + turns * (M <= 16 ? 1.1f : 1.75f));
+    return 3.f + ceilf(groups / kCUs) * (0.75f + turns * (0.72f + 0.035f * (float)M));
 }
 // The one choice that a launch and the queries make; shape -1: the kernel for few rows
 template <class T>
