@@ -78,8 +78,9 @@ def test_the_script_trains_it_from_a_teacher_and_serves_it(gpu, tmp_path):
     state = torch.load(os.path.join(second, "addernet.pt"), map_location="cpu", weights_only=True)
     assert "over_channels.0.gated.weight" in state and "stem.adder" in state
     again = ["--arch", "gated_mlp", "--eval-only", "--resume", os.path.join(second, "addernet.pt")] + common
-    full, eight = (train.run(train.parse_args(again + extra))[0] for extra in ([], ["--fp8"]))
-    assert eight["test_loss"] == eight["test_loss"] and abs(eight["test_loss"] - full["test_loss"]) < 1
+    full, eight, half = (train.run(train.parse_args(again + extra))[0] for extra in ([], ["--fp8"], ["--fp8", "--bf16-activations"]))
+    for got in (eight, half):
+        assert got["test_loss"] == got["test_loss"] and abs(got["test_loss"] - full["test_loss"]) < 1
     with pytest.raises(ValueError):
         train.run(train.parse_args(["--arch", "token_mlp", "--eval-only", "--fp8"] + common))
     with pytest.raises(ValueError):
