@@ -5,8 +5,8 @@
 // Memory decides: l is read and dl written.  Where there are rows enough a workgroup keeps a row in registers: it reads it once, and
 // writes the gradient for a loss whose own gradient is one on the way; the backward of any other computes it again.  Where rows are few
 // and long several workgroups share one, and the gradient is the backward's.  All sums in a fixed order.
-// 4096 x 32000 in bfloat16, 64 of the teacher's, T = 2: 120 us (4.4 TB/s), of which the teacher's classes are some 8, and 5 each for the rows that
-// count, the mean and the backward that finds nothing to do; 256 x 1000 in float32 6.4 us.
+// 4096 x 32000 in bfloat16, 64 of the teacher's, T = 2: 108 us (4.9 TB/s), and 4 each for the rows that count, the mean and the backward that
+// finds nothing to do; 256 x 1000 in float32 6.2 us.
 #include "blocks.hpp"
 
 #include <type_traits>
@@ -95,6 +95,8 @@ __device__ __forceinline__ float group_sum(float v, float *lds) {
 
 // How the exponentials of l / T and of l come: one of them (the other is not wanted, or T is one), the second as a power of the first (T two or
 // four: a multiplication where an instruction for an exponential takes the time of four), or each by itself.
+// The exponents are of differences from the row's largest, (l - m) / T: l / T - m / T would save an instruction (104 us for 108 at 4096 x 32000)
+// and lose digits, and all of them where a row lies far from zero or is masked by the type's lowest value.
 enum class Both { one, square, fourth, apart };
 __device__ __forceinline__ Both both_of(const DistillArgs &a) {
     if (!wants_q(a) || !wants_o(a) || a.temperature == 1.f) return Both::one;
@@ -102,8 +104,8 @@ __device__ __forceinline__ Both both_of(const DistillArgs &a) {
 }
 __device__ __forceinline__ float scale_q(const DistillArgs &a) { return wants_q(a) ? kLog2e / a.temperature : kLog2e; }
 template <Both B>
-__device__ __forceinline__ void add_exponentials(float v, float k, float km, float m, float &s_q, float &s_o) {   // of (v - m) k ln 2 and v - m; km = k m
-    const float q = __builtin_amdgcn_exp2f(fmaf(v, k, -km)), p = q * q;
+__device__ __forceinline__ void add_exponentials(float v, float k, float m, float &s_q, float &s_o) {   // of (v - m) k ln 2 and v - m
+    const float q = __builtin_amdgcn_exp2f((v - m) * k), p = q * q;
     s_q += q;
     if constexpr (B == Both::square) s_o = fmaf(q, q, s_o);
     if constexpr (B == Both::fourth) s_o = fmaf(p, p, s_o);
@@ -140,7 +142,7 @@ __device__ __forceinline__ float chunks_max(const uint4 (&u)[C]) {
 // A thread's sums of the exponentials behind m
 template <class T, int C>
 __device__ __forceinline__ void chunks_sums(const DistillArgs &a, const uint4 (&u)[C], float m, float &s_o, float &s_q) {
-    const float k = scale_q(a), km = k * m;
+    const float k = scale_q(a);
     float o = 0.f, q = 0.f;
     by_mode(both_of(a), [&](auto mode) {
         constexpr Both B = decltype(mode)::value;
@@ -149,7 +151,7 @@ __device__ __forceinline__ void chunks_sums(const DistillArgs &a, const uint4 (&
             float v[Chunk<T>::n];
             unpack(u[c], v);
 #pragma unroll
-            for (int e = 0; e < Chunk<T>::n; ++e) add_exponentials<B>(v[e], k, km, m, q, o);
+            for (int e = 0; e < Chunk<T>::n; ++e) add_exponentials<B>(v[e], k, m, q, o);
             __builtin_amdgcn_sched_barrier(0);   // (one chunk's values at a time)
         }
         if constexpr (B == Both::one) o = q;
@@ -202,7 +204,7 @@ __device__ __forceinline__ void teacher(const DistillArgs &a, long row, const Sp
         for (int j = lane; j < a.K; j += 64) {
             const float t = sp.off[j];
             m = fmaxf(m, t);
-            bad = bad || sp.idx[j] < 0 || t != t;
+            bad = bad || (sp.idx[j] < 0 && t > -__builtin_inff()) || t != t;   // (one of -infinity may name any class)
         }
         m = lanes_max<64>(m);
         const bool taught = m > -__builtin_inff();
@@ -231,16 +233,16 @@ __device__ __forceinline__ float row_loss(const DistillArgs &a, const Sparse &sp
 }
 
 // The dense part of a row's gradient: q and o are the exponentials behind m, times these
-struct Dense { float m, k, km, by_q, by_o; };
+struct Dense { float m, k, by_q, by_o; };
 __device__ __forceinline__ Dense dense_of(const DistillArgs &a, const RowStats &r, float up) {
     const float k = scale_q(a);
-    Dense d{r.m, k, k * r.m, r.by_q != 0.f ? r.by_q * up * expf(-r.log_q) : 0.f, r.by_o != 0.f ? r.by_o * up * expf(-r.log_o) : 0.f};
+    Dense d{r.m, k, r.by_q != 0.f ? r.by_q * up * expf(-r.log_q) : 0.f, r.by_o != 0.f ? r.by_o * up * expf(-r.log_o) : 0.f};
     if (both_of(a) == Both::one) d.by_q += d.by_o;
     return d;
 }
 template <Both B>
 __device__ __forceinline__ float gradient(float l, const Dense &d) {
-    const float q = __builtin_amdgcn_exp2f(fmaf(l, d.k, -d.km));
+    const float q = __builtin_amdgcn_exp2f((l - d.m) * d.k);
     if constexpr (B == Both::one) return d.by_q * q;
     else if constexpr (B == Both::square) return q * fmaf(d.by_o, q, d.by_q);
     else if constexpr (B == Both::fourth) return q * fmaf(d.by_o, q * q * q, d.by_q);

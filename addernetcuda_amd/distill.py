@@ -28,7 +28,7 @@ def _torch_distillation_loss(logits, top_logits, top_classes, labels, temperatur
     keep = torch.ones(logits.shape[0], dtype=torch.bool, device=logits.device) if labels is None else labels != ignore_index
     taught = torch.where((top > -torch.inf).any(1, keepdim=True), top, torch.zeros_like(top))
     log_p = F.log_softmax(taught / temperature, 1)
-    log_q = _at(F.log_softmax(logits / temperature, 1), top_classes)
+    log_q = _at(F.log_softmax(logits / temperature, 1), torch.where(top > -torch.inf, top_classes, 0))
     p = log_p.exp() * (top > -torch.inf)
     rows = temperature ** 2 * torch.where(p > 0, p * (log_p - log_q), torch.zeros_like(p)).sum(1)
     if labels is not None:
@@ -44,7 +44,7 @@ def distillation_loss(logits, top_logits, top_classes, labels=None, temperature=
 
     Rows with the label ``ignore_index`` do not count; where none does the loss is zero.  A top logit of -infinity adds nothing, and a row whose
     top logits all are has no teacher's part.  A class may be among the K twice.  A class that does not exist makes its row's loss and gradient
-    not a number."""
+    not a number (but beside a top logit of -infinity, where any number may stand)."""
     if logits.dim() != 2 or top_logits.dim() != 2 or not logits.shape[1] or not top_logits.shape[1] or top_logits.shape[0] != logits.shape[0]:
         raise RuntimeError(f"logits and top_logits must be matrices of as many rows, got {tuple(logits.shape)} and {tuple(top_logits.shape)}")
     if tuple(top_classes.shape) != tuple(top_logits.shape) or top_classes.dtype != torch.int64:

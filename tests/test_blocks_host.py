@@ -170,6 +170,7 @@ def test_distillation_on_the_cpu():
             assert abs(float(loss.detach() - want["loss"][0])) < 1e-12
             assert torch.allclose(torch.autograd.grad(loss, l)[0], want["grad"][0], atol=1e-12)
     assert float(distillation_loss(l, t, i, torch.full_like(y, -100)).detach()) == 0
+    i[0], i[1, 3] = -1, 99   # (beside -infinity: any number)
     i[5, 2] = 40
     y[6] = -3
     loss = distillation_loss(l, t, i, y, 2.0, 0.5)

@@ -87,6 +87,10 @@ def test_rows_that_leave_nothing(size, gpu):
     assert not g[4].any() and not g[1].any()
     g = check(l, t, i, None)
     assert not g[2].any()
+    from addernetcuda_amd.distill import distillation_loss
+    a, anywhere = l.clone().requires_grad_(True), i.clone()
+    anywhere[0, 3:], anywhere[2] = -1, size[1] + 7   # (beside -infinity)
+    assert torch.equal(torch.autograd.grad(distillation_loss(a, t, anywhere, None, 2.0), a)[0], g)
     everything = torch.full_like(y, -100)
     g = check(l, t, i, everything)
     assert not g.any()
@@ -98,6 +102,31 @@ def test_rows_that_leave_nothing(size, gpu):
     i[6] = torch.arange(8, device="cuda")
     y[6] = 3
     check(l, t, i, y)
+
+
+@pytest.mark.parametrize("T,alpha", [(1.0, 0.5), (2.0, 0.5), (4.0, 0.7), (3.0, 0.5), (2.0, 0.0), (2.0, 1.0)])
+@pytest.mark.parametrize("size", [(6, 300, 8), (3, 20000, 8), (260, 5000, 8)])
+def test_logits_far_from_zero(size, T, alpha, gpu):
+    """A row's logits and its teacher's may all be large: what counts is how far they are from each other."""
+    l, t, i, y = make(*size, torch.float32)
+    for off in (1000.0, -3e4):
+        check(l + off, t - off, i, y, T, alpha)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("T,alpha", [(1.0, 0.5), (2.0, 0.5), (0.5, 0.5), (3.0, 1.0), (2.0, 0.0)])
+@pytest.mark.parametrize("size", [(6, 300, 8), (3, 20000, 8), (260, 2500, 8)])
+def test_rows_masked_by_the_lowest_value(size, T, alpha, dtype, gpu):
+    """Of a row that is masked as a whole every class is as likely; of one that is masked but for a few, those are."""
+    l, t, i, y = make(*size, dtype)
+    lowest = torch.finfo(dtype).min
+    l[0] = t[0] = lowest
+    l[1] = lowest
+    l[2, :9000] = lowest
+    i[1], y[:3] = torch.arange(8, device="cuda"), 4
+    i[2] = size[1] - 1 - torch.arange(8, device="cuda") if size[1] > 9000 else torch.arange(8, device="cuda")
+    y[2] = i[2, 0]
+    check(l, t, i, y, T, alpha)
 
 
 @pytest.mark.parametrize("size", [(6, 300, 8), (3, 20000, 8)])
