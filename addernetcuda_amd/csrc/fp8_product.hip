@@ -61,7 +61,7 @@ __device__ __forceinline__ i32x8 join(const i32x4 &lo, const i32x4 &hi) {
 
 // ---- tiles that stream through LDS ------------------------------------------------------------------------------------------
 // As the bfloat16 products' (linear_stream.hip), a tile's row being a block of 128 bytes.  8192 x 4096 to 4096 and a shortcut 154 us, 1785 TFLOP/s.  What
-// bounds it is the way of the operands out of LDS, 24 reads of 1 KB a wave and block at 16 cycles each, 3072 cycles beside the matrix cores' 2048 (without
+// bounds it is the way of the operands out of LDS, 24 reads of 1 KB a wave and block at 16 cycles each, half as long again as the matrix cores take (without
 // 14 of the 24 it takes 133 us, without the multiply-adds 152, without the loads behind the first 128; further reads ahead, tiles that follow
 // each other in one workgroup, and a higher priority for waves that multiply changed nothing).  With every stage come the scales of the tile's
 // rows and columns, a float each, by one load more a wave.  A lane's 32 codes of a row are its chunks q and q + 4 (q = lane / 16): the
