@@ -17,9 +17,8 @@ import torch.nn.functional as F
 
 from ._lib import nodes, plain_tensors
 from .gated import _TORCH_ACTS
-from .layer_norm import _BELOW_F32
 from .linear import ACTS, TYPES, _torch_linear_act
-from .rms_norm import RMSNorm, _torch_rms_norm
+from .rms_norm import RMSNorm, _eps, _in_autocast, _torch_rms_norm
 
 BLOCK = 128   # ADDER_CODE_BLOCK
 TOP, LEAST = 448.0, 2.0 ** -100
@@ -85,8 +84,8 @@ def values(codes, scale):
 
 def rms_norm_fp8(x, weight=None, eps=1e-6, residual=None):
     """``rms_norm.rms_norm`` with its result as codes: ``(codes, scales)``, or with a residual ``(codes, scales, x + residual)``."""
-    if x.is_cuda and torch.is_autocast_enabled("cuda"):   # (as rms_norm)
-        x, weight, residual = (t.float() if t is not None and t.dtype in _BELOW_F32 else t for t in (x, weight, residual))
+    if x.is_cuda and torch.is_autocast_enabled("cuda"):
+        x, weight, residual = _in_autocast(x, weight, residual)
     if plain_tensors(x, weight, residual) and x.is_cuda and x.dtype in TYPES and x.shape[-1:] != (0,):
         return nodes().rms_norm_fp8(x, weight, eps, residual)
     _no_gradients("rms_norm_fp8", x, weight, residual)
@@ -174,9 +173,8 @@ class RMSNormFp8(nn.Module):
         self.register_buffer("weight", None if norm.weight is None else norm.weight.detach().clone())
 
     def forward(self, x, residual=None):
-        eps = self.eps if self.eps is not None else torch.finfo(x.dtype).eps
         w = self.weight if self.weight is None or x.dtype == torch.bfloat16 else self.weight.to(x.dtype)   # (as RMSNorm: float32 beside bfloat16 too)
-        got = rms_norm_fp8(x, w, eps, residual)
+        got = rms_norm_fp8(x, w, _eps(self.eps, x), residual)
         return got if residual is None else (got[:2], got[2])
 
 

@@ -2,8 +2,8 @@
 the backward, the shortcut's own gradient in one pass over the rows each (csrc/rms_norm.hip).  Arguments, outputs and the autograd node are
 csrc/nodes_blocks.cpp; the same norm with a result of 8-bit codes is ``fp8.rms_norm_fp8``.
 
-float32, or bfloat16 with a bfloat16 or float32 weight; sums and statistics are 32 bits.  Inside ``torch.autocast`` the result is float32, as
-torch's own is.  CPU tensors, other types, tensor subclasses and calls that something records, traces or transforms go through torch's own
+float32, or bfloat16 with a bfloat16 or float32 weight; sums and statistics are 32 bits.  Inside ``torch.autocast`` too the result has the type of
+``x`` (as torch's own), or of its sum with a residual of another type.  CPU tensors, other types, tensor subclasses and calls that something records, traces or transforms go through torch's own
 operators.
 """
 import torch
@@ -11,7 +11,6 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from ._lib import nodes, plain_tensors
-from .layer_norm import _BELOW_F32
 from .linear import TYPES, _plus
 
 
@@ -34,14 +33,29 @@ def _torch_rms_norm(x, weight, eps, residual):
     return y if residual is None else (y, s)
 
 
+def _in_autocast(x, weight, residual):
+    """Inside ``torch.autocast`` types may differ: ``x`` and the residual meet in the wider, a narrower weight beside them."""
+    if residual is not None and residual.dtype != x.dtype and x.is_floating_point() and residual.is_floating_point():
+        wider = torch.promote_types(x.dtype, residual.dtype)
+        x, residual = x.to(wider), residual.to(wider)
+    if weight is not None and x.dtype == torch.float32:
+        weight = weight.float()
+    return x, weight, residual
+
+
 def rms_norm(x, weight=None, eps=1e-6, residual=None):
     """``s / sqrt(mean(s^2) + eps) * weight`` over the last dimension of ``s``, which is ``x`` or, where a ``residual`` is given that broadcasts
     to its shape, ``x + residual``; then the result is the pair of this and ``s``."""
-    if x.is_cuda and torch.is_autocast_enabled("cuda"):   # (torch casts everything below float32 to it)
-        x, weight, residual = (t.float() if t is not None and t.dtype in _BELOW_F32 else t for t in (x, weight, residual))
+    if x.is_cuda and torch.is_autocast_enabled("cuda"):
+        x, weight, residual = _in_autocast(x, weight, residual)
     if plain_tensors(x, weight, residual) and x.is_cuda and x.dtype in TYPES and x.shape[-1:] != (0,):
         return nodes().rms_norm(x, weight, eps, residual)
     return _torch_rms_norm(x, weight, eps, residual)
+
+
+def _eps(eps, x):
+    """A norm's ``eps``; None: of the type that it computes in (as ``nn.RMSNorm``)."""
+    return eps if eps is not None else torch.finfo(torch.float64 if x.dtype == torch.float64 else torch.float32).eps
 
 
 class RMSNorm(nn.RMSNorm):
@@ -56,5 +70,4 @@ class RMSNorm(nn.RMSNorm):
     def forward(self, x, residual=None):
         if tuple(x.shape[-1:]) != tuple(self.normalized_shape):
             raise RuntimeError(f"x has shape {tuple(x.shape)} but the last dimension is to be {self.normalized_shape[0]}")
-        eps = self.eps if self.eps is not None else torch.finfo(x.dtype).eps
-        return rms_norm(x, self.weight, eps, residual)
+        return rms_norm(x, self.weight, _eps(self.eps, x), residual)

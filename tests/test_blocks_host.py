@@ -131,6 +131,8 @@ def test_cpu_tensors_take_torchs_operators(dtype):
     from addernetcuda_amd.fp8 import linear_fp8, quantize, quantize_weight, rms_norm_fp8
     from addernetcuda_amd.gated import GatedLinear
     from addernetcuda_amd.rms_norm import RMSNorm, rms_norm
+    small = torch.randn(5, 200).to(dtype) * 2.0 ** -10
+    assert torch.equal(RMSNorm(200, eps=None, dtype=dtype)(small), torch.nn.RMSNorm(200, eps=None, dtype=dtype)(small))
     g = torch.Generator().manual_seed(1)
     x, r = (torch.randn(6, 200, generator=g).to(dtype) for _ in range(2))
     norm, gated = RMSNorm(200, dtype=dtype), GatedLinear(200, 30, dtype=dtype)

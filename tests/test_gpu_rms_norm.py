@@ -1,6 +1,7 @@
 """``addernetcuda_amd.rms_norm`` and its 8-bit form against the formula in 64 bits, with bounds that follow from the roundings (tests/block_bounds.py)."""
 import pytest
 import torch
+import torch.nn.functional as F
 
 from tests import block_bounds as B
 from tests.layer_bounds import within
@@ -142,11 +143,32 @@ def test_streams_graphs_autocast_and_gradients_of_gradients(gpu):
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(eager, out))
     with torch.autocast("cuda", dtype=torch.bfloat16):
-        assert rms_norm(x, w).dtype == torch.float32
+        assert rms_norm(x, w).dtype == F.rms_norm(x, (512,), w).dtype == torch.bfloat16
+        assert rms_norm(x, w.float()).dtype == rms_norm(x, w).dtype
+        y, s = rms_norm(x, w, residual=r.float())   # (types that meet in the wider)
+        assert torch.equal(s, x.float() + r.float()) and y.dtype == torch.float32
+        assert all(torch.equal(p, q) for p, q in zip((y, s), rms_norm(x.float(), w.float(), residual=r.float())))
     y = rms_norm(a, b)
     g = torch.autograd.grad(y.float().square().sum(), a, create_graph=True)[0]
     with pytest.raises(RuntimeError, match="differentiate twice"):
         g.float().sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_the_module_without_eps(gpu, dtype):
+    """``eps=None`` is nn.RMSNorm's: of the type that the norm computes in.  Values of 2^-10 or so, whose mean square is some eight of it."""
+    from addernetcuda_amd.fp8 import RMSNormFp8, values
+    from addernetcuda_amd.rms_norm import RMSNorm
+    x = (make(16, 256, torch.float32)[0] * 2.0 ** -10).to(dtype)
+    norm = RMSNorm(256, eps=None, device=x.device, dtype=dtype)
+    want = B.rms_norm(x, None, None, None, None, torch.finfo(torch.float32).eps)["y"]
+    half = torch.finfo(dtype).eps / 2   # (float16 goes through torch's operators, which round the root and the product, and the weight's)
+    y = norm(x).detach().double()
+    assert ((y - want[0].to(y.device)).abs() <= (4 * half + 1e-5) * want[0].to(y.device).abs() + 1e-7).all()
+    if dtype != torch.float16:
+        q, scale = RMSNormFp8(norm)(x)
+        v = values(q, scale).double()
+        assert ((v - want[0].to(v.device)).abs() <= want[0].to(v.device).abs() * (2.0 ** -4 + 2 * half + 1e-5) + scale.max() * 2.0 ** -10).all()
 
 
 def test_refusals(gpu):
