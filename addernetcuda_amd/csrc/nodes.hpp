@@ -5,9 +5,11 @@
 #include <ATen/ops/empty.h>
 #include <ATen/ops/zeros.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -94,6 +96,23 @@ inline Rows as_rows(const Tensor &t, int64_t width) {
     Tensor v = t.dim() == 2 && t.size(1) == width ? t : t.reshape({rows, width});   // (two dimensions may also be one row: all of them normalised)
     if ((width > 1 && v.stride(1) != 1) || (rows > 1 && v.stride(0) < width && v.stride(0) != 0)) v = v.contiguous();
     return {v, rows > 1 ? (long)v.stride(0) : (long)width, (long)rows};
+}
+
+// A leaf whose earlier graph still lives keeps the stream that its gradients are added on.  Where that is the default stream, a gradient that is captured on
+// another one would have it wait for the capture, which no capture allows and which ends the process: said here instead, before anything is captured for it.
+inline void refuse_in_capture(const char *what) {
+    const auto node = torch::autograd::get_current_node();
+    if (!node) return;
+    for (const auto &edge : node->next_edges()) {
+        if (!dynamic_cast<torch::autograd::AccumulateGrad *>(edge.function.get())) continue;
+        const auto of = edge.function->stream();
+        if (!of || of->device_type() != c10::kCUDA) continue;
+        const auto own = c10::hip::getDefaultHIPStream(of->device_index()), now = c10::hip::getCurrentHIPStream(of->device_index());
+        if (of->id() != own.id() || now.id() == own.id()) continue;
+        TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None, what,
+                    ": a backward pass cannot be captured while a graph of the same leaves that was made on the default stream lives; drop its tensors first, or make it "
+                    "on the stream of the capture");
+    }
 }
 
 // Gradients that these nodes give have no formula to be differentiated again: whoever tries is told so

@@ -70,6 +70,7 @@ struct RmsNorm : public torch::autograd::Function<RmsNorm> {
         return residual.defined() ? variable_list{n.y, n.sum} : variable_list{n.y};
     }
     static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
+        refuse_in_capture("rms_norm");
         const auto saved = ctx->get_saved_variables();
         const Tensor &s = saved[0], &weight = saved[1], &rstd = saved[2];
         const bool has_w = ctx->saved_data["weight"].toBool(), has_r = ctx->saved_data["residual"].toBool();
@@ -302,6 +303,7 @@ struct GatedLinear : public torch::autograd::Function<GatedLinear> {
         return y;
     }
     static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
+        refuse_in_capture("gated_linear");
         const auto saved = ctx->get_saved_variables();
         const Tensor &dy = grads[0];
         const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1), want_b = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(2);
@@ -397,6 +399,7 @@ struct Distill : public torch::autograd::Function<Distill> {
         return loss;
     }
     static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
+        refuse_in_capture("distillation_loss");
         const auto saved = ctx->get_saved_variables();
         const Tensor &logits = saved[0], &top = saved[1];
         variable_list out(7);

@@ -106,3 +106,39 @@ def test_a_block_in_8_bits(dtype, gpu):
         for a, b in ((got, full(x, added)), (alone, full(x))):
             part = b.float() - (x + added if a is got else x).float()
             assert float((a.float() - b.float()).norm()) < 0.15 * float(part.norm()) + 0.01 * float(b.float().norm())   # (three roundings to an e4m3 of a sixteenth at most)
+
+
+@pytest.mark.parametrize("which", ["rms_norm", "gated_linear", "distillation_loss"])
+def test_a_capture_beside_a_living_graph_of_the_same_leaves_is_refused(which, gpu):
+    """Leaves that a graph of the default stream holds take their gradients there, where no capture may reach; without it they are captured."""
+    from addernetcuda_amd.distill import distillation_loss
+    from addernetcuda_amd.gated import gated_linear
+    from addernetcuda_amd.rms_norm import rms_norm
+    g = torch.Generator().manual_seed(11)
+    x, w = (torch.randn(*s, generator=g).cuda().requires_grad_(True) for s in ((8, 256), (64, 256)))
+    top, classes = torch.randn(8, 4, generator=g).cuda(), torch.randint(256, (8, 4), generator=g).cuda()
+    run = {"rms_norm": lambda: rms_norm(x).sum(), "gated_linear": lambda: gated_linear(x, w).sum(), "distillation_loss": lambda: distillation_loss(x, top, classes)}[which]
+    run().backward()
+    want, x.grad, w.grad = x.grad.clone(), None, None
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    held = run()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        loss = run()
+        with pytest.raises(RuntimeError, match="cannot be captured while"):
+            loss.backward()
+    del held, loss, graph
+    with torch.cuda.stream(side):
+        run().backward()   # (on the way to a capture: nothing that the first pass of a program makes)
+        side.synchronize()
+        x.grad = w.grad = None
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            run().backward()
+    for _ in range(3):
+        x.grad.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(x.grad, want)
