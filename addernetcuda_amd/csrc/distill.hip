@@ -5,7 +5,7 @@
 // Memory decides: l is read and dl written.  Where there are rows enough a workgroup keeps a row in registers: it reads it once, and
 // writes the gradient for a loss whose own gradient is one on the way; the backward of any other computes it again.  Where rows are few
 // and long several workgroups share one, and the gradient is the backward's.  All sums in a fixed order.
-// 4096 x 32000 in bfloat16, 64 of the teacher's, T = 2: 108 us (4.9 TB/s), and 4 each for the rows that count, the mean and the backward that
+// 4096 x 32000 in bfloat16, 64 of the teacher's, T = 2: 108 to 116 us (4.5 to 4.9 TB/s), and 4 each for the rows that count, the mean and the backward that
 // finds nothing to do; 256 x 1000 in float32 6.2 us.
 #include "blocks.hpp"
 
