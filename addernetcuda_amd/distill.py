@@ -16,24 +16,28 @@ from .linear import TYPES
 TOP_MOST = 1024   # ADDER_DISTILL_TOP_MAX
 
 
-def _at(values, classes):
-    """``values`` (rows, classes) at ``classes``; not a number, for the row's gradient too, where a class does not exist."""
-    there = (classes >= 0) & (classes < values.shape[1])
-    return values.gather(1, torch.where(there, classes, 0)) * torch.where(there, 1.0, torch.nan).to(values.dtype)
+def _at(values, classes, exist):
+    """``values`` (rows, classes) at ``classes``; not a number, for the row's gradient too, where one of a row's does not exist."""
+    found = values.gather(1, torch.where(exist, classes, 0))
+    return found * torch.where(exist.all(1, keepdim=True), 1.0, torch.nan).to(values.dtype)
 
 
 def _torch_distillation_loss(logits, top_logits, top_classes, labels, temperature, alpha, ignore_index):
     logits, top = logits.float() if logits.dtype in (torch.bfloat16, torch.float16) else logits, top_logits.detach()
     top = top.to(logits.dtype)
     keep = torch.ones(logits.shape[0], dtype=torch.bool, device=logits.device) if labels is None else labels != ignore_index
-    taught = torch.where((top > -torch.inf).any(1, keepdim=True), top, torch.zeros_like(top))
-    log_p = F.log_softmax(taught / temperature, 1)
-    log_q = _at(F.log_softmax(logits / temperature, 1), torch.where(top > -torch.inf, top_classes, 0))
-    p = log_p.exp() * (top > -torch.inf)
-    rows = temperature ** 2 * torch.where(p > 0, p * (log_p - log_q), torch.zeros_like(p)).sum(1)
+    exists = lambda classes: (classes >= 0) & (classes < logits.shape[1])
+    counts = keep.unsqueeze(1)
+    logits = torch.where(counts, logits, 0.0)   # (whatever a row that does not count holds reaches neither the loss nor a gradient)
+    there = counts & (top != -torch.inf)        # (one that is no number is)
+    top = torch.where(there.any(1, keepdim=True), torch.where(counts, top, 0.0), 0.0)
+    log_p = F.log_softmax(top / temperature, 1)
+    p = torch.where(there, log_p.exp(), 0.0)
+    log_q = _at(F.log_softmax(logits / temperature, 1), torch.where(there, top_classes, 0), exists(top_classes) | ~there)
+    rows = temperature ** 2 * torch.where(p == 0, torch.zeros_like(p), p * (log_p - log_q)).sum(1)
     if labels is not None:
-        of = torch.where(keep, labels, torch.zeros_like(labels))
-        hard = -_at(F.log_softmax(logits, 1), of.unsqueeze(1)).squeeze(1)
+        of = torch.where(keep, labels, torch.zeros_like(labels)).unsqueeze(1)
+        hard = -_at(F.log_softmax(logits, 1), of, exists(of)).squeeze(1)
         rows = hard if alpha == 0 else rows if alpha == 1 else alpha * rows + (1 - alpha) * hard
     return torch.where(keep, rows, torch.zeros_like(rows)).sum() / keep.sum().clamp(min=1)
 
