@@ -1,7 +1,7 @@
 // Gated linear layer: g = x wg' + bg, u = x wu' + bu, y = act(g) u (linear*.hip); here what its backward takes from g and u,
 //     dg = dy u act'(g),   du = dy act(g),
 // as one matrix of rows [dg du], for the two products gx = [dg du] w and gw = [dg du]' x, and the bias's gradient, its column sums.
-// Memory decides: dy, g and u are read and dg and du written, 8192 x 4096 in bfloat16 with a SiLU 55 us (6.1 TB/s).  bfloat16: g and u are what the forward kept of them (keep_pair), dz is
+// Memory decides: dy, g and u are read and dg and du written, 8192 x 4096 in bfloat16 with a SiLU 55 us (6.1 TB/s).  bfloat16: g and u are what the forward kept of them (keep_group), dz is
 // rounded to the type of the products' operands, and the bias's sums are not.
 #include "blocks.hpp"
 

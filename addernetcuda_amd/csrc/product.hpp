@@ -104,17 +104,21 @@ __device__ __forceinline__ void both(float z, Act act, float &value, float &slop
 }
 
 // What a gated layer's forward keeps of its two sums, g and u.  Unlike the z above they are factors of the gradients, so their range counts as
-// much as their digits.  In bfloat16 four neighbouring columns (from a multiple of four on) are four IEEE halves of 11 bits where the largest
-// magnitude among them is from 2^-12 to 65504 -- what is left out of a smaller one is then at most 2^-13 of the largest -- and else four bfloat16.
-// To nearest, unlike z above: rounded toward zero, all factors would be too small together.
-// The lowest bit of the first says which (one: halves): gradients are 0.0024 from float64 with it, 0.0029 from bfloat16 alone.  A ReLU's g is
-// always bfloat16: its derivative hangs on the sign of the smallest numbers.
+// much as their digits.  In bfloat16 four neighbouring columns (from a multiple of four on) are four IEEE halves of 11 bits where all of them are
+// such numbers, from 2^-14 to 65504, and else four bfloat16: one that is far smaller than its neighbours, or zero, stays what it is.  The lowest bit
+// of the first says which (one: halves): gradients are 0.0024 from float64 with it, 0.0029 from bfloat16 alone.  The first is rounded to the
+// nearest of the numbers that have this bit, the others to the nearest of all: rounded toward zero, all factors would be too small together.
+// A ReLU's g is always bfloat16: its derivative hangs on the sign of the smallest numbers.
 __device__ __forceinline__ uint2 keep_group(const float (&z)[4], bool halves = true) {
     const float top = fmaxf(fmaxf(fabsf(z[0]), fabsf(z[1])), fmaxf(fabsf(z[2]), fabsf(z[3])));
-    const bool half = halves && top >= 0x1p-12f && top <= 65504.f;
+    const float least = fminf(fminf(fabsf(z[0]), fabsf(z[1])), fminf(fabsf(z[2]), fabsf(z[3])));
+    const bool half = halves && least >= 0x1p-14f && top <= 65504.f;
     typedef _Float16 pair __attribute__((ext_vector_type(2)));
-    const uint32_t lo = __builtin_bit_cast(uint32_t, pair{(_Float16)z[0], (_Float16)z[1]}) | 1u, hi = __builtin_bit_cast(uint32_t, pair{(_Float16)z[2], (_Float16)z[3]});
-    const uint32_t blo = pack_bf16(z[0], z[1]) & ~1u, bhi = pack_bf16(z[2], z[3]);
+    const uint32_t first = __float_as_uint(z[0]);
+    const float cut = __uint_as_float(first & 0xffffe000u);   // (toward zero to a half, whose last bit then is set: the nearest that has it)
+    const uint32_t lo = __builtin_bit_cast(uint32_t, pair{(_Float16)cut, (_Float16)z[1]}) | 1u, hi = __builtin_bit_cast(uint32_t, pair{(_Float16)z[2], (_Float16)z[3]});
+    const uint32_t even = z[0] == z[0] ? (first + 0xffffu + (first >> 17 & 1u)) >> 16 & 0xfffeu : 0x7fc0u;   // (to nearest, on the grid of every other bfloat16)
+    const uint32_t blo = (pack_bf16(z[0], z[1]) & 0xffff0000u) | even, bhi = pack_bf16(z[2], z[3]);
     return make_uint2(half ? lo : blo, half ? hi : bhi);
 }
 __device__ __forceinline__ void unpack_kept(const uint4 &u, float (&v)[4]) { unpack(u, v); }
