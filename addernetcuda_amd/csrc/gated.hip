@@ -1,7 +1,7 @@
 // Gated linear layer: g = x wg' + bg, u = x wu' + bu, y = act(g) u (linear*.hip); here what its backward takes from g and u,
 //     dg = dy u act'(g),   du = dy act(g),
 // as one matrix of rows [dg du], for the two products gx = [dg du] w and gw = [dg du]' x, and the bias's gradient, its column sums.
-// Memory decides: dy, g and u are read and dg and du written, 8192 x 4096 in bfloat16 with a SiLU 55 us (6.1 TB/s).  bfloat16: g and u are what the forward kept of them (keep_group), dz is
+// Memory decides: dy, g and u are read and dg and du written, 8192 x 4096 in bfloat16 with a SiLU 55 us (6.1 TB/s).  bfloat16: g and u are what the forward kept of them (keep_gate, keep_group), dz is
 // rounded to the type of the products' operands, and the bias's sums are not.
 #include "blocks.hpp"
 
@@ -23,7 +23,9 @@ __global__ __launch_bounds__(kGatedThreads) void gated_bwd_kernel(const T *__res
     for (long m = (long)blockIdx.y * 4 + wave; m < rows; m += (long)gridDim.y * 4) {
         float d[V], g[V], u[V];
         load_part(dy + m * dy_stride + n, left, d);
-        unpack_kept(load_raw_part(z + m * 2 * N + n, left), g);
+        const uint4 gate = load_raw_part(z + m * 2 * N + n, left);
+        if constexpr (ACT == Act::relu) unpack(gate, g);
+        else unpack_kept(gate, g);
         unpack_kept(load_raw_part(z + m * 2 * N + N + n, left), u);
 #pragma unroll
         for (int e = 0; e < V; ++e) {

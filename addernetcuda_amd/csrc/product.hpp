@@ -108,11 +108,11 @@ __device__ __forceinline__ void both(float z, Act act, float &value, float &slop
 // such numbers, from 2^-14 to 65504, and else four bfloat16: one that is far smaller than its neighbours, or zero, stays what it is.  The lowest bit
 // of the first says which (one: halves): gradients are 0.0024 from float64 with it, 0.0029 from bfloat16 alone.  The first is rounded to the
 // nearest of the numbers that have this bit, the others to the nearest of all: rounded toward zero, all factors would be too small together.
-// A ReLU's g is always bfloat16: its derivative hangs on the sign of the smallest numbers.
-__device__ __forceinline__ uint2 keep_group(const float (&z)[4], bool halves = true) {
+// A ReLU's g is always four whole bfloat16, with nothing in their place: its derivative hangs on the sign of the smallest numbers (keep_gate).
+__device__ __forceinline__ uint2 keep_group(const float (&z)[4]) {
     const float top = fmaxf(fmaxf(fabsf(z[0]), fabsf(z[1])), fmaxf(fabsf(z[2]), fabsf(z[3])));
     const float least = fminf(fminf(fabsf(z[0]), fabsf(z[1])), fminf(fabsf(z[2]), fabsf(z[3])));
-    const bool half = halves && least >= 0x1p-14f && top <= 65504.f;
+    const bool half = least >= 0x1p-14f && top <= 65504.f;
     typedef _Float16 pair __attribute__((ext_vector_type(2)));
     const uint32_t first = __float_as_uint(z[0]);
     const float cut = __uint_as_float(first & 0xffffe000u);   // (toward zero to a half, whose last bit then is set: the nearest that has it)
@@ -120,6 +120,9 @@ __device__ __forceinline__ uint2 keep_group(const float (&z)[4], bool halves = t
     const uint32_t even = z[0] == z[0] ? (first + 0xffffu + (first >> 17 & 1u)) >> 16 & 0xfffeu : 0x7fc0u;   // (to nearest, on the grid of every other bfloat16)
     const uint32_t blo = (pack_bf16(z[0], z[1]) & 0xffff0000u) | even, bhi = pack_bf16(z[2], z[3]);
     return make_uint2(half ? lo : blo, half ? hi : bhi);
+}
+__device__ __forceinline__ uint2 keep_gate(const float (&z)[4], Act act) {
+    return act == Act::relu ? make_uint2(pack_bf16(z[0], z[1]), pack_bf16(z[2], z[3])) : keep_group(z);
 }
 __device__ __forceinline__ void unpack_kept(const uint4 &u, float (&v)[4]) { unpack(u, v); }
 __device__ __forceinline__ void unpack_kept(const uint4 &u, float (&v)[8]) {
@@ -321,7 +324,7 @@ __device__ __forceinline__ void finish_gated(const ProductArgs &p, long m, long 
                 ku[e] = u[e];
             }
     } else {
-        const uint2 a = keep_group(g, p.act != Act::relu), b = keep_group(u);
+        const uint2 a = keep_gate(g, p.act), b = keep_group(u);
         const uint32_t w[2][2] = {{a.x, a.y}, {b.x, b.y}};
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -377,7 +380,7 @@ __device__ __forceinline__ void finish_gated_tile(const ProductArgs &p, const f3
                 };
                 write(o, make_uint2(pack_bf16(y[0][0], y[0][1]), pack_bf16(y[0][2], y[0][3])), make_uint2(pack_bf16(y[1][0], y[1][1]), pack_bf16(y[1][2], y[1][3])));
                 if (pre) {
-                    write(k, keep_group(g[0], ACT != Act::relu), keep_group(g[1], ACT != Act::relu));
+                    write(k, keep_gate(g[0], ACT), keep_gate(g[1], ACT));
                     write(k + p.half, keep_group(u[0]), keep_group(u[1]));
                 }
             } else {
@@ -386,7 +389,7 @@ __device__ __forceinline__ void finish_gated_tile(const ProductArgs &p, const f3
                     const auto write = [](T *to, uint2 a) {
                         *reinterpret_cast<u16x4_any *>(to) = u16x4_any{(uint16_t)a.x, (uint16_t)(a.x >> 16), (uint16_t)a.y, (uint16_t)(a.y >> 16)};
                     };
-                    write(k, keep_group(g[0], ACT != Act::relu));
+                    write(k, keep_gate(g[0], ACT));
                     write(k + p.half, keep_group(u[0]));
                 }
             }

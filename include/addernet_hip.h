@@ -608,7 +608,7 @@ ADDER_API int adder_linear_codes_kernel(long rows, int in_features, int out_feat
  * y (rows, hidden).
  *   adder_gated_fwd: pre (nullable): receives what the backward needs of g and u, rows x 2 hidden values of the type's size.  In bfloat16 that is
  *     not g and u themselves but a form of 16 bits of its own: four neighbouring columns with three bits more than bfloat16 where all of them lie
- *     between 2^-14 and 65504, else bfloat16's own range and bits, of which the first of the four has one less.
+ *     between 2^-14 and 65504, else bfloat16's own range and bits, of which the first of the four has one less.  A ReLU's g is bfloat16.
  *   adder_gated_bwd: dg = dy u act'(g), du = dy act(g); gx = [dg du] w, gw = [dg du]' x, gbias the sums of [dg du] over the rows; each nullable.
  *     x is read only for gw, w only for gx.  bfloat16: dg and du are rounded to bfloat16 for the two products, and not for gbias.
  *   adder_gated_kernel: as adder_linear_kernel, of the forward's product. */

@@ -39,6 +39,15 @@ def test_small_values_beside_large_ones(k, h, lo, hi, gpu):
         assert ((got.double() - want).abs() <= ((1 + far) * (1 + V) - 1) * want.abs()).all()
 
 
+@pytest.mark.parametrize("k,h", SIZES)
+def test_a_relus_gate_is_kept_as_it_is(k, h, gpu):
+    """bfloat16 weights are sums that bfloat16 holds: the up half's gradient is the gate's positive part itself."""
+    wg, wu = spread(k, h, -20.0, 4.0, 3), spread(k, h, -3.0, 3.0, 4)
+    gate, up = gradients(wg, wu, "relu")
+    assert torch.equal(up, wg.clamp(min=0))
+    assert torch.equal(gate != 0, (wg > 0) & (wu != 0))
+
+
 def test_first_columns_are_not_all_off_the_same_way(gpu):
     """The last bit of the first of four says how they are kept: over many values that makes them neither smaller nor larger.  A value's error is at
     most a step, 2^-7 of it, evenly on both sides: the mean of n is within 5 of its deviations, 2^-7 / sqrt(n), of zero; one side would be 2^-8."""
