@@ -287,8 +287,8 @@ __device__ __forceinline__ void finish_gated(const ProductArgs &p, long m, long 
     float g[4], u[4], y[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        g[e] = e < cnt ? gate[e] + (bias ? ldf(bias + n + e) : 0.f) : 0.f;
-        u[e] = e < cnt ? up[e] + (bias ? ldf(bias + p.half + n + e) : 0.f) : 0.f;
+        g[e] = e < cnt ? gate[e] + (bias ? ldf(bias + n + e) : 0.f) : g[0];   // (a column that does not exist says nothing of how the group is kept)
+        u[e] = e < cnt ? up[e] + (bias ? ldf(bias + p.half + n + e) : 0.f) : u[0];
     }
     switch (p.act) {   // (outside the loop: one branch for four values)
         case Act::relu:
