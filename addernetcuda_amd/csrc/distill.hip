@@ -17,7 +17,7 @@ static constexpr int kTeacherMost = ADDER_DISTILL_TOP_MAX;
 static constexpr float kLog2e = 1.44269504f;
 // What a row's loss and gradient are made of.  m, top: the largest logit, the teacher's; log_*: logarithms of the sums of exponentials
 // behind them; by_*: factors of q and o in the gradient, zero where that part is not there (no teacher's logit above -infinity, a row that
-// does not count), not a number where a class does not exist.  Behind the last row's: the rows that count, in m.
+// does not count), not a number where a class does not exist or a teacher's logit is +infinity or none.  Behind the last row's: the rows that count, in m.
 struct RowStats { float m, log_o, log_q, top, log_p, by_q, by_o, spare; };
 static_assert(sizeof(RowStats) == kDistillStats * sizeof(float), "a row's statistics");
 
@@ -204,7 +204,7 @@ __device__ __forceinline__ void teacher(const DistillArgs &a, long row, const Sp
         for (int j = lane; j < a.K; j += 64) {
             const float t = sp.off[j];
             m = fmaxf(m, t);
-            bad = bad || (sp.idx[j] < 0 && t > -__builtin_inff()) || t != t;   // (one of -infinity may name any class)
+            bad = bad || (sp.idx[j] < 0 && t > -__builtin_inff()) || !(t < __builtin_inff());   // (one of -infinity may name any class)
         }
         m = lanes_max<64>(m);
         const bool taught = m > -__builtin_inff();

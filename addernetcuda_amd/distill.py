@@ -47,8 +47,8 @@ def distillation_loss(logits, top_logits, top_classes, labels=None, temperature=
     given, ``labels`` (rows; int64); without labels it is the teacher's part alone, whatever ``alpha``.
 
     Rows with the label ``ignore_index`` do not count; where none does the loss is zero.  A top logit of -infinity adds nothing, and a row whose
-    top logits all are has no teacher's part.  A class may be among the K twice.  A class that does not exist makes its row's loss and gradient
-    not a number (but beside a top logit of -infinity, where any number may stand)."""
+    top logits all are has no teacher's part.  A class may be among the K twice.  A class that does not exist (but beside a top logit
+    of -infinity, where any number may stand) makes its row's loss and gradient not a number, and so does a top logit of +infinity or one that is none."""
     if logits.dim() != 2 or top_logits.dim() != 2 or not logits.shape[1] or not top_logits.shape[1] or top_logits.shape[0] != logits.shape[0]:
         raise RuntimeError(f"logits and top_logits must be matrices of as many rows, got {tuple(logits.shape)} and {tuple(top_logits.shape)}")
     if tuple(top_classes.shape) != tuple(top_logits.shape) or top_classes.dtype != torch.int64:

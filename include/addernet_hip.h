@@ -626,7 +626,7 @@ ADDER_API int adder_gated_kernel(long rows, int in_features, int hidden, int typ
  *     row = a T^2 sum_k p_k (log p_k - log q[i_k]) - (1 - a) log o[y],   loss = sum of the rows that count / their number
  * Rows with y == ignore do not count; where none does the loss is zero.  Without labels a is 1.  A teacher's logit of -infinity has p = 0 and adds
  * nothing; where all K are, the row has no teacher's part.  A class may be among the K more than once.  A class that does not exist (but
- * beside a logit of -infinity), or a teacher's logit that is not a number, makes the row's loss and gradient not a number.  K at most ADDER_DISTILL_TOP_MAX.
+ * beside a logit of -infinity), or a teacher's logit that is +infinity or not a number, makes the row's loss and gradient not a number.  K at most ADDER_DISTILL_TOP_MAX.
  *   adder_distill_fwd: stats: ADDER_DISTILL_STATS (rows + 1) floats for the backward.  grad (rows, classes; nullable, and null where
  *     adder_distill_in_rows answers 0): the gradient for a grad_loss of one, written on the way.
  *   adder_distill_bwd: the gradient for grad_loss[0], one float in device memory.  unit: grad already holds the one for a grad_loss of one, and
