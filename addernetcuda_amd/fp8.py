@@ -30,6 +30,11 @@ def _no_gradients(what, *tensors):
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad(), or on detached tensors")
 
 
+def _largest(v, dims):
+    """Of the magnitudes that are numbers."""
+    return torch.where(v.isnan(), 0.0, v.abs()).amax(dims)
+
+
 def _torch_codes(v, largest, spread):
     top = largest.float().clamp(min=LEAST)
     return (v.float() * spread(torch.full_like(top, TOP) / top)).to(CODES), top / TOP   # (a number over a tensor is rounded twice)
@@ -37,7 +42,7 @@ def _torch_codes(v, largest, spread):
 
 def _torch_quantize(x):
     b = F.pad(x, (0, -x.shape[-1] % BLOCK)).unflatten(-1, (-1, BLOCK))
-    q, s = _torch_codes(b, b.abs().amax(-1), lambda t: t.unsqueeze(-1))
+    q, s = _torch_codes(b, _largest(b, -1), lambda t: t.unsqueeze(-1))
     return q.flatten(-2)[..., :x.shape[-1]].contiguous(), s
 
 
@@ -66,7 +71,7 @@ def quantize_weight(weight):
     _no_gradients("quantize_weight", weight)
     n, k = weight.shape
     b = F.pad(weight, (0, -k % BLOCK, 0, -n % BLOCK)).unflatten(0, (-1, BLOCK)).unflatten(2, (-1, BLOCK))
-    q, s = _torch_codes(b, b.abs().amax((1, 3)), lambda t: t[:, None, :, None])
+    q, s = _torch_codes(b, _largest(b, (1, 3)), lambda t: t[:, None, :, None])
     return q.flatten(2).flatten(0, 1)[:n, :k].contiguous(), s
 
 
