@@ -91,6 +91,7 @@ def rms_norm_fp8(x, weight=None, eps=1e-6, residual=None):
     """``rms_norm.rms_norm`` with its result as codes: ``(codes, scales)``, or with a residual ``(codes, scales, x + residual)``."""
     if x.is_cuda and torch.is_autocast_enabled("cuda"):
         x, weight, residual = _in_autocast(x, weight, residual)
+    eps = _eps(eps, x)
     if plain_tensors(x, weight, residual) and x.is_cuda and x.dtype in TYPES and x.shape[-1:] != (0,):
         return nodes().rms_norm_fp8(x, weight, eps, residual)
     _no_gradients("rms_norm_fp8", x, weight, residual)
@@ -179,7 +180,7 @@ class RMSNormFp8(nn.Module):
 
     def forward(self, x, residual=None):
         w = self.weight if self.weight is None or x.dtype == torch.bfloat16 else self.weight.to(x.dtype)   # (as RMSNorm: float32 beside bfloat16 too)
-        got = rms_norm_fp8(x, w, _eps(self.eps, x), residual)
+        got = rms_norm_fp8(x, w, self.eps, residual)
         return got if residual is None else (got[:2], got[2])
 
 

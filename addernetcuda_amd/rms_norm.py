@@ -43,24 +43,26 @@ def _in_autocast(x, weight, residual):
     return x, weight, residual
 
 
+def _eps(eps, x):
+    """A norm's ``eps``; None: of the type that it computes in (as ``F.rms_norm``)."""
+    return eps if eps is not None else torch.finfo(torch.float64 if x.dtype == torch.float64 else torch.float32).eps
+
+
 def rms_norm(x, weight=None, eps=1e-6, residual=None):
     """``s / sqrt(mean(s^2) + eps) * weight`` over the last dimension of ``s``, which is ``x`` or, where a ``residual`` is given that broadcasts
-    to its shape, ``x + residual``; then the result is the pair of this and ``s``."""
+    to its shape, ``x + residual``; then the result is the pair of this and ``s``.  ``eps=None``: the machine epsilon of the type that the norm is
+    computed in, as ``F.rms_norm``'s."""
     if x.is_cuda and torch.is_autocast_enabled("cuda"):
         x, weight, residual = _in_autocast(x, weight, residual)
+    eps = _eps(eps, x)
     if plain_tensors(x, weight, residual) and x.is_cuda and x.dtype in TYPES and x.shape[-1:] != (0,):
         return nodes().rms_norm(x, weight, eps, residual)
     return _torch_rms_norm(x, weight, eps, residual)
 
 
-def _eps(eps, x):
-    """A norm's ``eps``; None: of the type that it computes in (as ``nn.RMSNorm``)."""
-    return eps if eps is not None else torch.finfo(torch.float64 if x.dtype == torch.float64 else torch.float32).eps
-
-
 class RMSNorm(nn.RMSNorm):
-    """``nn.RMSNorm`` over the last dimension (same arguments, parameters and state_dict keys) through the kernels above; in the call, a
-    shortcut that is added first: ``y, s = norm(x, residual=shortcut)``."""
+    """``nn.RMSNorm`` over the last dimension, of ``width`` values (same parameters and state_dict keys; ``eps`` is 1e-6 where ``nn.RMSNorm``'s is
+    None unless it is given), through the kernels above; in the call, a shortcut that is added first: ``y, s = norm(x, residual=shortcut)``."""
 
     def __init__(self, width, eps=1e-6, elementwise_affine=True, device=None, dtype=None):
         super().__init__(width, eps=eps, elementwise_affine=elementwise_affine, device=device, dtype=dtype)
@@ -70,4 +72,4 @@ class RMSNorm(nn.RMSNorm):
     def forward(self, x, residual=None):
         if tuple(x.shape[-1:]) != tuple(self.normalized_shape):
             raise RuntimeError(f"x has shape {tuple(x.shape)} but the last dimension is to be {self.normalized_shape[0]}")
-        return rms_norm(x, self.weight, _eps(self.eps, x), residual)
+        return rms_norm(x, self.weight, self.eps, residual)
