@@ -163,8 +163,9 @@ class LinearFp8(nn.Module):
         else:
             codes, scale = quantize(x, self.gate)
             dtype = x.dtype if residual is None else residual.dtype
-        bias = None if self.bias is None else self.bias.to(dtype)
-        return linear_fp8(codes, scale, self.weight, self.weight_scale, bias, residual, self.act, dtype)
+        made = dtype if dtype in TYPES else torch.float32   # (the product has no others)
+        bias = None if self.bias is None else self.bias.to(made)
+        return linear_fp8(codes, scale, self.weight, self.weight_scale, bias, None if residual is None else residual.to(made), self.act, made).to(dtype)
 
     def extra_repr(self):
         return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}, act={self.act}, gate={self.gate}"

@@ -25,3 +25,20 @@ def test_what_is_no_number_stays_alone_in_its_block(dtype):
     assert torch.equal(quantize(torch.full((2, 128), float("nan"), dtype=dtype))[1], torch.full((2, 1), 2.0 ** -100) / 448)
     z = torch.cat([x, torch.ones_like(x)], 1)
     assert torch.equal(torch.isnan(values(*quantize(z, gate="none"))), torch.isnan(values(*quantize(x))))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float64])
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_layers_answer_in_the_type_of_their_input(dtype, device):
+    """Types that the products do not have: the float32 result, rounded once (float64: as it is)."""
+    from addernetcuda_amd.fp8 import LinearFp8, quantize
+    g = torch.Generator().manual_seed(4)
+    layer = torch.nn.Linear(130, 20)
+    x, r = torch.randn(3, 130, generator=g).to(dtype).to(device), torch.randn(3, 20, generator=g).to(dtype).to(device)
+    made = LinearFp8.of(layer).to(device)
+    gated = LinearFp8.of(torch.nn.Linear(65, 20), gate="silu").to(device)
+    with torch.no_grad():
+        assert torch.equal(made(x), made(x.float()).to(dtype)) and made(x).dtype == dtype
+        for y in (made(x, residual=r), made(quantize(x), residual=r)):
+            assert y.dtype == dtype and torch.equal(y, made(x.float(), residual=r.float()).to(dtype))
+        assert gated(x).dtype == dtype
