@@ -5,7 +5,7 @@ and of 128 x 128 values of a weight.  A code stands for ``code * scale``; a bloc
     codes, scales, s = rms_norm_fp8(x, w, residual=r)  # of the RMS norm of s = x + r
     w8, w8_scales = quantize_weight(weight)
     y = linear_fp8(codes, scales, w8, w8_scales, bias, residual=r)
-    serve_fp8(net)                                     # linear layers of a network, in place
+    serve_fp8(net)                                     # the gated blocks of a network (models.GatedMLP), in place
 
 The product is csrc/fp8_product.hip (the 8-bit matrix instructions; block sums are scaled and added up in 32 bits), the codes csrc/fp8.hip and
 csrc/rms_norm.hip.  There are no gradients through codes: a call that would need one raises.  float32 and bfloat16 values; CPU tensors, other
@@ -16,7 +16,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from ._lib import nodes, plain_tensors
-from .gated import _TORCH_ACTS
+from .gated import _TORCH_ACTS, GatedLinear
 from .linear import ACTS, TYPES, _torch_linear_act
 from .rms_norm import RMSNorm, _eps, _in_autocast, _torch_rms_norm
 
@@ -147,10 +147,16 @@ class LinearFp8(nn.Module):
         return super()._apply(moved, recurse)
 
     @classmethod
-    @torch.no_grad()
     def of(cls, layer, gate=None):
         """From an ``nn.Linear`` or ``LinearAct`` (its activation is kept)."""
-        made = cls(layer.in_features, layer.out_features, layer.bias is not None, getattr(layer, "act", "none"), gate, device=layer.weight.device)
+        if isinstance(layer, GatedLinear):
+            raise ValueError("a gated layer's halves meet where the layer behind it takes its input: serve_fp8 makes both")
+        return cls._holding(layer, getattr(layer, "act", "none"), gate)
+
+    @classmethod
+    @torch.no_grad()
+    def _holding(cls, layer, act, gate=None):
+        made = cls(layer.in_features, layer.out_features, layer.bias is not None, act, gate, device=layer.weight.device)
         made.weight, made.weight_scale = quantize_weight(layer.weight.detach())
         if layer.bias is not None:
             made.bias = layer.bias.detach().float().clone()
@@ -194,6 +200,6 @@ def serve_fp8(net):
         raise ValueError("serve_fp8: no gated block in this network")
     for block in blocks:
         gate = block.gated.act
-        block.norm, block.gated, block.down = RMSNormFp8(block.norm), LinearFp8.of(block.gated), LinearFp8.of(block.down, gate=gate)
-        block.gated.act = "none"   # (both halves' sums: the gate is applied where they become codes)
+        # (the first product gives both halves' sums: the gate is applied where they become codes)
+        block.norm, block.gated, block.down = RMSNormFp8(block.norm), LinearFp8._holding(block.gated, "none"), LinearFp8.of(block.down, gate=gate)
     return net

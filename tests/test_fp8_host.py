@@ -42,3 +42,21 @@ def test_layers_answer_in_the_type_of_their_input(dtype, device):
         for y in (made(x, residual=r), made(quantize(x), residual=r)):
             assert y.dtype == dtype and torch.equal(y, made(x.float(), residual=r.float()).to(dtype))
         assert gated(x).dtype == dtype
+
+
+def test_a_gated_layer_by_itself_is_refused():
+    """Its halves meet in the layer behind it: ``of`` would give both, activated, side by side."""
+    from addernetcuda_amd.fp8 import LinearFp8, RMSNormFp8, serve_fp8
+    from addernetcuda_amd.gated import GatedLinear
+    from addernetcuda_amd.models import GatedMLP
+    with pytest.raises(ValueError, match="gated"):
+        LinearFp8.of(GatedLinear(256, 128))
+    block = torch.nn.Sequential(GatedMLP(64, 40, act="gelu"))
+    weight = block[0].gated.weight.detach().clone()
+    serve_fp8(block)
+    assert isinstance(block[0].norm, RMSNormFp8) and block[0].gated.act == "none" and block[0].down.gate == "gelu"
+    assert block[0].gated.weight.shape == weight.shape == (80, 64)
+    with torch.no_grad():
+        assert block(torch.randn(5, 64)).shape == (5, 64)
+    with pytest.raises(ValueError):
+        serve_fp8(block)
