@@ -52,6 +52,7 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
         return y;
     }
     static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
+        refuse_in_capture("linear_act");
         const auto saved = ctx->get_saved_variables();
         const Tensor &dy = grads[0];
         const bool bias = ctx->saved_data["bias"].toBool(), want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
@@ -154,6 +155,7 @@ struct LayerNorm : public torch::autograd::Function<LayerNorm> {
         return y;
     }
     static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
+        refuse_in_capture("layer_norm");
         const auto saved = ctx->get_saved_variables();
         const Tensor &dy = grads[0], &x = saved[0], &weight = saved[1], &bias = saved[2];
         const bool want_x = ctx->needs_input_grad(0), want_w = weight.defined() && ctx->needs_input_grad(1);
@@ -406,6 +408,23 @@ PyObject *py_adamw_step(PyObject *, PyObject *const *args, Py_ssize_t count) {
     END_HANDLE_TH_ERRORS
 }
 
+// leaves_below(y): the leaves that a backward pass comes to from y on, where a node of this module asks for them.  Host code, for tests.
+PyObject *py_leaves_below(PyObject *, PyObject *o) {
+    HANDLE_TH_ERRORS
+    const Tensor y = optional_tensor(o, "y");
+    std::vector<Tensor> leaves;
+    if (y.defined() && y.grad_fn())
+        any_leaf(y.grad_fn().get(), [&](torch::autograd::AccumulateGrad &leaf) {
+            leaves.push_back(leaf.variable);
+            return false;
+        });
+    PyObject *list = PyList_New((Py_ssize_t)leaves.size());
+    if (!list) throw python_error();
+    for (size_t i = 0; i < leaves.size(); ++i) PyList_SET_ITEM(list, (Py_ssize_t)i, THPVariable_Wrap(leaves[i]));
+    return list;
+    END_HANDLE_TH_ERRORS
+}
+
 // bind({name: address}): the entry points of the loaded library
 PyObject *py_bind(PyObject *, PyObject *names) {
     HANDLE_TH_ERRORS
@@ -449,6 +468,7 @@ PyObject *py_bind(PyObject *, PyObject *names) {
 
 PyMethodDef own_methods[] = {
     {"bind", py_bind, METH_O, nullptr},
+    {"leaves_below", py_leaves_below, METH_O, nullptr},
     {"linear_act", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(py_linear_act)), METH_FASTCALL, nullptr},
     {"layer_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(py_layer_norm)), METH_FASTCALL, nullptr},
     {"adamw_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(py_adamw_step)), METH_FASTCALL, nullptr},

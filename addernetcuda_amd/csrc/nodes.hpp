@@ -11,9 +11,11 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <string>
+#include <unordered_set>
 #include <vector>
 
 #include "../../include/addernet_hip.h"
@@ -98,21 +100,46 @@ inline Rows as_rows(const Tensor &t, int64_t width) {
     return {v, rows > 1 ? (long)v.stride(0) : (long)width, (long)rows};
 }
 
+// Calls f with the leaves' nodes that a backward pass reaches from `from` on (inside a pass: this one), each once, until it says true
+template <class F>
+bool any_leaf(torch::autograd::Node *from, const F &f) {
+    const auto *runs = torch::autograd::get_current_graph_task_exec_info();   // of a pass for some inputs only: what it runs
+    std::vector<torch::autograd::Node *> open{from};
+    std::unordered_set<torch::autograd::Node *> seen{from};
+    while (!open.empty()) {
+        torch::autograd::Node *node = open.back();
+        open.pop_back();
+        if (auto *leaf = dynamic_cast<torch::autograd::AccumulateGrad *>(node))
+            if (f(*leaf)) return true;
+        for (const auto &edge : node->next_edges()) {
+            torch::autograd::Node *next = edge.function.get();
+            if (!next || !seen.insert(next).second) continue;
+            if (runs && !runs->empty()) {
+                const auto it = runs->find(next);
+                if (it == runs->end() || !it->second.should_execute()) continue;
+            }
+            open.push_back(next);
+        }
+    }
+    return false;
+}
+
 // A leaf whose earlier graph still lives keeps the stream that its gradients are added on.  Where that is the default stream, a gradient that is captured on
 // another one would have it wait for the capture, which no capture allows and which ends the process: said here instead, before anything is captured for it.
+// All leaves that the pass comes to behind this node are looked at, whatever lies between (a cast, a view, other layers): the first of these nodes speaks for them.
 inline void refuse_in_capture(const char *what) {
     const auto node = torch::autograd::get_current_node();
     if (!node) return;
-    for (const auto &edge : node->next_edges()) {
-        if (!dynamic_cast<torch::autograd::AccumulateGrad *>(edge.function.get())) continue;
-        const auto of = edge.function->stream();
-        if (!of || of->device_type() != c10::kCUDA) continue;
-        const auto own = c10::hip::getDefaultHIPStream(of->device_index()), now = c10::hip::getCurrentHIPStream(of->device_index());
-        if (of->id() != own.id() || now.id() == own.id()) continue;
-        TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None, what,
-                    ": a backward pass cannot be captured while a graph of the same leaves that was made on the default stream lives; drop its tensors first, or make it "
-                    "on the stream of the capture");
-    }
+    const auto now = c10::hip::getCurrentHIPStream();
+    if (now.id() == c10::hip::getDefaultHIPStream(now.device_index()).id()) return;   // (captures nothing)
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    const bool waits = any_leaf(node.get(), [](torch::autograd::AccumulateGrad &leaf) {
+        const auto of = leaf.stream();
+        return of && of->device_type() == c10::kCUDA && of->id() == c10::hip::getDefaultHIPStream(of->device_index()).id();
+    });
+    TORCH_CHECK(!waits, what,
+                ": a backward pass cannot be captured while a graph of the same leaves that was made on the default stream lives; drop its tensors first, or make it "
+                "on the stream of the capture");
 }
 
 // Gradients that these nodes give have no formula to be differentiated again: whoever tries is told so
