@@ -386,13 +386,27 @@ Tensor distill_forward(const Tensor &logits, const Teacher &t, Tensor *stats_out
     return loss;
 }
 
+// The capture that the current stream is in; zero: none
+int64_t capture_here() {
+    const auto now = c10::hip::getCurrentHIPStream();
+    if (now.id() == c10::hip::getDefaultHIPStream(now.device_index()).id()) return 0;   // (captures nothing, and must not be asked while another does)
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    C10_HIP_CHECK(hipStreamGetCaptureInfo(now.stream(), &status, &id));
+    return status == hipStreamCaptureStatusActive ? (int64_t)id : 0;
+}
+
 struct Distill : public torch::autograd::Function<Distill> {
     static Variable forward(AutogradContext *ctx, const Variable &logits, const Tensor &top, const Tensor &classes, const Maybe &labels, double temperature, double alpha,
                             int64_t ignore) {
         Tensor stats, grad;
         const Tensor loss = distill_forward(logits, {top, classes, labels.value_or(Tensor()), (float)temperature, (float)alpha, ignore}, &stats, &grad);
         ctx->save_for_backward({logits, top, classes, labels.value_or(Tensor()), stats});
-        if (grad.defined()) ctx->saved_data["grad"] = grad;   // for a loss whose gradient is one
+        if (grad.defined()) {   // for a loss whose gradient is one
+            const c10::DeviceGuard guard(logits.device());
+            ctx->saved_data["grad"] = grad;
+            ctx->saved_data["capture"] = capture_here();
+        }
         ctx->saved_data["temperature"] = temperature;
         ctx->saved_data["alpha"] = alpha;
         ctx->saved_data["ignore"] = ignore;
@@ -407,9 +421,10 @@ struct Distill : public torch::autograd::Function<Distill> {
         {
             const at::AutoGradMode off(false);
             const c10::DeviceGuard guard(logits.device());
-            // the forward's gradient is handed on, so a second pass over the same graph computes its own
+            // The forward's gradient is handed on, so a second pass over the same graph computes its own; so does one that is replayed without that forward, or
+            // is not replayed with it: what was handed on would hold what the last replay, or its reader, left there.
             const auto ready = ctx->saved_data.find("grad");
-            const bool unit = ready != ctx->saved_data.end();
+            const bool unit = ready != ctx->saved_data.end() && ctx->saved_data["capture"].toInt() == capture_here();
             if (unit) {
                 out[0] = ready->second.toTensor();
                 ctx->saved_data.erase(ready);
