@@ -154,8 +154,8 @@ int adder_linear_codes(const unsigned char *x, long x_row_stride, const float *x
         (residual && bad_stride(residual_row_stride, rows, out_features)))
         return ADDER_ERR_BAD_SHAPE;
     // (a tile's rows lie within 2^32 bytes of each other)
-    if (wide(rows, x_row_stride) || wide(out_features, w_row_stride) || x_row_stride >= (1L << 23) || w_row_stride >= (1L << 23) ||
-        in_features >= (1 << 23) || (residual && wide(rows, residual_row_stride)))
+    if (wide(rows, x_row_stride) || wide(out_features, w_row_stride) || x_row_stride >= ADDER_CODES_STRIDE_MAX ||
+        w_row_stride >= ADDER_CODES_STRIDE_MAX || in_features >= ADDER_CODES_STRIDE_MAX || (residual && wide(rows, residual_row_stride)))
         return ADDER_ERR_TOO_LARGE;
     const auto aligned = [](const void *p, long ld) { return !((reinterpret_cast<uintptr_t>(p) | (uintptr_t)ld) & 15); };
     const size_t need = codes_bytes(rows, in_features, out_features, type, aligned(x, x_row_stride), aligned(w, w_row_stride));

@@ -251,7 +251,9 @@ PyObject *py_linear_fp8(PyObject *, PyObject *const *args, Py_ssize_t count) {
         y = at::empty(shape, x.options().dtype(dtype));
         if (y.numel()) {
             const c10::DeviceGuard guard(x.device());
-            const Rows a = as_rows(x, k), b = as_rows(w, k), r = residual.defined() ? as_rows(residual, n) : Rows{Tensor(), 0, 0};
+            // (rows that the entry point finds too far apart, as the last tokens of long sequences are, are copied)
+            const auto near = [k](Rows t) { return t.stride < ADDER_CODES_STRIDE_MAX ? t : Rows{t.t.contiguous(), (long)k, t.rows}; };
+            const Rows a = near(as_rows(x, k)), b = near(as_rows(w, k)), r = residual.defined() ? as_rows(residual, n) : Rows{Tensor(), 0, 0};
             xs = xs.contiguous();
             ws = ws.contiguous();
             if (bias.defined()) bias = bias.contiguous();

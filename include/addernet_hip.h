@@ -590,11 +590,13 @@ ADDER_API int adder_rms_norm_bwd(const void *dy, long dy_row_stride, const void 
  *     of 2 width values, and act(first half) * second half is what becomes codes.
  *   adder_quantize_weight: codes (rows, width), scales (ceil(rows / ADDER_CODE_BLOCK), ceil(width / ADDER_CODE_BLOCK)).
  *   adder_linear_codes: y = act(x w' + bias) + residual of such codes, x (rows, in_features) with x_scales as adder_quantize gives them, w (out_features,
- *     in_features) with w_scales as adder_quantize_weight does; bias, residual and y of `type`.  Row strides in codes.  Sums in 32 bits.
+ *     in_features) with w_scales as adder_quantize_weight does; bias, residual and y of `type`.  Row strides in codes, below ADDER_CODES_STRIDE_MAX
+ *     as in_features is.  Sums in 32 bits.
  *     The workspace's size depends on whether bases and row strides of x and w are multiples of 16 (the others are copied into it first).
  *   adder_linear_codes_kernel: which kernel it takes: 10000 x (1 for few rows, 2 streamed) + 100 x its shape + the shares of k, as
  *     adder_linear_kernel says. */
 #define ADDER_CODE_BLOCK 128
+#define ADDER_CODES_STRIDE_MAX (1L << 23)
 ADDER_API int adder_quantize(const void *x, long x_row_stride, int act, unsigned char *codes, float *scales, long rows, int width, int type, void *stream);
 ADDER_API int adder_quantize_weight(const void *w, long w_row_stride, unsigned char *codes, float *scales, long rows, int width, int type, void *stream);
 ADDER_API int adder_linear_codes_workspace_bytes(long rows, int in_features, int out_features, int type, int x_aligned, int w_aligned,
