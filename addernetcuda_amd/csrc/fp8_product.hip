@@ -60,10 +60,12 @@ __device__ __forceinline__ i32x8 join(const i32x4 &lo, const i32x4 &hi) {
 }
 
 // ---- tiles that stream through LDS ------------------------------------------------------------------------------------------
-// As the bfloat16 products' (linear_stream.hip), a tile's row being a block of 128 bytes.  8192 x 4096 to 4096 and a shortcut 154 us, 1785 TFLOP/s.  What
-// bounds it is the way of the operands out of LDS, 24 reads of 1 KB a wave and block at 16 cycles each, half as long again as the matrix cores take (without
-// 14 of the 24 it takes 133 us, without the multiply-adds 152, without the loads behind the first 128; further reads ahead, tiles that follow
-// each other in one workgroup, and a higher priority for waves that multiply changed nothing).  With every stage come the scales of the tile's
+// As the bfloat16 products' (linear_stream.hip), a tile's row being a block of 128 bytes.  8192 x 4096 to 4096 and a shortcut 153 us, 1800 TFLOP/s: 64
+// steps of some 2.07 us a compute unit.  Nothing is busy all that time: a step's 24 reads of 1 KB a wave out of LDS alone take 0.35 us (4.6 cycles each), its products alone
+// 1.05 (0.88 on zeros, for which the card keeps its clock), both with the multiply-adds and a barrier 1.33.  The rest is waiting, behind the barrier that all waves
+// leave together, for the next block's loads and, once they are there, for the first operands (without 14 of the 24 reads it takes 133 us, without the
+// multiply-adds 152, without the loads behind the first 128; further reads ahead, tiles that follow each other in one workgroup, and a higher
+// priority for waves that multiply changed nothing).  With every stage come the scales of the tile's
 // rows and columns, a float each, by one load more a wave.  A lane's 32 codes of a row are its chunks q and q + 4 (q = lane / 16): the
 // instruction adds the products of all 128, so any order does that is the same for both operands.
 __device__ __forceinline__ void stream4(const i32x4 &d, unsigned offset, unsigned to) {   // 4 bytes a lane

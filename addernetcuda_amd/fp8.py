@@ -127,7 +127,8 @@ class LinearFp8(nn.Module):
     """A linear layer that serves in 8 bits: ``linear.LinearAct``'s arguments and call.  The weight is held as codes and scales (buffers), rounded once by
     ``LinearFp8.of(layer)``; the input is rounded in the call, or comes as the pair ``(codes, scales)`` that ``quantize`` or ``rms_norm_fp8`` gave.
     ``gate``: an activation; the input has 2 in_features values, and ``act(first half) * second half`` is what the layer takes.  The
-    result has the type of the residual, of the input, or bfloat16 where that comes as codes."""
+    result has the type of the residual, of the input, or bfloat16 where that comes as codes: 2^-8, on the way to the next codes' 2^-4.  Types that the
+    product does not have are rounded from its float32."""
 
     def __init__(self, in_features, out_features, bias=True, act="none", gate=None, device=None):
         for name, value in (("act", act), ("gate", gate)):
