@@ -37,7 +37,8 @@ def _largest(v, dims):
 
 def _torch_codes(v, largest, spread):
     top = largest.float().clamp(min=LEAST)
-    return (v.float() * spread(torch.full_like(top, TOP) / top)).to(CODES), top / TOP   # (a number over a tensor is rounded twice)
+    most = torch.full_like(top, TOP)   # (a number over a tensor is rounded twice, and a tensor on the GPU over a number multiplied by the reciprocal)
+    return (v.float() * spread(most / top)).to(CODES), top / most
 
 
 def _torch_quantize(x):

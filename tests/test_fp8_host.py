@@ -60,3 +60,13 @@ def test_a_gated_layer_by_itself_is_refused():
         assert block(torch.randn(5, 64)).shape == (5, 64)
     with pytest.raises(ValueError):
         serve_fp8(block)
+
+
+@pytest.mark.gpu
+def test_torchs_operators_give_the_kernels_codes_and_scales(gpu):
+    """float64 values that are float32 numbers, which torch's operators take: bit for bit what the kernels make of those."""
+    from addernetcuda_amd.fp8 import quantize, quantize_weight
+    x = (torch.randn(300, 400, generator=torch.Generator().manual_seed(6)) * torch.exp(torch.randn(300, 1, generator=torch.Generator().manual_seed(7)))).cuda()
+    for make in (quantize, quantize_weight):
+        for got, want in zip(make(x.double()), make(x)):
+            assert torch.equal(got.float(), want.float())
