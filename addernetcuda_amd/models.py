@@ -430,7 +430,11 @@ class GatedMLP(nn.Module):
 
     def forward(self, x, added=None):
         if self.fused:
-            y, s = (self.norm(x), x) if added is None else self.norm(added, residual=x)
+            if added is not None and added.shape == x.shape:
+                y, s = self.norm(added, residual=x)
+            else:
+                s = x if added is None else added + x
+                y = self.norm(s)
             return self.down(self.gated(y), residual=s)
         s = x if added is None else added + x
         gate, up = self.gated(self.norm(s)).chunk(2, -1)
